@@ -337,6 +337,81 @@ int triattn_compress_paged(const triattn_paged_layout* layout /* host */, void* 
                            int normalize, int layer_reduce, void* workspace, size_t workspace_bytes,
                            int32_t* keep_out, int keep_pitch, uint32_t* device_status, void* stream);
 
+/*
+ * Attention of the query tokens of a step over ONE layer's paged cache: decode steps and trees of drafted tokens.
+ * Request b owns the query tokens query_start_loc[b] .. query_start_loc[b+1]-1 of q (none: the request is skipped; at most
+ * max_query_len <= 64); their keys and values are already in the cache, in the last slots of the request's
+ * seq_lens[b] tokens.  Query token i sees every earlier token, and drafted token j (0-based, in slot order) of its request
+ * if bit j of tree_mask[query_start_loc[b] + i] is set; tree_mask NULL means a chain (bits 0..i).
+ *   out[n, hq, :] = softmax(scale * q . k) v in bf16 (statistics and sums in fp32);  lse[n, hq]: natural log of the
+ *   sum of exponentials, fp32.  A row that sees nothing gives zeros and -inf.  Rows of q that no request owns are left as
+ *   they are in out and lse.
+ * block_list (may be NULL) [num_reqs, num_kv_heads, num_listed]: distinct logical block indices each KV head reads (in
+ * any order, negative entries are unused); the first min(num_listed, blocks of the request) entries count.
+ * weight_sums (may be NULL) [num_blocks, num_kv_heads, block_size] fp32: every token read receives the sum over the
+ * query rows of its KV head of exp(s - lse); older tokens add it to what is there (or start anew with
+ * reset_weight_sums), the query's own tokens always start anew.
+ * layout: num_reqs, group_size (query heads per KV head), the cache geometry; head_dim 64, 128 or 256; any block size and
+ * strides that are multiples of 8 elements.  k_cache / v_cache: the layer's base pointers (device memory, 16-byte
+ * aligned).  q [num_query_tokens, num_kv_heads * group_size, head_dim] bf16 with the given strides, out likewise, lse contiguous.
+ * No two calls that may overlap share a workspace.  Results do not depend on scheduling: equal calls give equal bits.
+ * Requests with more query tokens than max_query_len or than cached tokens, or more tokens than their block-table row holds, are skipped
+ * (TRIATTN_DEV_BAD_LENGTH); tokens of blocks outside the cache are not read (TRIATTN_DEV_BAD_BLOCK_ID), nor listed
+ * blocks behind the request's end (TRIATTN_DEV_BAD_KEEP_INDEX).  No counterpart in the reference (its engine attends).
+ */
+int triattn_attend_paged(const triattn_paged_layout* layout /* host */, const void* k_cache, const void* v_cache,
+                         const int32_t* block_table, const int32_t* seq_lens, const int32_t* query_start_loc,
+                         const void* q, int64_t q_token_stride, int64_t q_head_stride, int num_query_tokens,
+                         int max_query_len, float scale, const int64_t* tree_mask, const int32_t* block_list,
+                         int num_listed, float* weight_sums, int reset_weight_sums, void* out,
+                         int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
+                         size_t workspace_bytes, uint32_t* device_status, void* stream);
+
+/* Bytes of workspace triattn_attend_paged needs (num_listed 0 without a block list); 0 for an unsupported geometry. */
+size_t triattn_attend_workspace_bytes(const triattn_paged_layout* layout /* host */, int max_query_len, int num_listed);
+
+/*
+ * Eviction by accumulated attention weight: per (layer, request, KV head) keep the keep_counts[b] tokens with the
+ * largest weight_sums, ranking the last `window` tokens and the first prefill_lens[b] (may be NULL) above all others;
+ * ties go to the lowest index, NaN ranks last.  K, V and weight_sums of the kept tokens are compacted in place to the
+ * front of the request's blocks; slots behind them are left as they are.
+ *   weight_sums [num_layers, num_blocks, num_kv_heads, block_size] fp32
+ *   keep_out    [num_layers, num_reqs, num_kv_heads, keep_pitch] int32, ascending, tail filled with -1
+ * Head dimension: any multiple of 8 the compaction takes.  Stands beside triattn_compress_paged, whose scores come
+ * from calibrated statistics (triattention/vllm/runtime/selector_hf.py:749-1033).
+ */
+int triattn_evict_paged(const triattn_paged_layout* layout /* host */, void* const* k_layer_ptrs,
+                        void* const* v_layer_ptrs, float* weight_sums, const int32_t* block_table,
+                        const int32_t* seq_lens, const int32_t* keep_counts, const int32_t* prefill_lens, int window,
+                        int32_t* keep_out, int keep_pitch, uint32_t* device_status, void* stream);
+
+/*
+ * Per-block key bounds for block-sparse attention: for every layer, KV head and block of request b that holds a token
+ * >= first_tokens[b], bounds[l, block, h, 0, :] / [.., 1, :] = smallest / largest key value per channel over the
+ * block's tokens below seq_lens[b] (bf16, exact; NaN propagates).  Other blocks' bounds are left as they are.
+ *   bounds [num_layers, num_blocks, num_kv_heads, 2, head_dim] bf16, 16-byte aligned; head_dim 64, 128 or 256
+ */
+int triattn_update_block_bounds(const triattn_paged_layout* layout /* host */, const void* const* k_layer_ptrs,
+                                const int32_t* block_table, const int32_t* first_tokens, const int32_t* seq_lens,
+                                void* bounds, uint32_t* device_status, void* stream);
+
+/*
+ * The blocks a step reads: per request and KV head the num_selected blocks with the largest upper bound of the
+ * attention logits, summed over the request's query tokens and the heads of the group (ties: lowest index), ascending, tail filled
+ * with -1.  The first sink_blocks, the last recent_blocks and the blocks of the query's own tokens are always taken;
+ * num_selected must hold them.  bounds: ONE layer's [num_blocks, num_kv_heads, 2, head_dim].
+ *   block_list [num_reqs, num_kv_heads, num_selected] int32: the argument of triattn_attend_paged.
+ */
+int triattn_select_blocks(const triattn_paged_layout* layout /* host */, const void* q, int64_t q_token_stride,
+                          int64_t q_head_stride, int num_query_tokens, int max_query_len,
+                          const int32_t* query_start_loc, const void* bounds, const int32_t* block_table,
+                          const int32_t* seq_lens, int num_selected, int sink_blocks, int recent_blocks,
+                          int32_t* block_list, void* workspace, size_t workspace_bytes, uint32_t* device_status,
+                          void* stream);
+
+/* Bytes of workspace triattn_select_blocks needs. */
+size_t triattn_select_blocks_workspace_bytes(const triattn_paged_layout* layout /* host */);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
 from .constants import TRITON_SCORING_REQUIRED_MARKER
@@ -49,6 +49,12 @@ EXPORTED_SYMBOLS = (
     "triattn_compress_paged",
     "triattn_rewrite_block_tables",
     "triattn_apply_effective_overrides",
+    "triattn_attend_workspace_bytes",
+    "triattn_attend_paged",
+    "triattn_evict_paged",
+    "triattn_update_block_bounds",
+    "triattn_select_blocks_workspace_bytes",
+    "triattn_select_blocks",
 )
 
 
@@ -126,6 +132,20 @@ def _declare(lib) -> None:
                                            c_int, c_int, P, c_size_t, P, c_int, P, P]
     lib.triattn_rewrite_block_tables.restype = c_int
     lib.triattn_rewrite_block_tables.argtypes = [P, c_int, c_int, c_int, P, P, P, P, c_int, P, c_int, P, P]
+    lib.triattn_attend_workspace_bytes.restype = c_size_t
+    lib.triattn_attend_workspace_bytes.argtypes = [LP, c_int, c_int]
+    lib.triattn_attend_paged.restype = c_int
+    lib.triattn_attend_paged.argtypes = [LP, P, P, P, P, P, P, c_int64, c_int64, c_int, c_int, c_float, P, P, c_int, P,
+                                         c_int, P, c_int64, c_int64, P, P, c_size_t, P, P]
+    lib.triattn_evict_paged.restype = c_int
+    lib.triattn_evict_paged.argtypes = [LP, P, P, P, P, P, P, P, c_int, P, c_int, P, P]
+    lib.triattn_update_block_bounds.restype = c_int
+    lib.triattn_update_block_bounds.argtypes = [LP, P, P, P, P, P, P, P]
+    lib.triattn_select_blocks_workspace_bytes.restype = c_size_t
+    lib.triattn_select_blocks_workspace_bytes.argtypes = [LP]
+    lib.triattn_select_blocks.restype = c_int
+    lib.triattn_select_blocks.argtypes = [LP, P, c_int64, c_int64, c_int, c_int, P, P, P, P, c_int, c_int, c_int, P, P,
+                                          c_size_t, P, P]
     lib.triattn_apply_effective_overrides.restype = c_int
     lib.triattn_apply_effective_overrides.argtypes = [P, P, c_int, P, P, c_int, P, P, P, c_int, P, c_int, P]
 

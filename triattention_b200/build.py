@@ -16,8 +16,9 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libtriattn_b200.so"
-SOURCES = ["api.cu"]
+SOURCES = ["api.cu", "attend_api.cu"]
 HEADERS = ["common.cuh", "prep.cuh", "score.cuh", "score_fma.cuh", "score_mma.cuh", "score_mma_max.cuh", "score_umma_max.cuh", "finalize.cuh", "select.cuh", "compact.cuh", "reclaim.cuh", "overrides.cuh",
+           "launch.cuh", "attend.cuh", "blocks.cuh", "evict.cuh", "topk_row.cuh",
            "../../include/triattn_b200.h"]
 
 NVCC_FLAGS = [
@@ -25,6 +26,7 @@ NVCC_FLAGS = [
     "-lineinfo", "-O3", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC",
     "-cudart", "shared",
+    "--threads", "0",
 ]
 
 

@@ -14,7 +14,9 @@
 #include "../../include/triattn_b200.h"
 #include "common.cuh"
 #include "compact.cuh"
+#include "evict.cuh"
 #include "finalize.cuh"
+#include "launch.cuh"
 #include "overrides.cuh"
 #include "prep.cuh"
 #include "reclaim.cuh"
@@ -28,54 +30,6 @@
 using namespace triattn;
 
 namespace {
-
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-
-int check_launch() { return cudaGetLastError() == cudaSuccess ? TRIATTN_OK : TRIATTN_ERR_CUDA; }
-
-// Kernel launch, optionally as a programmatic dependent of the preceding kernel in the stream: the launch is
-// processed and its CTAs become resident while that kernel drains (every kernel of this library starts with
-// griddepcontrol.wait, so nothing is read or written before the predecessor has completed).
-template <typename... KArgs, typename... Args>
-int launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) == cudaSuccess ? TRIATTN_OK : TRIATTN_ERR_CUDA;
-}
-
-// Opt a kernel in to `smem` bytes of dynamic shared memory; the attribute call is made only when a device has
-// not yet been raised to that size for this kernel.
-constexpr int kMaxDevicesSmem = 64;
-template <auto Kern>
-bool ensure_dynamic_smem(size_t smem) {
-  static std::atomic<size_t> raised[kMaxDevicesSmem];
-  int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevicesSmem) return false;
-  if (raised[dev].load(std::memory_order_relaxed) >= smem) return true;
-  if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
-  raised[dev].store(smem, std::memory_order_relaxed);
-  return true;
-}
-
-int validate_layout(const triattn_paged_layout* L) {
-  if (L == nullptr) return TRIATTN_ERR_INVALID_ARGUMENT;
-  if (L->num_layers <= 0 || L->num_reqs <= 0 || L->num_kv_heads <= 0 || L->group_size <= 0 || L->head_dim <= 0 ||
-      L->block_size <= 0 || L->num_blocks <= 0 || L->max_blocks_per_req <= 0)
-    return TRIATTN_ERR_INVALID_ARGUMENT;
-  if (L->head_dim % 8 != 0) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
-  if (L->num_reqs > 65535 || L->num_layers > 65535) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
-  if (L->block_stride % 8 != 0 || L->token_stride % 8 != 0 || L->head_stride % 8 != 0) return TRIATTN_ERR_MISALIGNED;
-  return TRIATTN_OK;
-}
 
 // true when the K region of a block is one dense run of bs*Hkv*D elements in NHD or HND order
 bool block_is_dense(const triattn_paged_layout* L) {
@@ -465,6 +419,43 @@ int triattn_compact_paged_preserve(const triattn_paged_layout* layout, void* con
   return compact_common(layout, k_layer_ptrs, v_layer_ptrs, block_table, seq_lens, keep, keep_layer_stride,
                         keep_req_stride, keep_head_stride, keep_counts, scratch, (long long)per_stream,
                         max_dropped_rows, true, device_status, stream);
+}
+
+int triattn_evict_paged(const triattn_paged_layout* layout, void* const* k_layer_ptrs, void* const* v_layer_ptrs,
+                        float* weight_sums, const int32_t* block_table, const int32_t* seq_lens,
+                        const int32_t* keep_counts, const int32_t* prefill_lens, int window, int32_t* keep_out,
+                        int keep_pitch, uint32_t* device_status, void* stream) {
+  int rc = validate_layout(layout);
+  if (rc != TRIATTN_OK) return rc;
+  if (!k_layer_ptrs || !v_layer_ptrs || !weight_sums || !block_table || !seq_lens || !keep_counts || !keep_out)
+    return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (window < 0 || keep_pitch <= 0) return TRIATTN_ERR_INVALID_ARGUMENT;
+  const triattn_paged_layout& Y = *layout;
+  if ((long long)Y.max_blocks_per_req * Y.block_size > (1ll << 30)) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  EvictParams p{};
+  p.sums = weight_sums;
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.keep_counts = keep_counts;
+  p.prefill_lens = prefill_lens;
+  p.keep = keep_out;
+  p.pitch = keep_pitch;
+  p.window = window;
+  p.B = Y.num_reqs;
+  p.Hkv = Y.num_kv_heads;
+  p.bs = Y.block_size;
+  p.num_blocks = Y.num_blocks;
+  p.max_blocks = Y.max_blocks_per_req;
+  p.cap = (int)std::min<long long>((long long)Y.max_blocks_per_req * Y.block_size, kEvictCap);
+  p.status = device_status;
+  const size_t smem = (size_t)p.cap * sizeof(unsigned);
+  if (!ensure_dynamic_smem<evict_select_kernel>(smem)) return TRIATTN_ERR_CUDA;
+  rc = launch_kernel(evict_select_kernel, dim3((unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs, (unsigned)Y.num_layers),
+                     dim3(kEvictThreads), smem, static_cast<cudaStream_t>(stream), true, p);
+  if (rc != TRIATTN_OK) return rc;
+  const int64_t hs = keep_pitch, rs = hs * Y.num_kv_heads, ls = rs * Y.num_reqs;
+  return compact_common(layout, k_layer_ptrs, v_layer_ptrs, block_table, seq_lens, keep_out, ls, rs, hs, keep_counts,
+                        nullptr, 0, 0, false, device_status, stream, true);
 }
 
 int triattn_rewrite_block_tables(int32_t* block_table, int num_reqs, int max_blocks_per_req, int block_size,

@@ -1,0 +1,260 @@
+// C ABI of the operators that attend to the paged cache: attention (with weight sums), block bounds, block choice.
+// No allocation, no synchronisation, no exceptions: every entry returns a triattn_status.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "../../include/triattn_b200.h"
+#include "attend.cuh"
+#include "blocks.cuh"
+#include "common.cuh"
+#include "launch.cuh"
+
+using namespace triattn;
+
+namespace {
+
+// Which attention kernel serves a call, from its geometry alone.
+struct AttendPlan {
+  int rows;      // query rows per row tile
+  int mt;        // 16-row groups of the tile
+  bool split_p;  // at most 8 rows: probabilities in two bf16 parts
+  int grid;
+  size_t part_o, part_ml, bytes;
+};
+
+long long attend_max_tiles(const triattn_paged_layout& Y, int max_q, int num_listed, int tile, int rows) {
+  long long blocks = Y.max_blocks_per_req;
+  if (num_listed > 0) blocks = std::min<long long>(blocks, num_listed);
+  const long long tiles = (blocks * Y.block_size + tile - 1) / tile;
+  const long long row_tiles = ((long long)max_q * Y.group_size + rows - 1) / rows;
+  return tiles * row_tiles * Y.num_kv_heads * Y.num_reqs;
+}
+
+AttendPlan attend_plan(const triattn_paged_layout& Y, int max_q, int num_listed) {
+  AttendPlan a{};
+  const long long R = (long long)max_q * Y.group_size;
+  a.split_p = R <= 8;
+  a.mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  a.rows = a.split_p ? 8 : 16 * a.mt;
+  const int per_sm = Y.head_dim > 128 ? 1 : 2;
+  a.grid = (int)std::min<long long>((long long)kSMs * per_sm, attend_max_tiles(Y, max_q, num_listed, kAttendTile, a.rows));
+  a.part_o = (size_t)2 * a.grid * a.rows * Y.head_dim * sizeof(float);
+  a.part_ml = (size_t)2 * a.grid * a.rows * 2 * sizeof(float);
+  a.bytes = round_up(a.part_o, 256) + round_up(a.part_ml, 256);
+  return a;
+}
+
+int validate_attend(const triattn_paged_layout* Y, int max_q, int num_listed) {
+  const int rc = validate_layout(Y);
+  if (rc != TRIATTN_OK) return rc;
+  if (max_q <= 0 || num_listed < 0) return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (max_q > kAttendMaxQuery || Y->group_size > 64) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  if (Y->head_dim != 64 && Y->head_dim != 128 && Y->head_dim != 256) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  // token positions are 32-bit
+  if ((long long)Y->max_blocks_per_req * Y->block_size > (1ll << 30) || (long long)num_listed * Y->block_size > (1ll << 30))
+    return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  if (Y->num_kv_heads > 65535) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  return TRIATTN_OK;
+}
+
+template <int D>
+int launch_attend(const AttendParams& p, const AttendPlan& a, cudaStream_t st) {
+#define TRIATTN_LAUNCH(MT, SP)                                                                                            \
+  {                                                                                                                       \
+    if (!ensure_dynamic_smem<attend_paged_kernel<D, MT, SP>>(attend_smem_bytes<D, MT>())) return TRIATTN_ERR_CUDA;         \
+    return launch_kernel(attend_paged_kernel<D, MT, SP>, dim3((unsigned)a.grid), dim3(kAttendThreads),                    \
+                         attend_smem_bytes<D, MT>(), st, true, p, a.grid);                                                \
+  }
+  if (a.split_p) TRIATTN_LAUNCH(1, true)
+  if (a.mt == 1) TRIATTN_LAUNCH(1, false)
+  if (a.mt == 2) TRIATTN_LAUNCH(2, false)
+  TRIATTN_LAUNCH(4, false)
+#undef TRIATTN_LAUNCH
+}
+
+template <int D>
+int launch_attend_all(const AttendParams& p, const AttendPlan& a, int max_row_tiles, int observe_grid, cudaStream_t st) {
+  int rc = launch_attend<D>(p, a, st);
+  if (rc != TRIATTN_OK) return rc;
+  rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)max_row_tiles, (unsigned)p.Hkv, (unsigned)p.B),
+                     dim3(kCombineThreads), 0, st, true, p, a.grid, kAttendTile, a.rows);
+  if (rc != TRIATTN_OK || p.sums == nullptr) return rc;
+  if (!ensure_dynamic_smem<attend_observe_kernel<D>>(observe_smem_bytes<D>())) return TRIATTN_ERR_CUDA;
+  return launch_kernel(attend_observe_kernel<D>, dim3((unsigned)observe_grid), dim3(kAttendThreads),
+                       observe_smem_bytes<D>(), st, true, p, observe_grid);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t triattn_attend_workspace_bytes(const triattn_paged_layout* layout, int max_query_len, int num_listed) {
+  if (validate_attend(layout, max_query_len, num_listed) != TRIATTN_OK) return 0;
+  return attend_plan(*layout, max_query_len, num_listed).bytes;
+}
+
+int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache, const void* v_cache,
+                         const int32_t* block_table, const int32_t* seq_lens, const int32_t* query_start_loc,
+                         const void* q, int64_t q_token_stride, int64_t q_head_stride, int num_query_tokens,
+                         int max_query_len, float scale, const int64_t* tree_mask, const int32_t* block_list,
+                         int num_listed, float* weight_sums, int reset_weight_sums, void* out,
+                         int64_t out_token_stride, int64_t out_head_stride, float* lse, void* workspace,
+                         size_t workspace_bytes, uint32_t* device_status, void* stream) {
+  if (block_list == nullptr) num_listed = 0;
+  int rc = validate_attend(layout, max_query_len, num_listed);
+  if (rc != TRIATTN_OK) return rc;
+  if (!k_cache || !v_cache || !block_table || !seq_lens || !query_start_loc || !lse || !workspace)
+    return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (num_query_tokens < 0 || !(scale > 0.f) || !std::isfinite(scale) || (block_list && num_listed <= 0))
+    return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (num_query_tokens == 0) return TRIATTN_OK;
+  if (!q || !out) return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q) || !aligned16(out) || !aligned16(workspace) ||
+      q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8)
+    return TRIATTN_ERR_MISALIGNED;
+  const triattn_paged_layout& Y = *layout;
+  const AttendPlan a = attend_plan(Y, max_query_len, num_listed);
+  if (workspace_bytes < a.bytes) return TRIATTN_ERR_WORKSPACE_TOO_SMALL;
+  AttendParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_ts = q_token_stride;
+  p.q_hs = q_head_stride;
+  p.k = static_cast<const unsigned char*>(k_cache);
+  p.v = static_cast<const unsigned char*>(v_cache);
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.qsl = query_start_loc;
+  p.tree = tree_mask;
+  p.block_list = block_list;
+  p.num_listed = num_listed;
+  p.B = Y.num_reqs;
+  p.Hkv = Y.num_kv_heads;
+  p.g = Y.group_size;
+  p.bs = Y.block_size;
+  p.num_blocks = Y.num_blocks;
+  p.max_blocks = Y.max_blocks_per_req;
+  p.block_stride = Y.block_stride;
+  p.token_stride = Y.token_stride;
+  p.head_stride = Y.head_stride;
+  p.N = num_query_tokens;
+  p.max_q = max_query_len;
+  p.scale_log2 = scale * kLog2e;
+  p.out = static_cast<uint16_t*>(out);
+  p.o_ts = out_token_stride;
+  p.o_hs = out_head_stride;
+  p.lse = lse;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + round_up(a.part_o, 256));
+  p.sums = weight_sums;
+  p.reset_sums = reset_weight_sums ? 1 : 0;
+  p.status = device_status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int row_tiles = (int)(((long long)max_query_len * Y.group_size + a.rows - 1) / a.rows);
+  const int observe_grid = (int)std::min<long long>((long long)kSMs * (Y.head_dim > 128 ? 1 : 2),
+                                                    attend_max_tiles(Y, 1, num_listed, kAttendTile, 64));
+  switch (Y.head_dim) {
+    case 64: return launch_attend_all<64>(p, a, row_tiles, observe_grid, st);
+    case 128: return launch_attend_all<128>(p, a, row_tiles, observe_grid, st);
+    default: return launch_attend_all<256>(p, a, row_tiles, observe_grid, st);
+  }
+}
+
+int triattn_update_block_bounds(const triattn_paged_layout* layout, const void* const* k_layer_ptrs,
+                                const int32_t* block_table, const int32_t* first_tokens, const int32_t* seq_lens,
+                                void* bounds, uint32_t* device_status, void* stream) {
+  const int rc = validate_layout(layout);
+  if (rc != TRIATTN_OK) return rc;
+  if (!k_layer_ptrs || !block_table || !first_tokens || !seq_lens || !bounds) return TRIATTN_ERR_INVALID_ARGUMENT;
+  const triattn_paged_layout& Y = *layout;
+  if (Y.head_dim != 64 && Y.head_dim != 128 && Y.head_dim != 256) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  if ((long long)Y.max_blocks_per_req * Y.block_size > (1ll << 30)) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  if (!aligned16(bounds)) return TRIATTN_ERR_MISALIGNED;
+  BoundsParams p{};
+  p.k_ptrs = k_layer_ptrs;
+  p.bounds = static_cast<uint16_t*>(bounds);
+  p.block_table = block_table;
+  p.first = first_tokens;
+  p.seq_lens = seq_lens;
+  p.B = Y.num_reqs;
+  p.Hkv = Y.num_kv_heads;
+  p.D = Y.head_dim;
+  p.bs = Y.block_size;
+  p.num_blocks = Y.num_blocks;
+  p.max_blocks = Y.max_blocks_per_req;
+  p.block_stride = Y.block_stride;
+  p.token_stride = Y.token_stride;
+  p.head_stride = Y.head_stride;
+  p.status = device_status;
+  const long long pairs = (long long)Y.num_layers * Y.num_reqs;
+  const long long warps = (long long)Y.max_blocks_per_req * Y.num_kv_heads;
+  const long long gx = std::max<long long>(1, std::min((warps + 7) / 8, (kSMs * 16 + pairs - 1) / pairs));
+  return launch_kernel(block_bounds_kernel, dim3((unsigned)gx, (unsigned)Y.num_reqs, (unsigned)Y.num_layers),
+                       dim3(kBoundsThreads), 0, static_cast<cudaStream_t>(stream), true, p);
+}
+
+size_t triattn_select_blocks_workspace_bytes(const triattn_paged_layout* layout) {
+  if (validate_layout(layout) != TRIATTN_OK) return 0;
+  return round_up((size_t)layout->num_reqs * layout->num_kv_heads * layout->max_blocks_per_req * sizeof(float), 256);
+}
+
+int triattn_select_blocks(const triattn_paged_layout* layout, const void* q, int64_t q_token_stride,
+                          int64_t q_head_stride, int num_query_tokens, int max_query_len,
+                          const int32_t* query_start_loc, const void* bounds, const int32_t* block_table,
+                          const int32_t* seq_lens, int num_selected, int sink_blocks, int recent_blocks,
+                          int32_t* block_list, void* workspace, size_t workspace_bytes, uint32_t* device_status,
+                          void* stream) {
+  int rc = validate_attend(layout, max_query_len, 0);
+  if (rc != TRIATTN_OK) return rc;
+  if (!query_start_loc || !bounds || !block_table || !seq_lens || !block_list || !workspace) return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (num_query_tokens < 0 || num_selected <= 0 || sink_blocks < 0 || recent_blocks < 0) return TRIATTN_ERR_INVALID_ARGUMENT;
+  const triattn_paged_layout& Y = *layout;
+  // what is always read has to fit: the sink, the recent blocks and the blocks of the query's own tokens
+  const long long own = (max_query_len + Y.block_size - 2) / Y.block_size + 1;
+  if (num_selected < sink_blocks + std::max<long long>(recent_blocks, own)) return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (num_query_tokens > 0 && !q) return TRIATTN_ERR_INVALID_ARGUMENT;
+  if (!aligned16(bounds) || !aligned16(workspace)) return TRIATTN_ERR_MISALIGNED;
+  if (workspace_bytes < triattn_select_blocks_workspace_bytes(layout)) return TRIATTN_ERR_WORKSPACE_TOO_SMALL;
+  SelectBlocksParams p{};
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_ts = q_token_stride;
+  p.q_hs = q_head_stride;
+  p.qsl = query_start_loc;
+  p.bounds = static_cast<const uint16_t*>(bounds);
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.B = Y.num_reqs;
+  p.Hkv = Y.num_kv_heads;
+  p.g = Y.group_size;
+  p.bs = Y.block_size;
+  p.num_blocks = Y.num_blocks;
+  p.max_blocks = Y.max_blocks_per_req;
+  p.N = num_query_tokens;
+  p.max_q = max_query_len;
+  p.num_selected = num_selected;
+  p.sink = sink_blocks;
+  p.recent = recent_blocks;
+  p.scores = static_cast<float*>(workspace);
+  p.block_list = block_list;
+  p.status = device_status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long rows = (long long)Y.num_reqs * Y.num_kv_heads;
+  const long long gx = std::max<long long>(1, std::min<long long>((Y.max_blocks_per_req + 7) / 8, (kSMs * 8 + rows - 1) / rows));
+  const dim3 grid((unsigned)gx, (unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs);
+  switch (Y.head_dim) {
+    case 64: rc = launch_kernel(block_scores_kernel<64>, grid, dim3(kScoreThreads), 0, st, true, p); break;
+    case 128: rc = launch_kernel(block_scores_kernel<128>, grid, dim3(kScoreThreads), 0, st, true, p); break;
+    default: rc = launch_kernel(block_scores_kernel<256>, grid, dim3(kScoreThreads), 0, st, true, p); break;
+  }
+  if (rc != TRIATTN_OK) return rc;
+  const int cap = (int)std::min<long long>(Y.max_blocks_per_req, 32768);
+  const size_t smem = (size_t)cap * 4;
+  if (!ensure_dynamic_smem<pick_blocks_kernel>(smem)) return TRIATTN_ERR_CUDA;
+  return launch_kernel(pick_blocks_kernel, dim3((unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs), dim3(kPickThreads), smem, st,
+                       true, p, cap);
+}
+
+}  // extern "C"

@@ -1,0 +1,86 @@
+// Eviction by accumulated attention weight: per (layer, request, KV head) row the keep_counts[b] tokens with the
+// largest sums survive; the last `window` tokens and the first prefill_lens[b] are ranked above all others.  The
+// sums live beside the cache, [num_blocks, Hkv, block_size] fp32 per layer, and are compacted with it.
+//
+// One CTA per row.  A row's sums are read once through the block table into shared memory (runs of block_size values),
+// the radix passes and the output pass run from there, and the surviving sums move to their new slots in the output
+// pass: rank r <= index i, and a chunk's values are in registers or shared memory before any slot of it is written.
+#pragma once
+
+#include "common.cuh"
+#include "topk_row.cuh"
+
+namespace triattn {
+
+constexpr int kEvictThreads = 1024;
+constexpr int kEvictCap = 49152;  // keys of a row kept in shared memory (192 KB)
+
+struct EvictParams {
+  float* sums;  // [L, num_blocks, Hkv, bs]
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* keep_counts;
+  const int32_t* prefill_lens;  // or null
+  int32_t* keep;                // [L, B, Hkv, pitch]
+  int pitch, window;
+  int B, Hkv, bs, num_blocks, max_blocks, cap;
+  uint32_t* status;
+};
+
+__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ __align__(16) unsigned char evict_smem[];
+  __shared__ TopkShared<kEvictThreads> sh;
+  grid_dependency_wait();
+  trigger_dependents();
+  const int h = blockIdx.x, b = blockIdx.y, l = blockIdx.z;
+  unsigned err = 0u;
+  int n = p.seq_lens[b];
+  if (n > (long long)p.max_blocks * p.bs) {
+    err |= TRIATTN_DEV_BAD_LENGTH;
+    n = p.max_blocks * p.bs;
+  }
+  n = max(n, 0);
+  const int k = max(0, min(p.keep_counts[b], min(n, p.pitch)));
+  const int guard = p.prefill_lens != nullptr ? p.prefill_lens[b] : 0;
+  const int recent = n - p.window;
+  const int32_t* bt = p.block_table + (long long)b * p.max_blocks;
+  int32_t* out = p.keep + (((long long)l * p.B + b) * p.Hkv + h) * p.pitch;
+  float* sums = p.sums + (long long)l * p.num_blocks * p.Hkv * p.bs;
+  auto slot = [&](int t) -> long long {
+    const int lb = t / p.bs;
+    const int blk = bt[lb];
+    if ((unsigned)blk >= (unsigned)p.num_blocks) {
+      err |= TRIATTN_DEV_BAD_BLOCK_ID;
+      return -1;
+    }
+    return ((long long)blk * p.Hkv + h) * p.bs + (t - lb * p.bs);
+  };
+  for (int i = k + threadIdx.x; i < p.pitch; i += kEvictThreads) out[i] = -1;
+  topk_row<kEvictThreads>(
+      n, k, reinterpret_cast<unsigned*>(evict_smem), p.cap, sh,
+      [&](int i) -> unsigned {
+        if (i >= recent || i < guard) return float_to_ordered(INFINITY);
+        const long long at = slot(i);
+        const float w = at < 0 ? -INFINITY : sums[at];
+        return float_to_ordered(w == w ? w + 0.f : -INFINITY);  // -0 ranks as 0, NaN last
+      },
+      [&](bool sel, int rank, int i) {
+        // all threads of the CTA come here together; the sums of a run of indices are read before any of its
+        // destinations (at or below the run's indices) is written
+        long long from = -1, to = -1;
+        float w = 0.f;
+        if (sel) {
+          out[rank] = i;
+          if (rank != i) {
+            from = slot(i);
+            to = slot(rank);
+            if (from >= 0) w = sums[from];
+          }
+        }
+        __syncthreads();
+        if (from >= 0 && to >= 0) sums[to] = w;
+      });
+  if (err) flag_status(p.status, err);
+}
+
+}  // namespace triattn

@@ -6,7 +6,9 @@ current torch stream and does not synchronise.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -390,3 +392,207 @@ def rewrite_block_tables(block_table: torch.Tensor, blocks_before: torch.Tensor,
         _ptr(block_table), B, width, int(block_size), _ptr(blocks_before), _ptr(lens_after), _ptr(blocks_after),
         _ptr(freed), cap, _ptr(count), int(fill_value), _ptr(status), _stream()), "rewrite_block_tables")
     return blocks_after, freed, count
+
+
+# ------------------------------------------------------------------------------------------ attention over the cache
+_NO_GUARD = contextlib.nullcontext()
+
+
+def _on_device(dev: torch.device):
+    """Makes ``dev`` current for the launches inside (nothing to do when it already is)."""
+    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _expect(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, shape: tuple) -> None:
+    """``t`` is a contiguous ``dtype`` tensor of ``shape`` on ``dev`` (-1: any extent)."""
+    if t.dtype != dtype or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor on {dev}, got {t.dtype} on {t.device}")
+    if t.dim() != len(shape) or any(s not in (-1, d) for s, d in zip(shape, t.shape)):
+        raise ValueError(f"{name} must have shape {list(shape)} (-1: any), got {list(t.shape)}")
+
+
+def _check_queries(q: torch.Tensor, num_kv_heads: int, head_dim: int) -> int:
+    """Query heads per KV head of ``q`` [N, Hq, D]."""
+    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError("q must be a bf16 [N, Hq, D] tensor with a contiguous last axis")
+    if int(q.shape[2]) != head_dim:
+        raise ValueError(f"q has head_dim {int(q.shape[2])}, the cache has {head_dim}")
+    g, rem = divmod(int(q.shape[1]), num_kv_heads)
+    if rem or g <= 0:
+        raise ValueError(f"q has {int(q.shape[1])} heads, not a multiple of the cache's {num_kv_heads} KV heads")
+    return g
+
+
+def attend_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                 query_start_loc: torch.Tensor, max_query_len: int, *, scale: Optional[float] = None,
+                 tree_mask: Optional[torch.Tensor] = None, block_list: Optional[torch.Tensor] = None,
+                 weight_sums: Optional[torch.Tensor] = None, reset_weight_sums: bool = False,
+                 kv_axis: Optional[int] = None, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+                 workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None):
+    """Attention of a step's query tokens over one layer's paged cache (``triattn_attend_paged``); returns ``(out, lse)``.
+
+    ``q`` ``[N, Hq, D]`` bf16, request ``b`` owning rows ``query_start_loc[b] .. query_start_loc[b + 1] - 1`` (at most
+    ``max_query_len`` <= 64); the keys and values of these tokens are already in the cache, in the last slots of the
+    request's ``seq_lens[b]`` tokens.  ``kv_cache`` is the layer's 5-D tensor (see :func:`split_kv_axes`), ``block_table``
+    ``[B, width]`` int32.  Every query token sees all earlier tokens; among the request's own tokens it sees token ``j`` if
+    bit ``j`` of its ``tree_mask`` word (``[N]`` int64) is set, without a mask the tokens up to itself.
+
+    ``block_list`` ``[B, Hkv, S]`` int32 (:func:`select_blocks`) restricts each KV head to the listed blocks.
+    ``weight_sums`` ``[num_blocks, Hkv, block_size]`` fp32 receives, per cached token and KV head, the attention weight the
+    token got from this call's rows: added to what older tokens have (``reset_weight_sums``: starting anew), while the
+    request's own tokens always start anew, whatever their slots held.  ``out`` ``[N, Hq, D]`` bf16, ``lse`` ``[N, Hq]`` fp32
+    (natural log); rows that no request owns are left as they are.  ``workspace``: at least
+    :func:`attend_workspace_bytes` bytes that no overlapping call uses.
+    """
+    lib = _native.load()
+    _require_cuda(q, "q")
+    k, v = split_kv_axes(kv_cache, kv_axis)
+    dev = q.device
+    if k.dtype != torch.bfloat16 or k.device != dev or k.stride(3) != 1:
+        raise ValueError(f"kv_cache must be a bf16 tensor on {dev} with a contiguous head_dim axis")
+    nb, bs, H, D = k.shape
+    g = _check_queries(q, H, D)
+    B = int(seq_lens.shape[0])
+    N = int(q.shape[0])
+    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
+    _expect(block_table, "block_table", torch.int32, dev, (B, -1))
+    _expect(query_start_loc, "query_start_loc", torch.int32, dev, (B + 1,))
+    if B == 0 or int(block_table.shape[1]) == 0:
+        raise ValueError("seq_lens and block_table must not be empty")
+    S = 0
+    if tree_mask is not None:
+        _expect(tree_mask, "tree_mask", torch.int64, dev, (N,))
+    if block_list is not None:
+        _expect(block_list, "block_list", torch.int32, dev, (B, H, -1))
+        S = int(block_list.shape[2])
+        if S == 0:
+            raise ValueError("block_list must not be empty")
+    if weight_sums is not None:
+        _expect(weight_sums, "weight_sums", torch.float32, dev, (nb, H, bs))
+    if status is not None:
+        _expect(status, "status", torch.int32, dev, (-1,))
+    st = k.stride()
+    layout = PagedLayout(1, B, H, g, D, bs, nb, int(block_table.shape[1]), st[0], st[1], st[2], 0, 0)
+    with _on_device(dev):
+        if out is None:
+            out = torch.empty((N, H * g, D), dtype=torch.bfloat16, device=dev)
+        elif out.dtype != torch.bfloat16 or out.device != dev or out.shape != q.shape or out.stride(2) != 1:
+            raise ValueError("out must be a bf16 tensor of q's shape on q's device with a contiguous last axis")
+        if lse is None:
+            lse = torch.empty((N, H * g), dtype=torch.float32, device=dev)
+        else:
+            _expect(lse, "lse", torch.float32, dev, (N, H * g))
+        if workspace is None:
+            workspace = torch.empty(max(lib.triattn_attend_workspace_bytes(ctypes.byref(layout), max_query_len, S), 16),
+                                    dtype=torch.uint8, device=dev)
+        _native.check(lib.triattn_attend_paged(
+            ctypes.byref(layout), k.data_ptr(), v.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+            query_start_loc.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), N, max_query_len,
+            1.0 / math.sqrt(D) if scale is None else scale, _ptr(tree_mask), _ptr(block_list), S, _ptr(weight_sums),
+            1 if reset_weight_sums else 0, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _ptr(status), _stream()), "attend_paged")
+    return out, lse
+
+
+def attend_workspace_bytes(layout: PagedLayout, max_query_len: int, num_listed: int = 0) -> int:
+    """Bytes of workspace :func:`attend_paged` needs (``num_listed`` = entries per row of a ``block_list``)."""
+    return int(_native.load().triattn_attend_workspace_bytes(ctypes.byref(layout), int(max_query_len), int(num_listed)))
+
+
+def evict_paged(view: PagedCacheView, layout: PagedLayout, weight_sums: torch.Tensor, block_table: torch.Tensor,
+                seq_lens: torch.Tensor, keep_counts: torch.Tensor, keep_pitch: int, window: int,
+                prefill_lens: Optional[torch.Tensor] = None, keep_out: Optional[torch.Tensor] = None,
+                status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Keep, per layer, request and KV head, the tokens with the largest attention weight sums (``triattn_evict_paged``).
+
+    ``weight_sums`` ``[L, num_blocks, Hkv, block_size]`` fp32, as :func:`attend_paged` fills it layer by layer.  The last
+    ``window`` tokens and the first ``prefill_lens[b]`` rank above all others.  K, V and the sums are compacted in place;
+    returns keep ``[L, B, Hkv, keep_pitch]`` int32 (ascending, -1 behind ``keep_counts[b]``).
+    """
+    lib = _native.load()
+    _require_cuda(weight_sums, "weight_sums")
+    dev = view.device
+    L, B, H = view.num_layers, layout.num_reqs, view.num_kv_heads
+    _expect(weight_sums, "weight_sums", torch.float32, dev, (L, view.num_blocks, H, view.block_size))
+    _expect(block_table, "block_table", torch.int32, dev, (B, layout.max_blocks_per_req))
+    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
+    _expect(keep_counts, "keep_counts", torch.int32, dev, (B,))
+    if prefill_lens is not None:
+        _expect(prefill_lens, "prefill_lens", torch.int32, dev, (B,))
+    if status is not None:
+        _expect(status, "status", torch.int32, dev, (-1,))
+    with _on_device(dev):
+        if keep_out is None:
+            keep_out = torch.empty((L, B, H, keep_pitch), dtype=torch.int32, device=dev)
+        else:
+            _expect(keep_out, "keep_out", torch.int32, dev, (L, B, H, keep_pitch))
+        _native.check(lib.triattn_evict_paged(
+            ctypes.byref(layout), view.k_ptrs.data_ptr(), view.v_ptrs.data_ptr(), weight_sums.data_ptr(),
+            block_table.data_ptr(), seq_lens.data_ptr(), keep_counts.data_ptr(), _ptr(prefill_lens), int(window),
+            keep_out.data_ptr(), int(keep_pitch), _ptr(status), _stream()), "evict_paged")
+    return keep_out
+
+
+def update_block_bounds(view: PagedCacheView, layout: PagedLayout, bounds: torch.Tensor, block_table: torch.Tensor,
+                        first_tokens: torch.Tensor, seq_lens: torch.Tensor, status: Optional[torch.Tensor] = None) -> None:
+    """Rebuild the key bounds of every block holding tokens ``first_tokens[b] .. seq_lens[b] - 1``
+    (``triattn_update_block_bounds``); ``bounds`` ``[L, num_blocks, Hkv, 2, D]`` bf16 (smallest, largest)."""
+    lib = _native.load()
+    _require_cuda(bounds, "bounds")
+    dev, B = view.device, layout.num_reqs
+    _expect(bounds, "bounds", torch.bfloat16, dev, (view.num_layers, view.num_blocks, view.num_kv_heads, 2, view.head_dim))
+    _expect(block_table, "block_table", torch.int32, dev, (B, layout.max_blocks_per_req))
+    _expect(first_tokens, "first_tokens", torch.int32, dev, (B,))
+    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
+    if status is not None:
+        _expect(status, "status", torch.int32, dev, (-1,))
+    with _on_device(dev):
+        _native.check(lib.triattn_update_block_bounds(
+            ctypes.byref(layout), view.k_ptrs.data_ptr(), block_table.data_ptr(), first_tokens.data_ptr(),
+            seq_lens.data_ptr(), bounds.data_ptr(), _ptr(status), _stream()), "update_block_bounds")
+
+
+def select_blocks(q: torch.Tensor, bounds: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
+                  block_table: torch.Tensor, max_query_len: int, block_size: int, num_selected: int, *,
+                  sink_blocks: int = 1, recent_blocks: int = 2, block_list: Optional[torch.Tensor] = None,
+                  workspace: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The ``num_selected`` blocks per request and KV head with the largest bound of the attention logits, summed over
+    the request's query tokens and the group's heads (``triattn_select_blocks``).
+
+    ``bounds`` ``[num_blocks, Hkv, 2, D]``: one layer of :func:`update_block_bounds`.  The first ``sink_blocks``, the last
+    ``recent_blocks`` and the blocks of the query's own tokens are always among them, so these must fit.  Returns
+    ``[B, Hkv, num_selected]`` int32, ascending, -1 behind the request's last block.
+    """
+    lib = _native.load()
+    _require_cuda(q, "q")
+    dev = q.device
+    _expect(bounds, "bounds", torch.bfloat16, dev, (-1, -1, 2, -1))
+    nb, H, _, D = bounds.shape
+    g = _check_queries(q, H, D)
+    B, width = int(seq_lens.shape[0]), int(block_table.shape[1])
+    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
+    _expect(block_table, "block_table", torch.int32, dev, (B, -1))
+    _expect(query_start_loc, "query_start_loc", torch.int32, dev, (B + 1,))
+    if B == 0 or width == 0:
+        raise ValueError("seq_lens and block_table must not be empty")
+    own = (max_query_len + block_size - 2) // block_size + 1
+    if num_selected < sink_blocks + max(recent_blocks, own):
+        raise ValueError(f"num_selected={num_selected} cannot hold {sink_blocks} sink and {max(recent_blocks, own)} recent blocks")
+    if status is not None:
+        _expect(status, "status", torch.int32, dev, (-1,))
+    # strides play no part in the choice: any that pass the layout check
+    layout = PagedLayout(1, B, H, g, D, block_size, nb, width, block_size * H * D, H * D, D, 0, 0)
+    with _on_device(dev):
+        if block_list is None:
+            block_list = torch.empty((B, H, num_selected), dtype=torch.int32, device=dev)
+        else:
+            _expect(block_list, "block_list", torch.int32, dev, (B, H, num_selected))
+        if workspace is None:
+            workspace = torch.empty(max(lib.triattn_select_blocks_workspace_bytes(ctypes.byref(layout)), 16),
+                                    dtype=torch.uint8, device=dev)
+        _native.check(lib.triattn_select_blocks(
+            ctypes.byref(layout), q.data_ptr(), q.stride(0), q.stride(1), int(q.shape[0]), max_query_len,
+            query_start_loc.data_ptr(), bounds.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), num_selected,
+            sink_blocks, recent_blocks, block_list.data_ptr(), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _ptr(status), _stream()), "select_blocks")
+    return block_list
