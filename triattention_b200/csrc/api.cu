@@ -26,6 +26,7 @@
 #include "score_mma_max.cuh"
 #include "score_umma_max.cuh"
 #include "select.cuh"
+#include "tensor_map.cuh"
 
 using namespace triattn;
 
@@ -77,22 +78,6 @@ static __device__ __align__(128) unsigned char g_tmap_slots[kTmapRing * kTmapMax
 std::mutex g_tmap_mutex;
 unsigned char* g_tmap_ptr[kMaxDevicesSmem] = {};
 std::atomic<unsigned> g_tmap_call{0};
-
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiledFn encode_tiled_fn() {
-  static std::atomic<void*> cached{nullptr};
-  void* f = cached.load(std::memory_order_acquire);
-  if (f == nullptr) {
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    cached.store(f, std::memory_order_release);
-  }
-  return reinterpret_cast<EncodeTiledFn>(f);
-}
 
 // Slots of this call (device pointer) or nullptr; also stamps the layers' K pointers into them on `st`.
 const unsigned char* stamp_layer_tensor_maps(const triattn_paged_layout& Y, const void* const* k_layer_ptrs,

@@ -8,9 +8,11 @@
 // running maximum and sum in fp32, in the base-2 domain.
 //
 // Bound: K and V are read once, 4 D bytes per (KV head, token), for 4 D R operations with R rows; up to about 32 rows the cache
-// stream is the limit, so what counts is that all SMs stream all the time.  The work of a call - the sequence of
-// 64-token tiles of all (request, KV head, row tile) segments - is therefore cut into equal runs of tiles, one per
-// CTA, wherever the cut falls: lengths may be as ragged as they like, and a single long request fills the device.
+// stream is the limit, so what counts is that all SMs stream all the time.  The work of a KV head - the sequence of
+// token tiles of all (request, row tile) segments - is therefore cut into J equal runs of tiles, wherever the cut falls:
+// lengths may be as ragged as they like, and a single long request fills the device.  CTA j * Hkv + h takes run j of
+// head h, so that neighbouring CTAs read the heads of the same tokens at the same time: a token's heads lie side by side
+// in memory, and runs over all (head, token) tiles, in which the heads of a token are read far apart in time, streamed a fifth slower.
 // A CTA that owns a whole segment writes its output; the others leave (m, l, unnormalised o) in a workspace slot, at most two
 // per CTA, and attend_combine_kernel joins them in a fixed order (no atomics: results repeat bit for bit).
 #pragma once
@@ -37,6 +39,9 @@ struct AttendParams {
   int B, Hkv, g, bs, num_blocks, max_blocks;
   long long block_stride, token_stride, head_stride;  // elements
   int N, max_q;
+  int box;        // tokens per TMA box: the largest of 32, 16, 8 that divides the block size (tiled kernels)
+  int slots_per_block;  // head slots per block: block_stride / head_stride (tiled kernels)
+  int min_tiles;  // tiles a CTA should have before another one is started
   float scale_log2;
   uint16_t* out;
   long long o_ts, o_hs;
@@ -86,31 +91,35 @@ __device__ __forceinline__ long long block_sum_ll(long long v, long long* red) {
   return t;
 }
 
-// tiles of requests [0, upto)
+// tiles of requests [0, upto) per KV head
 template <int THREADS>
 __device__ __forceinline__ long long attend_work_before(const AttendParams& p, int upto, int tile, int rows_per_tile,
                                                         unsigned& err, long long* red) {
   long long w = 0;
   for (int b = threadIdx.x; b < upto; b += THREADS) {
     const AttendReq r = attend_req(p, b, tile, rows_per_tile, err);
-    w += (long long)r.tiles * r.row_tiles * p.Hkv;
+    w += (long long)r.tiles * r.row_tiles;
   }
   return block_sum_ll<THREADS>(w, red);
 }
 
-// first tile of CTA i of G over W >= G tiles (every CTA has one at least), and the CTA that owns a tile
-__device__ __forceinline__ long long attend_first_tile(long long W, int G, int i) { return W * i / G; }
-__device__ __forceinline__ int attend_owner(long long W, int G, long long tile) {
-  return (int)(((tile + 1) * G - 1) / W);
+// runs that W tiles are cut into, of at most `runs`
+__device__ __forceinline__ int attend_runs(int runs, long long W, int min_tiles) {
+  return (int)min((long long)runs, (W + min_tiles - 1) / min_tiles);
+}
+// first tile of run j of J over W >= J tiles (every run has one at least), and the run that owns a tile
+__device__ __forceinline__ long long attend_first_tile(long long W, int J, int j) { return W * j / J; }
+__device__ __forceinline__ int attend_owner(long long W, int J, long long tile) {
+  return (int)(((tile + 1) * J - 1) / W);
 }
 
-// A position in the sequence of tiles: segment (request b, KV head h, row tile rt), tile t of it.
+// A position in a KV head's sequence of tiles: segment (request b, row tile rt), tile t of it.
 struct AttendCursor {
   AttendReq r;
   int b, h, rt, t;
 };
 
-// The cursor of tile `at`.  All threads call it; `found` and `red` are shared memory.
+// The cursor (but for its head) of tile `at`.  All threads call it; `found` and `red` are shared memory.
 template <int THREADS>
 __device__ __forceinline__ void attend_seek(const AttendParams& p, long long at, int tile, int rows_per_tile,
                                             long long* red, long long* found, AttendCursor& c) {
@@ -122,7 +131,7 @@ __device__ __forceinline__ void attend_seek(const AttendParams& p, long long at,
     long long w = 0;
     if (b < p.B) {
       const AttendReq r = attend_req(p, b, tile, rows_per_tile, err);
-      w = (long long)r.tiles * r.row_tiles * p.Hkv;
+      w = (long long)r.tiles * r.row_tiles;
     }
     long long incl = w;
 #pragma unroll
@@ -149,13 +158,9 @@ __device__ __forceinline__ void attend_seek(const AttendParams& p, long long at,
   }
   __syncthreads();
   c.b = (int)found[0];
-  long long rest = found[1];
   c.r = attend_req(p, c.b, tile, rows_per_tile, err);
-  const long long per_head = (long long)c.r.tiles * c.r.row_tiles;
-  c.h = (int)(rest / per_head);
-  rest -= c.h * per_head;
-  c.rt = (int)(rest / c.r.tiles);
-  c.t = (int)(rest - (long long)c.rt * c.r.tiles);
+  c.rt = (int)(found[1] / c.r.tiles);
+  c.t = (int)(found[1] - (long long)c.rt * c.r.tiles);
 }
 
 __device__ __forceinline__ void attend_advance(const AttendParams& p, AttendCursor& c, int tile, int rows_per_tile) {
@@ -163,8 +168,6 @@ __device__ __forceinline__ void attend_advance(const AttendParams& p, AttendCurs
   c.t = 0;
   if (++c.rt < c.r.row_tiles) return;
   c.rt = 0;
-  if (++c.h < p.Hkv) return;
-  c.h = 0;
   unsigned err = 0u;
   do {
     if (++c.b >= p.B) return;  // behind the last tile: never used again
@@ -288,7 +291,7 @@ __device__ __forceinline__ unsigned long long attend_word(const AttendParams& p,
 // SPLIT_P (at most 8 rows): the probabilities are carried as bf16 + bf16 remainder; the remainders ride in the
 // eight rows of the operand that would otherwise be padding, so their products cost nothing.
 template <int D, int MT, bool SPLIT_P>
-__global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __grid_constant__ AttendParams p, const int grid) {
+__global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __grid_constant__ AttendParams p, const int runs) {
   static_assert(!SPLIT_P || MT == 1, "");
   constexpr int WK = 4 / MT;                // warps over the tokens
   constexpr int KW = kAttendTile / WK;      // tokens per warp and tile
@@ -308,16 +311,18 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
   const int wr = wid % MT, wk = wid / MT;
 
   grid_dependency_wait();
+  trigger_dependents();
   unsigned err = 0u;
   const long long W = attend_work_before<kAttendThreads>(p, p.B, kAttendTile, ROWS, err, red);
   if (blockIdx.x == 0 && err) flag_status(p.status, err);
   err = 0u;
-  const int G = (int)min((long long)grid, W);
-  if ((int)blockIdx.x >= G) return;
-  const long long first = attend_first_tile(W, G, blockIdx.x), last = attend_first_tile(W, G, blockIdx.x + 1);
+  const int J = attend_runs(runs, W, p.min_tiles), run = (int)blockIdx.x / p.Hkv;
+  if (run >= J) return;
+  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
   if (tid < kStages) bad_tile[tid] = -1;
   AttendCursor lc;  // loads
   attend_seek<kAttendThreads>(p, first, kAttendTile, ROWS, red, found, lc);
+  lc.h = (int)blockIdx.x - run * p.Hkv;
   AttendCursor c = lc;  // arithmetic
   const int count = (int)(last - first);
 
@@ -617,7 +622,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
           if (r >= c.r.n * p.g) continue;
           if (whole) {
             const int i = r / p.g, hq = c.h * p.g + (r - i * p.g);
-            const float inv = l[x] > 0.f ? 1.f / l[x] : 0.f;
+            const float inv = l[x] > 0.f ? 1.f / l[x] : l[x];  // a NaN sum stays one
             uint16_t* dst = p.out + (long long)(c.r.q0 + i) * p.o_ts + (long long)hq * p.o_hs;
 #pragma unroll
             for (int j = 0; j < D / 8; ++j)
@@ -640,63 +645,108 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
   if (err) flag_status(p.status, err);
 }
 
-// Joins the parts of segments that several CTAs worked on.  One CTA per (request, KV head, row tile), one warp per row;
-// the parts are visited in the order of the tokens.
+// Joins the parts of segments that several CTAs worked on.  One CTA per (request, KV head, row tile); its warps share the
+// rows, or - fewer rows than warps - the parts of a row, visited in the order of the tokens and joined in a fixed one.
+// Everything that depends on lengths alone runs before the wait for the attention kernel, which releases this one
+// early: by then its own predecessors are complete.
 constexpr int kCombineThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kCombineThreads) attend_combine_kernel(const __grid_constant__ AttendParams p,
-                                                                         const int grid, const int tile, const int rows) {
+                                                                         const int runs, const int tile, const int rows) {
   constexpr int V = D / 32;  // columns per lane
-  __shared__ long long red[kCombineThreads / 32];
-  grid_dependency_wait();
+  constexpr int WARPS = kCombineThreads / 32;
+  __shared__ long long red[WARPS];
+  __shared__ float part[WARPS][D];
+  __shared__ float part_ml[WARPS][2];
   unsigned err = 0u;
   const int b = blockIdx.z, h = blockIdx.y, rt = blockIdx.x;
   const AttendReq r = attend_req(p, b, tile, rows, err);
-  if (rt >= r.row_tiles) return;
-  const long long before = attend_work_before<kCombineThreads>(p, b, tile, rows, err, red);
-  const long long W = attend_work_before<kCombineThreads>(p, p.B, tile, rows, err, red);
-  const long long s0 = before + ((long long)h * r.row_tiles + rt) * r.tiles;
-  const int G = (int)min((long long)grid, W);
-  const int i0 = attend_owner(W, G, s0), i1 = attend_owner(W, G, s0 + r.tiles - 1);
+  int i0 = 0, i1 = 0;
+  if (rt < r.row_tiles) {
+    const long long before = attend_work_before<kCombineThreads>(p, b, tile, rows, err, red);
+    const long long W = attend_work_before<kCombineThreads>(p, p.B, tile, rows, err, red);
+    const long long s0 = before + (long long)rt * r.tiles;
+    const int J = attend_runs(runs, W, p.min_tiles);
+    i0 = attend_owner(W, J, s0);
+    i1 = attend_owner(W, J, s0 + r.tiles - 1);
+  }
+  grid_dependency_wait();
+  trigger_dependents();
   if (i0 == i1) return;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  for (int row = wid; row < rows; row += kCombineThreads / 32) {
-    const int rr = rt * rows + row;
-    if (rr >= r.n * p.g) break;
-    float top = -INFINITY;
-    for (int i = i0; i <= i1; ++i) top = fmaxf(top, p.part_ml[((long long)(2 * i + (i == i0)) * rows + row) * 2]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float acc[V], l = 0.f;
+  const int live = min(rows, r.n * p.g - rt * rows);
+  const int share = live >= WARPS ? 1 : WARPS / live;       // warps per row
+  const int lanes_of_rows = WARPS / share;                  // rows in work at a time
+  const int mine = wid / share, turn = wid - mine * share;
+  const int parts = i1 - i0 + 1;
+  const int from = i0 + (int)((long long)parts * turn / share), to = i0 + (int)((long long)parts * (turn + 1) / share);
+  for (int row0 = 0; row0 < live; row0 += lanes_of_rows) {
+    const int row = row0 + mine;
+    const bool on = mine < lanes_of_rows && row < live;
+    float acc[V], l = 0.f, top = -INFINITY;
 #pragma unroll
     for (int x = 0; x < V; ++x) acc[x] = 0.f;
-#pragma unroll 4
-    for (int i = i0; i <= i1; ++i) {
-      const long long at = (long long)(2 * i + (i == i0)) * rows + row;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      const float f = ex2(ml.x - base);
-      l = fmaf(ml.y, f, l);
-      const float* src = p.part_o + at * D + lane * V;
-      if constexpr (V % 4 == 0) {
+    if (on) {
+      for (int i = from + lane; i < to; i += 32) top = fmaxf(top, p.part_ml[((long long)(2 * (i * p.Hkv + h) + (i == i0)) * rows + row) * 2]);
 #pragma unroll
-        for (int x = 0; x < V; x += 4) {
-          const float4 u = *reinterpret_cast<const float4*>(src + x);
-          acc[x] = fmaf(u.x, f, acc[x]);
-          acc[x + 1] = fmaf(u.y, f, acc[x + 1]);
-          acc[x + 2] = fmaf(u.z, f, acc[x + 2]);
-          acc[x + 3] = fmaf(u.w, f, acc[x + 3]);
+      for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+      for (int i = from; i < to; ++i) {
+        const long long at = (long long)(2 * (i * p.Hkv + h) + (i == i0)) * rows + row;
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+        const float f = ex2(ml.x - base);
+        l = fmaf(ml.y, f, l);
+        const float* src = p.part_o + at * D + lane * V;
+        if constexpr (V % 4 == 0) {
+#pragma unroll
+          for (int x = 0; x < V; x += 4) {
+            const float4 u = *reinterpret_cast<const float4*>(src + x);
+            acc[x] = fmaf(u.x, f, acc[x]);
+            acc[x + 1] = fmaf(u.y, f, acc[x + 1]);
+            acc[x + 2] = fmaf(u.z, f, acc[x + 2]);
+            acc[x + 3] = fmaf(u.w, f, acc[x + 3]);
+          }
+        } else {
+          const float2 u = *reinterpret_cast<const float2*>(src);
+          acc[0] = fmaf(u.x, f, acc[0]);
+          acc[1] = fmaf(u.y, f, acc[1]);
         }
-      } else {
-        const float2 u = *reinterpret_cast<const float2*>(src);
-        acc[0] = fmaf(u.x, f, acc[0]);
-        acc[1] = fmaf(u.y, f, acc[1]);
       }
     }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    const int i = rr / p.g, hq = h * p.g + (rr - i * p.g);
-    uint16_t* dst = p.out + (long long)(r.q0 + i) * p.o_ts + (long long)hq * p.o_hs + lane * V;
+    if (share > 1) {
+      if (row0 > 0) __syncthreads();
 #pragma unroll
-    for (int x = 0; x < V; x += 2) *reinterpret_cast<uint32_t*>(dst + x) = pack_bf16(acc[x] * inv, acc[x + 1] * inv);
-    if (lane == 0) p.lse[(long long)(r.q0 + i) * (p.Hkv * p.g) + hq] = (top + log2f(l)) * kLn2;
+      for (int x = 0; x < V; ++x) part[wid][lane * V + x] = acc[x];
+      if (lane == 0) {
+        part_ml[wid][0] = top;
+        part_ml[wid][1] = l;
+      }
+      __syncthreads();
+      if (turn == 0 && on) {
+        const float mine_top = top;
+        for (int w = 1; w < share; ++w) top = fmaxf(top, part_ml[wid + w][0]);
+        const float base = top == -INFINITY ? 0.f : top;
+        const float f0 = ex2(mine_top - base);
+        l *= f0;
+#pragma unroll
+        for (int x = 0; x < V; ++x) acc[x] *= f0;
+        for (int w = 1; w < share; ++w) {
+          const float f = ex2(part_ml[wid + w][0] - base);
+          l = fmaf(part_ml[wid + w][1], f, l);
+#pragma unroll
+          for (int x = 0; x < V; ++x) acc[x] = fmaf(part[wid + w][lane * V + x], f, acc[x]);
+        }
+      }
+    }
+    if (on && turn == 0) {
+      const int rr = rt * rows + row, i = rr / p.g, hq = h * p.g + (rr - i * p.g);
+      const float inv = l > 0.f ? 1.f / l : l;
+      uint16_t* dst = p.out + (long long)(r.q0 + i) * p.o_ts + (long long)hq * p.o_hs + lane * V;
+#pragma unroll
+      for (int x = 0; x < V; x += 2) *reinterpret_cast<uint32_t*>(dst + x) = pack_bf16(acc[x] * inv, acc[x + 1] * inv);
+      if (lane == 0) p.lse[(long long)(r.q0 + i) * (p.Hkv * p.g) + hq] = (top + log2f(l)) * kLn2;
+    }
   }
 }
 
@@ -711,7 +761,7 @@ template <int D>
 constexpr size_t observe_smem_bytes() { return (size_t)kAttendStages<D> * kAttendStageBytes<D> + (size_t)kObserveRows * D * 2; }
 
 template <int D>
-__global__ void __launch_bounds__(kAttendThreads) attend_observe_kernel(const __grid_constant__ AttendParams p, const int grid) {
+__global__ void __launch_bounds__(kAttendThreads) attend_observe_kernel(const __grid_constant__ AttendParams p, const int runs) {
   constexpr int PPR = D / 8, RPI = kAttendThreads / PPR, STEPS = kAttendTile / RPI;
   constexpr int kStages = kAttendStages<D>;
   constexpr int kAll = 1 << 24;  // one row tile per segment: all rows of a (request, KV head)
@@ -726,11 +776,12 @@ __global__ void __launch_bounds__(kAttendThreads) attend_observe_kernel(const __
   grid_dependency_wait();
   unsigned err = 0u;
   const long long W = attend_work_before<kAttendThreads>(p, p.B, kAttendTile, kAll, err, red);
-  const int G = (int)min((long long)grid, W);
-  if ((int)blockIdx.x >= G) return;
-  const long long first = attend_first_tile(W, G, blockIdx.x), last = attend_first_tile(W, G, blockIdx.x + 1);
+  const int J = attend_runs(runs, W, 1), run = (int)blockIdx.x / p.Hkv;
+  if (run >= J) return;
+  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
   AttendCursor lc;
   attend_seek<kAttendThreads>(p, first, kAttendTile, kAll, red, found, lc);
+  lc.h = (int)blockIdx.x - run * p.Hkv;
   AttendCursor c = lc;
   const int count = (int)(last - first);
   const uint32_t stage0 = smem_u32(smem);

@@ -8,20 +8,27 @@
 
 #include "../../include/triattn_b200.h"
 #include "attend.cuh"
+#include "attend_tma.cuh"
 #include "blocks.cuh"
 #include "common.cuh"
 #include "launch.cuh"
+#include "tensor_map.cuh"
 
 using namespace triattn;
 
 namespace {
 
 // Which attention kernel serves a call, from its geometry alone.
+//   decode   at most 16 query rows per KV head (query tokens x group size), block sizes that are multiples of 8: cache tiles by
+//            tiled TMA, products on mma.sync
+//   general  everything else: tiles gathered token by token with cp.async
+enum class AttendKind { kGeneral, kDecode };
 struct AttendPlan {
-  int rows;      // query rows per row tile
-  int mt;        // 16-row groups of the tile
-  bool split_p;  // at most 8 rows: probabilities in two bf16 parts
-  int grid;
+  AttendKind kind;
+  int tile, rows;  // tokens per tile, query rows per row tile
+  int mt;          // general kernel: 16-row groups of the tile
+  bool split_p;    // at most 8 rows: probabilities in two bf16 parts
+  int runs, min_tiles, box;  // runs per KV head
   size_t part_o, part_ml, bytes;
 };
 
@@ -30,19 +37,48 @@ long long attend_max_tiles(const triattn_paged_layout& Y, int max_q, int num_lis
   if (num_listed > 0) blocks = std::min<long long>(blocks, num_listed);
   const long long tiles = (blocks * Y.block_size + tile - 1) / tile;
   const long long row_tiles = ((long long)max_q * Y.group_size + rows - 1) / rows;
-  return tiles * row_tiles * Y.num_kv_heads * Y.num_reqs;
+  return tiles * row_tiles * Y.num_reqs;
+}
+
+// Runs per KV head on `slots` resident CTAs: as many as fit, or as fit twice where once leaves over 7 % of the slots idle.
+int attend_max_runs(int slots, int heads) {
+  int runs = slots / heads;
+  if (runs * heads * 100 < slots * 93) runs = std::max(1, 2 * slots / heads);
+  return runs;
+}
+
+// Can the layer's K and V be described by the tensor maps of attend_tma.cuh?
+bool tileable(const triattn_paged_layout& Y) {
+  const int64_t strides[3] = {Y.block_stride, Y.token_stride, Y.head_stride};
+  for (int64_t s : strides)
+    if (s <= 0 || s >= (1ll << 35)) return false;
+  return Y.block_size % 8 == 0 && Y.block_stride % Y.head_stride == 0 &&
+         Y.num_blocks * (Y.block_stride / Y.head_stride) < (1ll << 31);
 }
 
 AttendPlan attend_plan(const triattn_paged_layout& Y, int max_q, int num_listed) {
   AttendPlan a{};
   const long long R = (long long)max_q * Y.group_size;
   a.split_p = R <= 8;
-  a.mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  a.rows = a.split_p ? 8 : 16 * a.mt;
-  const int per_sm = Y.head_dim > 128 ? 1 : 2;
-  a.grid = (int)std::min<long long>((long long)kSMs * per_sm, attend_max_tiles(Y, max_q, num_listed, kAttendTile, a.rows));
-  a.part_o = (size_t)2 * a.grid * a.rows * Y.head_dim * sizeof(float);
-  a.part_ml = (size_t)2 * a.grid * a.rows * 2 * sizeof(float);
+  a.min_tiles = 1;
+  int ctas = kSMs;
+  if (R <= 16 && tileable(Y)) {
+    a.kind = AttendKind::kDecode;
+    a.tile = kDecodeTile;
+    a.rows = a.split_p ? 8 : 16;
+    a.min_tiles = kDecodeWarps;
+  } else {
+    a.kind = AttendKind::kGeneral;
+    a.tile = kAttendTile;
+    a.mt = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+    a.rows = a.split_p ? 8 : 16 * a.mt;
+    if (Y.head_dim <= 128) ctas = 2 * kSMs;
+  }
+  for (a.box = a.tile; a.box > 8 && Y.block_size % a.box; a.box /= 2) {
+  }
+  a.runs = (int)std::min<long long>(attend_max_runs(ctas, Y.num_kv_heads), attend_max_tiles(Y, max_q, num_listed, a.tile, a.rows));
+  a.part_o = (size_t)2 * a.runs * Y.num_kv_heads * a.rows * Y.head_dim * sizeof(float);
+  a.part_ml = (size_t)2 * a.runs * Y.num_kv_heads * a.rows * 2 * sizeof(float);
   a.bytes = round_up(a.part_o, 256) + round_up(a.part_ml, 256);
   return a;
 }
@@ -60,13 +96,37 @@ int validate_attend(const triattn_paged_layout* Y, int max_q, int num_listed) {
   return TRIATTN_OK;
 }
 
+// K or V of a layer as (64 channels, token mod 8, 64-channel part, token / 8, head slot): see attend_tma.cuh.  The last
+// block holds only num_kv_heads slots: the extent stops there, so no box reaches behind the cache.
+bool encode_cache_map(CUtensorMap* map, const void* base, const triattn_paged_layout& Y, int box) {
+  EncodeTiledFn encode = encode_tiled_fn();
+  if (encode == nullptr) return false;
+  const cuuint64_t parts = (cuuint64_t)Y.head_dim / 64;
+  const cuuint64_t slots = (cuuint64_t)(Y.num_blocks - 1) * (cuuint64_t)(Y.block_stride / Y.head_stride) + (cuuint64_t)Y.num_kv_heads;
+  const cuuint64_t dims[5] = {64, 8, parts, (cuuint64_t)Y.block_size / 8, slots};
+  const cuuint64_t strides[4] = {(cuuint64_t)Y.token_stride * 2, 128, (cuuint64_t)Y.token_stride * 16, (cuuint64_t)Y.head_stride * 2};
+  const cuuint32_t boxes[5] = {64, 8, (cuuint32_t)parts, (cuuint32_t)box / 8, 1}, elem[5] = {1, 1, 1, 1, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, boxes, elem,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D, bool SP>
+int launch_decode(const AttendParams& p, const AttendPlan& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  constexpr size_t smem = decode_smem_bytes<D, SP>();
+  if (!ensure_dynamic_smem<attend_decode_kernel<D, SP>>(smem)) return TRIATTN_ERR_CUDA;
+  return launch_kernel(attend_decode_kernel<D, SP>, dim3((unsigned)(a.runs * p.Hkv)), dim3(kDecodeThreads), smem, st, true, p, km, vm, a.runs);
+}
+
 template <int D>
-int launch_attend(const AttendParams& p, const AttendPlan& a, cudaStream_t st) {
+int launch_attend(const AttendParams& p, const AttendPlan& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  if (a.kind == AttendKind::kDecode)
+    return a.split_p ? launch_decode<D, true>(p, a, km, vm, st) : launch_decode<D, false>(p, a, km, vm, st);
 #define TRIATTN_LAUNCH(MT, SP)                                                                                            \
   {                                                                                                                       \
     if (!ensure_dynamic_smem<attend_paged_kernel<D, MT, SP>>(attend_smem_bytes<D, MT>())) return TRIATTN_ERR_CUDA;         \
-    return launch_kernel(attend_paged_kernel<D, MT, SP>, dim3((unsigned)a.grid), dim3(kAttendThreads),                    \
-                         attend_smem_bytes<D, MT>(), st, true, p, a.grid);                                                \
+    return launch_kernel(attend_paged_kernel<D, MT, SP>, dim3((unsigned)(a.runs * p.Hkv)), dim3(kAttendThreads),                    \
+                         attend_smem_bytes<D, MT>(), st, true, p, a.runs);                                                \
   }
   if (a.split_p) TRIATTN_LAUNCH(1, true)
   if (a.mt == 1) TRIATTN_LAUNCH(1, false)
@@ -76,15 +136,16 @@ int launch_attend(const AttendParams& p, const AttendPlan& a, cudaStream_t st) {
 }
 
 template <int D>
-int launch_attend_all(const AttendParams& p, const AttendPlan& a, int max_row_tiles, int observe_grid, cudaStream_t st) {
-  int rc = launch_attend<D>(p, a, st);
+int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensorMap& km, const CUtensorMap& vm,
+                      int max_row_tiles, int observe_runs, cudaStream_t st) {
+  int rc = launch_attend<D>(p, a, km, vm, st);
   if (rc != TRIATTN_OK) return rc;
   rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)max_row_tiles, (unsigned)p.Hkv, (unsigned)p.B),
-                     dim3(kCombineThreads), 0, st, true, p, a.grid, kAttendTile, a.rows);
+                     dim3(kCombineThreads), 0, st, true, p, a.runs, a.tile, a.rows);
   if (rc != TRIATTN_OK || p.sums == nullptr) return rc;
   if (!ensure_dynamic_smem<attend_observe_kernel<D>>(observe_smem_bytes<D>())) return TRIATTN_ERR_CUDA;
-  return launch_kernel(attend_observe_kernel<D>, dim3((unsigned)observe_grid), dim3(kAttendThreads),
-                       observe_smem_bytes<D>(), st, true, p, observe_grid);
+  return launch_kernel(attend_observe_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kAttendThreads),
+                       observe_smem_bytes<D>(), st, true, p, observe_runs);
 }
 
 }  // namespace
@@ -141,6 +202,9 @@ int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache
   p.head_stride = Y.head_stride;
   p.N = num_query_tokens;
   p.max_q = max_query_len;
+  p.box = a.box;
+  p.min_tiles = a.min_tiles;
+  p.slots_per_block = a.kind == AttendKind::kGeneral ? 0 : (int)(Y.block_stride / Y.head_stride);
   p.scale_log2 = scale * kLog2e;
   p.out = static_cast<uint16_t*>(out);
   p.o_ts = out_token_stride;
@@ -154,12 +218,15 @@ int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache
   p.status = device_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int row_tiles = (int)(((long long)max_query_len * Y.group_size + a.rows - 1) / a.rows);
-  const int observe_grid = (int)std::min<long long>((long long)kSMs * (Y.head_dim > 128 ? 1 : 2),
+  const int observe_runs = (int)std::min<long long>(attend_max_runs(kSMs * (Y.head_dim > 128 ? 1 : 2), Y.num_kv_heads),
                                                     attend_max_tiles(Y, 1, num_listed, kAttendTile, 64));
+  CUtensorMap km{}, vm{};
+  if (a.kind != AttendKind::kGeneral && (!encode_cache_map(&km, k_cache, Y, a.box) || !encode_cache_map(&vm, v_cache, Y, a.box)))
+    return TRIATTN_ERR_CUDA;
   switch (Y.head_dim) {
-    case 64: return launch_attend_all<64>(p, a, row_tiles, observe_grid, st);
-    case 128: return launch_attend_all<128>(p, a, row_tiles, observe_grid, st);
-    default: return launch_attend_all<256>(p, a, row_tiles, observe_grid, st);
+    case 64: return launch_attend_all<64>(p, a, km, vm, row_tiles, observe_runs, st);
+    case 128: return launch_attend_all<128>(p, a, km, vm, row_tiles, observe_runs, st);
+    default: return launch_attend_all<256>(p, a, km, vm, row_tiles, observe_runs, st);
   }
 }
 
