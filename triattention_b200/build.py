@@ -18,7 +18,7 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libtriattn_b200.so"
 SOURCES = ["api.cu", "attend_api.cu"]
 HEADERS = ["common.cuh", "prep.cuh", "score.cuh", "score_fma.cuh", "score_mma.cuh", "score_mma_max.cuh", "score_umma_max.cuh", "finalize.cuh", "select.cuh", "compact.cuh", "reclaim.cuh", "overrides.cuh",
-           "launch.cuh", "tensor_map.cuh", "attend.cuh", "attend_tma.cuh", "blocks.cuh", "evict.cuh", "topk_row.cuh",
+           "launch.cuh", "tensor_map.cuh", "attend.cuh", "attend_tma.cuh", "attend_umma.cuh", "umma.cuh", "blocks.cuh", "evict.cuh", "topk_row.cuh",
            "../../include/triattn_b200.h"]
 
 NVCC_FLAGS = [

@@ -9,6 +9,7 @@
 #include "../../include/triattn_b200.h"
 #include "attend.cuh"
 #include "attend_tma.cuh"
+#include "attend_umma.cuh"
 #include "blocks.cuh"
 #include "common.cuh"
 #include "launch.cuh"
@@ -21,8 +22,9 @@ namespace {
 // Which attention kernel serves a call, from its geometry alone.
 //   decode   at most 16 query rows per KV head (query tokens x group size), block sizes that are multiples of 8: cache tiles by
 //            tiled TMA, products on mma.sync
+//   tree     more rows (head dimensions 64 and 128): the same ring, products on tcgen05, 128 rows or, above that, 256 per CTA
 //   general  everything else: tiles gathered token by token with cp.async
-enum class AttendKind { kGeneral, kDecode };
+enum class AttendKind { kGeneral, kDecode, kTree };
 struct AttendPlan {
   AttendKind kind;
   int tile, rows;  // tokens per tile, query rows per row tile
@@ -67,6 +69,11 @@ AttendPlan attend_plan(const triattn_paged_layout& Y, int max_q, int num_listed)
     a.tile = kDecodeTile;
     a.rows = a.split_p ? 8 : 16;
     a.min_tiles = kDecodeWarps;
+  } else if (tileable(Y) && Y.head_dim <= 128) {
+    a.kind = AttendKind::kTree;
+    a.tile = kTreeTile;
+    a.rows = R <= 128 ? 128 : 256;
+    a.min_tiles = 4;
   } else {
     a.kind = AttendKind::kGeneral;
     a.tile = kAttendTile;
@@ -118,10 +125,20 @@ int launch_decode(const AttendParams& p, const AttendPlan& a, const CUtensorMap&
   return launch_kernel(attend_decode_kernel<D, SP>, dim3((unsigned)(a.runs * p.Hkv)), dim3(kDecodeThreads), smem, st, true, p, km, vm, a.runs);
 }
 
+template <int D, int NT>
+int launch_tree(const AttendParams& p, const AttendPlan& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
+  constexpr size_t smem = tree_smem_bytes<D, NT>();
+  if (!ensure_dynamic_smem<attend_tree_kernel<D, NT>>(smem)) return TRIATTN_ERR_CUDA;
+  return launch_kernel(attend_tree_kernel<D, NT>, dim3((unsigned)(a.runs * p.Hkv)), dim3(kTreeThreads<NT>), smem, st, true, p, km, vm, a.runs);
+}
+
 template <int D>
 int launch_attend(const AttendParams& p, const AttendPlan& a, const CUtensorMap& km, const CUtensorMap& vm, cudaStream_t st) {
   if (a.kind == AttendKind::kDecode)
     return a.split_p ? launch_decode<D, true>(p, a, km, vm, st) : launch_decode<D, false>(p, a, km, vm, st);
+  if constexpr (D <= 128) {
+    if (a.kind == AttendKind::kTree) return a.rows == 128 ? launch_tree<D, 1>(p, a, km, vm, st) : launch_tree<D, 2>(p, a, km, vm, st);
+  }
 #define TRIATTN_LAUNCH(MT, SP)                                                                                            \
   {                                                                                                                       \
     if (!ensure_dynamic_smem<attend_paged_kernel<D, MT, SP>>(attend_smem_bytes<D, MT>())) return TRIATTN_ERR_CUDA;         \

@@ -31,14 +31,17 @@ __device__ __forceinline__ uint32_t swz_off(int row, int piece) {
 
 // A ring of K/V tiles in shared memory.  pos[tile % kPosRing][i]: logical position of the first token of the tile's i-th run of
 // 8 tokens, -1 where there is none (behind the sequence, an unused list entry, a block outside the cache): such runs
-// are not loaded.  The positions are written a batch of up to 32 tiles at a time, so their ring is deeper: at most
-// STAGES + 32 tiles are between the last one read and the last one written.
-constexpr int kPosRing = 64;
+// are not loaded.  The positions are written a batch of up to kBatch tiles at a time, so their ring is deeper: at most
+// STAGES + kBatch tiles are between the last one read and the last one written.
+template <int TILE>
+constexpr int kPosRing = TILE == 32 ? 64 : 32;
+template <int TILE>
+constexpr int kBatch = kPosRing<TILE> / 2;
 template <int TILE, int STAGES>
 struct AttendRing {
-  static_assert(STAGES + 32 <= kPosRing, "positions of tiles still being read would be overwritten");
+  static_assert(STAGES + kBatch<TILE> <= kPosRing<TILE>, "positions of tiles still being read would be overwritten");
   uint64_t full[STAGES], empty[STAGES];
-  int pos[kPosRing][TILE / 8];
+  int pos[kPosRing<TILE>][TILE / 8];
   int err;
 };
 
@@ -72,7 +75,7 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
     int blk, in, pos, head, tiles;
   };
   auto look_up = [&](int left) {
-    Batch u{0, 0, -1, c.h, min(min(32 / boxes, c.r.tiles - c.t), left)};
+    Batch u{0, 0, -1, c.h, min(min(min(32 / boxes, kBatch<TILE>), c.r.tiles - c.t), left)};
     const int vp = (c.t + my_tile) * TILE + my_box * p.box;
     if (my_tile < u.tiles && vp < c.r.vlen) {
       int lb = vp / p.bs;
@@ -111,7 +114,7 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
       u.pos = -1;
     }
     if (which == 0 && my_tile < u.tiles)
-      for (int i = 0; i < p.box; i += 8) ring.pos[(it + my_tile) % kPosRing][(my_box * p.box + i) >> 3] = u.pos < 0 ? -1 : u.pos + i;
+      for (int i = 0; i < p.box; i += 8) ring.pos[(it + my_tile) % kPosRing<TILE>][(my_box * p.box + i) >> 3] = u.pos < 0 ? -1 : u.pos + i;
     __syncwarp();  // before lane 0 arrives for the batch's tiles
     const unsigned live = __ballot_sync(0xffffffffu, u.pos >= 0);
     const int slot = u.blk * p.slots_per_block + u.head, group = u.in >> 3;
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
       int top_pos = -1, low_pos = 1;
 #pragma unroll
       for (int j = 0; j < TILE / 8; ++j) {
-        const int q8 = ring.pos[n % kPosRing][j];
+        const int q8 = ring.pos[n % kPosRing<TILE>][j];
         top_pos = max(top_pos, q8);
         low_pos = min(low_pos, q8);
       }
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
       if (edge) {
 #pragma unroll
         for (int j = 0; j < TILE / 8; ++j) {
-          const int q8 = ring.pos[n % kPosRing][j];
+          const int q8 = ring.pos[n % kPosRing<TILE>][j];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int pos = q8 + (lane & 3) * 2 + (x & 1), d = pos - ctx;
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
       if (edge) {
 #pragma unroll 1
         for (int row = 0; row < TILE; ++row) {
-          const int q8 = ring.pos[n % kPosRing][row >> 3], pos = q8 + (row & 7);
+          const int q8 = ring.pos[n % kPosRing<TILE>][row >> 3], pos = q8 + (row & 7);
           uint4* v = reinterpret_cast<uint4*>(base_ptr + (vb - base) + swz_off<D>(row, lane % (D / 8)));
           if (q8 < 0 || pos >= c.r.T) {
             if (lane < D / 8) *v = make_uint4(0u, 0u, 0u, 0u);
