@@ -645,8 +645,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
   if (err) flag_status(p.status, err);
 }
 
-// Joins the parts of segments that several CTAs worked on.  One CTA per (request, KV head, row tile); its warps share the
-// rows, or - fewer rows than warps - the parts of a row, visited in the order of the tokens and joined in a fixed one.
+// Joins the parts of segments that several CTAs worked on.  One CTA per (request, KV head, 8 rows); a warp takes a row, or -
+// fewer rows than warps - a share of a row's parts, visited in the order of the tokens and joined in a fixed one.
 // Everything that depends on lengths alone runs before the wait for the attention kernel, which releases this one
 // early: by then its own predecessors are complete.
 constexpr int kCombineThreads = 256;
@@ -659,7 +659,9 @@ __global__ void __launch_bounds__(kCombineThreads) attend_combine_kernel(const _
   __shared__ float part[WARPS][D];
   __shared__ float part_ml[WARPS][2];
   unsigned err = 0u;
-  const int b = blockIdx.z, h = blockIdx.y, rt = blockIdx.x;
+  const int chunks = (rows + WARPS - 1) / WARPS;  // CTAs per row tile
+  const int b = blockIdx.z, h = blockIdx.y, rt = (int)blockIdx.x / chunks;
+  const int first_row = ((int)blockIdx.x - rt * chunks) * WARPS;
   const AttendReq r = attend_req(p, b, tile, rows, err);
   int i0 = 0, i1 = 0;
   if (rt < r.row_tiles) {
@@ -672,81 +674,77 @@ __global__ void __launch_bounds__(kCombineThreads) attend_combine_kernel(const _
   }
   grid_dependency_wait();
   trigger_dependents();
-  if (i0 == i1) return;
+  const int live = min(min(WARPS, rows - first_row), r.n * p.g - rt * rows - first_row);
+  if (i0 == i1 || live <= 0) return;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  const int live = min(rows, r.n * p.g - rt * rows);
-  const int share = live >= WARPS ? 1 : WARPS / live;       // warps per row
-  const int lanes_of_rows = WARPS / share;                  // rows in work at a time
+  const int share = WARPS / live;  // warps per row
   const int mine = wid / share, turn = wid - mine * share;
   const int parts = i1 - i0 + 1;
   const int from = i0 + (int)((long long)parts * turn / share), to = i0 + (int)((long long)parts * (turn + 1) / share);
-  for (int row0 = 0; row0 < live; row0 += lanes_of_rows) {
-    const int row = row0 + mine;
-    const bool on = mine < lanes_of_rows && row < live;
-    float acc[V], l = 0.f, top = -INFINITY;
+  const int row = first_row + mine;
+  const bool on = mine < live;
+  float acc[V], l = 0.f, top = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < V; ++x) acc[x] = 0.f;
-    if (on) {
-      for (int i = from + lane; i < to; i += 32) top = fmaxf(top, p.part_ml[((long long)(2 * (i * p.Hkv + h) + (i == i0)) * rows + row) * 2]);
+  for (int x = 0; x < V; ++x) acc[x] = 0.f;
+  if (on) {
+    for (int i = from + lane; i < to; i += 32) top = fmaxf(top, p.part_ml[((long long)(2 * (i * p.Hkv + h) + (i == i0)) * rows + row) * 2]);
 #pragma unroll
-      for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-      const float base = top == -INFINITY ? 0.f : top;
+    for (int s = 16; s; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
-      for (int i = from; i < to; ++i) {
-        const long long at = (long long)(2 * (i * p.Hkv + h) + (i == i0)) * rows + row;
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-        const float f = ex2(ml.x - base);
-        l = fmaf(ml.y, f, l);
-        const float* src = p.part_o + at * D + lane * V;
-        if constexpr (V % 4 == 0) {
+    for (int i = from; i < to; ++i) {
+      const long long at = (long long)(2 * (i * p.Hkv + h) + (i == i0)) * rows + row;
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+      const float f = ex2(ml.x - base);
+      l = fmaf(ml.y, f, l);
+      const float* src = p.part_o + at * D + lane * V;
+      if constexpr (V % 4 == 0) {
 #pragma unroll
-          for (int x = 0; x < V; x += 4) {
-            const float4 u = *reinterpret_cast<const float4*>(src + x);
-            acc[x] = fmaf(u.x, f, acc[x]);
-            acc[x + 1] = fmaf(u.y, f, acc[x + 1]);
-            acc[x + 2] = fmaf(u.z, f, acc[x + 2]);
-            acc[x + 3] = fmaf(u.w, f, acc[x + 3]);
-          }
-        } else {
-          const float2 u = *reinterpret_cast<const float2*>(src);
-          acc[0] = fmaf(u.x, f, acc[0]);
-          acc[1] = fmaf(u.y, f, acc[1]);
+        for (int x = 0; x < V; x += 4) {
+          const float4 u = *reinterpret_cast<const float4*>(src + x);
+          acc[x] = fmaf(u.x, f, acc[x]);
+          acc[x + 1] = fmaf(u.y, f, acc[x + 1]);
+          acc[x + 2] = fmaf(u.z, f, acc[x + 2]);
+          acc[x + 3] = fmaf(u.w, f, acc[x + 3]);
         }
+      } else {
+        const float2 u = *reinterpret_cast<const float2*>(src);
+        acc[0] = fmaf(u.x, f, acc[0]);
+        acc[1] = fmaf(u.y, f, acc[1]);
       }
     }
-    if (share > 1) {
-      if (row0 > 0) __syncthreads();
+  }
+  if (share > 1) {
 #pragma unroll
-      for (int x = 0; x < V; ++x) part[wid][lane * V + x] = acc[x];
-      if (lane == 0) {
-        part_ml[wid][0] = top;
-        part_ml[wid][1] = l;
-      }
-      __syncthreads();
-      if (turn == 0 && on) {
-        const float mine_top = top;
-        for (int w = 1; w < share; ++w) top = fmaxf(top, part_ml[wid + w][0]);
-        const float base = top == -INFINITY ? 0.f : top;
-        const float f0 = ex2(mine_top - base);
-        l *= f0;
+    for (int x = 0; x < V; ++x) part[wid][lane * V + x] = acc[x];
+    if (lane == 0) {
+      part_ml[wid][0] = top;
+      part_ml[wid][1] = l;
+    }
+    __syncthreads();
+    if (turn == 0 && on) {
+      const float mine_top = top;
+      for (int w = 1; w < share; ++w) top = fmaxf(top, part_ml[wid + w][0]);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float f0 = ex2(mine_top - base);
+      l *= f0;
 #pragma unroll
-        for (int x = 0; x < V; ++x) acc[x] *= f0;
-        for (int w = 1; w < share; ++w) {
-          const float f = ex2(part_ml[wid + w][0] - base);
-          l = fmaf(part_ml[wid + w][1], f, l);
+      for (int x = 0; x < V; ++x) acc[x] *= f0;
+      for (int w = 1; w < share; ++w) {
+        const float f = ex2(part_ml[wid + w][0] - base);
+        l = fmaf(part_ml[wid + w][1], f, l);
 #pragma unroll
-          for (int x = 0; x < V; ++x) acc[x] = fmaf(part[wid + w][lane * V + x], f, acc[x]);
-        }
+        for (int x = 0; x < V; ++x) acc[x] = fmaf(part[wid + w][lane * V + x], f, acc[x]);
       }
     }
-    if (on && turn == 0) {
-      const int rr = rt * rows + row, i = rr / p.g, hq = h * p.g + (rr - i * p.g);
-      const float inv = l > 0.f ? 1.f / l : l;
-      uint16_t* dst = p.out + (long long)(r.q0 + i) * p.o_ts + (long long)hq * p.o_hs + lane * V;
+  }
+  if (on && turn == 0) {
+    const int rr = rt * rows + row, i = rr / p.g, hq = h * p.g + (rr - i * p.g);
+    const float inv = l > 0.f ? 1.f / l : l;
+    uint16_t* dst = p.out + (long long)(r.q0 + i) * p.o_ts + (long long)hq * p.o_hs + lane * V;
 #pragma unroll
-      for (int x = 0; x < V; x += 2) *reinterpret_cast<uint32_t*>(dst + x) = pack_bf16(acc[x] * inv, acc[x + 1] * inv);
-      if (lane == 0) p.lse[(long long)(r.q0 + i) * (p.Hkv * p.g) + hq] = (top + log2f(l)) * kLn2;
-    }
+    for (int x = 0; x < V; x += 2) *reinterpret_cast<uint32_t*>(dst + x) = pack_bf16(acc[x] * inv, acc[x + 1] * inv);
+    if (lane == 0) p.lse[(long long)(r.q0 + i) * (p.Hkv * p.g) + hq] = (top + log2f(l)) * kLn2;
   }
 }
 

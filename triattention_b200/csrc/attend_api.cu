@@ -157,7 +157,7 @@ int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensor
                       int max_row_tiles, int observe_runs, cudaStream_t st) {
   int rc = launch_attend<D>(p, a, km, vm, st);
   if (rc != TRIATTN_OK) return rc;
-  rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)max_row_tiles, (unsigned)p.Hkv, (unsigned)p.B),
+  rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)(max_row_tiles * ((a.rows + 7) / 8)), (unsigned)p.Hkv, (unsigned)p.B),
                      dim3(kCombineThreads), 0, st, true, p, a.runs, a.tile, a.rows);
   if (rc != TRIATTN_OK || p.sums == nullptr) return rc;
   if (!ensure_dynamic_smem<attend_observe_kernel<D>>(observe_smem_bytes<D>())) return TRIATTN_ERR_CUDA;

@@ -42,6 +42,7 @@ struct AttendRing {
   static_assert(STAGES + kBatch<TILE> <= kPosRing<TILE>, "positions of tiles still being read would be overwritten");
   uint64_t full[STAGES], empty[STAGES];
   int pos[kPosRing<TILE>][TILE / 8];
+  int gaps;  // not 0: a block outside the cache was met (its tokens are not there)
   int err;
 };
 
@@ -112,6 +113,7 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
     if (u.pos >= 0 && (unsigned)u.blk >= (unsigned)p.num_blocks) {
       err |= TRIATTN_DEV_BAD_BLOCK_ID;
       u.pos = -1;
+      *(volatile int*)&ring.gaps = 1;
     }
     if (which == 0 && my_tile < u.tiles)
       for (int i = 0; i < p.box; i += 8) ring.pos[(it + my_tile) % kPosRing<TILE>][(my_box * p.box + i) >> 3] = u.pos < 0 ? -1 : u.pos + i;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
       mbar_init(smem_u32(&ring.empty[s]), 1);
     }
     mbar_fence_init();
-    ring.err = 0;
+    ring.err = ring.gaps = 0;
   }
   grid_dependency_wait();
   trigger_dependents();

@@ -60,6 +60,13 @@ __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, u
       "r"(idesc), "r"(accumulate)
       : "memory");
 }
+__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(d))
+      : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return d;
+}
 // shared-memory matrix descriptor, 128-byte swizzle.  K-major: sbo = stride of 8-row groups.  MN-major: lbo = stride of
 // 64-element groups along M / N, sbo = stride of 8-row groups along K.
 __device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
@@ -101,7 +108,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     }
     mbar_init(smem_u32(&drained), 1);
     mbar_fence_init();
-    ring.err = 0;
+    ring.err = ring.gaps = 0;
     odd_piece = -1;
   }
   grid_dependency_wait();
@@ -226,11 +233,10 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&q_ready[g]));
     };
-    // P V of tile k is over (negative: nothing to wait for).  The barrier of tile k is that of k + 2, whose product needs this
-    // thread's P: it is never more than one phase ahead, and a wait may be repeated.
-    auto wait_o = [&](int k) {
-      return k < 0 || ring_wait(o_done[g][k & 1], (uint32_t)(k >> 1) & 1u, &ring.err, p.status);
-    };
+    // P V of tile k is over.  Asked for k = n - 1 while tile n is in work, and at the end of a piece for its last tile: the
+    // barrier's phase of tile k - 2 is over by then (S of tile n came after that product), and its phase of tile k + 2
+    // needs this thread's P.
+    auto wait_o = [&](int k) { return ring_wait(o_done[g][k & 1], (uint32_t)(k >> 1) & 1u, &ring.err, p.status); };
     load_q(c);
     int piece_no = 0;
     for (int it = 0; it < count && ok; ++piece_no) {
@@ -244,25 +250,29 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       for (int x = 0; x < piece; ++x) {
         const int n = it + x, s = n % STAGES;
         const uint32_t t_s = tmem + lanes + (uint32_t)(g * 2 + (n & 1)) * 64u;
-        ok = ring_wait(ring.full[s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status) &&
-             wait_o(n - 2) &&  // long over
-             ring_wait(s_full[g][n & 1], (uint32_t)(n >> 1) & 1u, &ring.err, p.status);
+        ok = ring_wait(s_full[g][n & 1], (uint32_t)(n >> 1) & 1u, &ring.err, p.status);
         if (!ok) break;
         tc_fence_after();
-        int top_pos = -1, low_pos = 1;
+        // tiles that reach the query's own tokens, the end, or a run of tokens that is not there
+        bool edge = false;
+        if (p.block_list != nullptr || (t_begin + x + 1) * TILE > ctx || *(volatile int*)&ring.gaps != 0) {
+          // positions and values are read here: wait for the tile itself (it stays until this thread's P has been used)
+          ok = ring_wait(ring.full[s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status);
+          if (!ok) break;
+          int top_pos = -1, low_pos = 1;
 #pragma unroll
-        for (int j = 0; j < TILE / 8; ++j) {
-          const int q8 = ring.pos[n % kPosRing<TILE>][j];
-          top_pos = max(top_pos, q8);
-          low_pos = min(low_pos, q8);
+          for (int j = 0; j < TILE / 8; ++j) {
+            const int q8 = ring.pos[n % kPosRing<TILE>][j];
+            top_pos = max(top_pos, q8);
+            low_pos = min(low_pos, q8);
+          }
+          edge = low_pos < 0 || top_pos + 8 > ctx;
         }
-        const bool edge = low_pos < 0 || top_pos + 8 > ctx;
         if (!idle) {
           uint32_t sv[2][32];
           tmem_ld32(t_s, sv[0]);
           tmem_ld32(t_s + 32, sv[1]);
           tmem_ld_wait();
-          float mx = -INFINITY;
           if (edge) {
 #pragma unroll
             for (int j = 0; j < TILE; ++j) {
@@ -271,8 +281,10 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
               if (!sees) sv[j >> 5][j & 31] = 0xff800000u;  // -inf
             }
           }
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < TILE; ++j) mx = fmaxf(mx, __uint_as_float(sv[j >> 5][j & 31]));
+          for (int j = 0; j < TILE; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(sv[j >> 5][j & 31]));
+          float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
           mx *= p.scale_log2;
           const bool raise = mx > m + kTreeSlack || (m == -INFINITY && mx > m);
           if (__any_sync(0xffffffffu, raise)) {
@@ -297,16 +309,19 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
           }
           const float mbase = m == -INFINITY ? 0.f : m;
           uint32_t pv[32];
-          float l0 = 0.f, l1 = 0.f;
+          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mb2 = make_float2(-mbase, -mbase);
+          float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
 #pragma unroll
           for (int j = 0; j < TILE / 2; ++j) {
-            const float p0 = ex2(fmaf(__uint_as_float(sv[j >> 4][(2 * j) & 31]), p.scale_log2, -mbase));
-            const float p1 = ex2(fmaf(__uint_as_float(sv[j >> 4][(2 * j + 1) & 31]), p.scale_log2, -mbase));
-            l0 += p0;
-            l1 += p1;
-            pv[j] = pack_bf16(p0, p1);
+            float2 e = ffma2(make_float2(__uint_as_float(sv[j >> 4][(2 * j) & 31]), __uint_as_float(sv[j >> 4][(2 * j + 1) & 31])), sc2, mb2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            if (j & 1) lb = fadd2(lb, e);
+            else la = fadd2(la, e);
+            pv[j] = pack_bf16(e.x, e.y);
           }
-          l += l0 + l1;
+          la = fadd2(la, lb);
+          l += la.x + la.y;
           tmem_st32(t_s, pv);
           tmem_st_wait();
         }
