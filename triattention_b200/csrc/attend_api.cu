@@ -73,7 +73,7 @@ AttendPlan attend_plan(const triattn_paged_layout& Y, int max_q, int num_listed)
     a.kind = AttendKind::kTree;
     a.tile = kTreeTile;
     a.rows = R <= 128 ? 128 : 256;
-    a.min_tiles = 4;
+    a.min_tiles = 2;
   } else {
     a.kind = AttendKind::kGeneral;
     a.tile = kAttendTile;

@@ -32,15 +32,15 @@ __device__ __forceinline__ uint32_t swz_off(int row, int piece) {
 // A ring of K/V tiles in shared memory.  pos[tile % kPosRing][i]: logical position of the first token of the tile's i-th run of
 // 8 tokens, -1 where there is none (behind the sequence, an unused list entry, a block outside the cache): such runs
 // are not loaded.  The positions are written a batch of up to kBatch tiles at a time, so their ring is deeper: at most
-// STAGES + kBatch tiles are between the last one read and the last one written.
+// STAGES + kBatch + 1 tiles are between the last one read and the last one written.
 template <int TILE>
-constexpr int kPosRing = TILE == 32 ? 64 : 32;
+constexpr int kPosRing = TILE == 32 ? 64 : 16;
 template <int TILE>
 constexpr int kBatch = kPosRing<TILE> / 2;
 template <int TILE, int STAGES>
 struct AttendRing {
-  static_assert(STAGES + kBatch<TILE> <= kPosRing<TILE>, "positions of tiles still being read would be overwritten");
-  uint64_t full[STAGES], empty[STAGES];
+  static_assert(STAGES + kBatch<TILE> + 2 <= kPosRing<TILE>, "positions of tiles still being read would be overwritten");
+  uint64_t full[2][STAGES], empty[2][STAGES];  // K and V; the kernel for few rows has one pair for both
   int pos[kPosRing<TILE>][TILE / 8];
   int gaps;  // not 0: a block outside the cache was met (its tokens are not there)
   int err;
@@ -56,19 +56,28 @@ __device__ __forceinline__ bool ring_wait(uint64_t& bar, uint32_t parity, int* e
   return ok;
 }
 
-// A producer warp: K (which = 0) or V (1) of tiles 0 .. count - 1 of the run that starts at `c`, into the ring at `base`.
+// The same for a single thread.
+__device__ __forceinline__ bool thread_wait(uint64_t& bar, uint32_t parity, int* err, uint32_t* status) {
+  const bool ok = mbar_try_wait(smem_u32(&bar), parity) || mbar_wait_bounded(smem_u32(&bar), parity, err);
+  if (!ok) {
+    if (*(volatile int*)err == 0) flag_status(status, TRIATTN_DEV_WAIT_TIMEOUT);
+    *(volatile int*)err = 1;
+  }
+  return ok;
+}
+
+// A producer warp: K (which = 0) or V (1) of tiles 0 .. count - 1 of the run that starts at `c`; stage s is at
+// dst + s * stride, its barriers are full[s] and empty[s].
 // Two warps, because a warp spends some 400 cycles on a tile - waiting for the stage, arming its barrier and above all
 // issuing the loads - while the SM's share of the bandwidth moves a 16 KB tile in 700.
 template <int D, int TILE, int STAGES>
 __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUtensorMap* map, int which, AttendCursor c,
-                                               int count, int rows_per_tile, uint32_t base,
-                                               AttendRing<TILE, STAGES>& ring) {
-  constexpr uint32_t kTileBytes = TILE * D * 2;
+                                               int count, int rows_per_tile, uint32_t dst, uint32_t stride,
+                                               uint64_t* full, uint64_t* empty, AttendRing<TILE, STAGES>& ring) {
   const int lane = threadIdx.x & 31;
   const int boxes = TILE / p.box;
   const int my_tile = lane / boxes, my_box = lane - my_tile * boxes;
   const uint32_t box_bytes = (uint32_t)p.box * D * 2;
-  const uint32_t dst = base + (uint32_t)which * kTileBytes;
   unsigned err = 0u;
   // The warp looks 32 boxes up at a time, one per lane (the next 32 / boxes tiles of the segment), a batch ahead of the
   // loads: a look-up is one or two dependent global loads, as long as a tile's transfer.
@@ -122,16 +131,16 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
     const int slot = u.blk * p.slots_per_block + u.head, group = u.in >> 3;
     const uint32_t at = dst + (uint32_t)my_box * box_bytes;
     for (int j = 0; j < u.tiles; ++j, ++it) {
-      if (it >= STAGES && !ring_wait(ring.empty[s], phase, &ring.err, p.status)) {
+      if (it >= STAGES && !ring_wait(empty[s], phase, &ring.err, p.status)) {
         stop = true;
         break;
       }
       fence_proxy_async();  // the readers' accesses (acquired above) before the refill
-      const uint32_t bar = smem_u32(&ring.full[s]);
+      const uint32_t bar = smem_u32(&full[s]);
       if (lane == 0)
         mbar_arrive_expect_tx(bar, (uint32_t)__popc((live >> (j * boxes)) & ((1u << boxes) - 1u)) * box_bytes + kTestExtraTxBytes);
       __syncwarp();
-      if (my_tile == j && u.pos >= 0) tma_load_tokens(at + (uint32_t)s * 2 * kTileBytes, map, bar, group, slot);
+      if (my_tile == j && u.pos >= 0) tma_load_tokens(at + (uint32_t)s * stride, map, bar, group, slot);
       if (++s == STAGES) {
         s = 0;
         phase ^= 1u;
@@ -141,7 +150,7 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
   if (err) flag_status(p.status, err);
   // after a timeout: nothing may still be landing when the CTA retires
   if (*(volatile int*)&ring.err != 0)
-    for (int j = max(0, it - STAGES); j < it; ++j) mbar_wait_bounded(smem_u32(&ring.full[j % STAGES]), (uint32_t)(j / STAGES) & 1u);
+    for (int j = max(0, it - STAGES); j < it; ++j) mbar_wait_bounded(smem_u32(&full[j % STAGES]), (uint32_t)(j / STAGES) & 1u);
 }
 
 // ------------------------------------------------------------------------------------------ few query rows
@@ -176,8 +185,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&ring.full[s]), 2);  // the K and the V producer
-      mbar_init(smem_u32(&ring.empty[s]), 1);
+      mbar_init(smem_u32(&ring.full[0][s]), 2);  // the K and the V producer
+      mbar_init(smem_u32(&ring.empty[0][s]), 1);
     }
     mbar_fence_init();
     ring.err = ring.gaps = 0;
@@ -199,7 +208,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   float* const join = reinterpret_cast<float*>(base_ptr + STAGES * 2 * kTileBytes);
 
   if (wid >= WARPS) {
-    attend_produce<D, TILE, STAGES>(p, wid == WARPS ? &kmap : &vmap, wid - WARPS, c, count, ROWS, base, ring);
+    attend_produce<D, TILE, STAGES>(p, wid == WARPS ? &kmap : &vmap, wid - WARPS, c, count, ROWS,
+                                    base + (wid - WARPS) * kTileBytes, 2 * kTileBytes, ring.full[0], ring.empty[0], ring);
     return;
   }
 
@@ -239,7 +249,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
 
     for (int x0 = (wid + WARPS - it % WARPS) % WARPS; x0 < piece; x0 += WARPS) {
       const int n = it + x0, s = n % STAGES;
-      if (dead || !ring_wait(ring.full[s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status)) {
+      if (dead || !ring_wait(ring.full[0][s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status)) {
         dead = true;
         break;
       }
@@ -377,7 +387,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
       }
       if (edge) fence_proxy_async();  // what this warp wrote to the tile, before the refill
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ring.empty[s]));
+      if (lane == 0) mbar_arrive(smem_u32(&ring.empty[0][s]));
     }
 
     // ---- the end of the segment or of this CTA's run: the warps' parts together

@@ -1,16 +1,21 @@
 // Attention over the paged cache for many query rows (trees of drafted tokens, prompt ends): the 5th-generation tensor cores.
 //
-// A row tile is NT x 128 query rows of one KV head; token tiles of 64 come in through the ring of attend_tma.cuh.  Per
-// token tile and 128 rows:
-//   S = Q K^T      tcgen05.mma M 128, N 64, both operands K-major in shared memory, S in tensor memory (two buffers),
-//   softmax        one thread per row: 64 logits from tensor memory, running maximum and sum, P = exp2(..) as bf16
+// A row tile is NT x 128 query rows of one KV head; token tiles of 128 come in through the producers of attend_tma.cuh, K and
+// V in rings of their own (K is left earlier).  Per token tile and 128 rows:
+//   S = Q K^T      tcgen05.mma M 128, N 128, both operands K-major in shared memory, S in tensor memory,
+//   softmax        one thread per row: 128 logits from tensor memory, running maximum and sum, P = exp2(..) as bf16
 //                  back into the columns of S,
 //   O += P V       A operand P from tensor memory, B operand V as it lies in the cache (channels contiguous), O in
 //                  tensor memory for the whole segment.
-// One warp issues S of tile i before P V of tile i - 1, so the tensor cores work while the softmax threads do; with
-// NT = 2 two groups of softmax threads share every K/V tile.  The maximum a row's exponentials are taken against is only
-// raised when it has grown by more than 2^8 (P stays far inside bf16's and fp32's range, whose precision is relative): the
-// accumulator in tensor memory is then rescaled by the row's own thread, which happens a few times per segment.
+// N = 128 because the A operand is read again for every product: at N = 64 the reads of Q, 4 KB per product, take longer than the
+// product (measured: the issuing warp spent 65 cycles on each of 16 products a tile).
+// NT = 2 (more than 128 rows): two groups of softmax threads share every K/V tile and take turns with the tensor cores,
+// P V and the next S of one group running while the other group is at its exponentials.  NT = 1: S has two buffers, and S of tile i
+// is issued before P V of tile i - 1.
+// A row's exponentials are taken against the maximum of the first logits it saw, which is raised only when a logit exceeds
+// it by more than 2^64: P, the sums and O stay inside the range of bf16 and fp32 (2^127), and their precision is relative, so a
+// stale reference costs no accuracy.  That leaves one pass over a tile's logits; the rare raise rescales what the
+// row has accumulated, in its own thread.
 #pragma once
 
 #include "attend_tma.cuh"
@@ -18,15 +23,16 @@
 
 namespace triattn {
 
-constexpr int kTreeTile = 64;
-constexpr int kTreeStages = 5;
-constexpr float kTreeSlack = 8.f;  // log2 of how far a row's logits may exceed its reference maximum
+constexpr int kTreeTile = 128;
+template <int D, int NT>
+constexpr int kTreeStages = (NT == 1 ? 3 : 2) * (128 / D);  // of K and of V: 96 or 64 KB each
+constexpr float kTreeSlack = 64.f;  // log2 of how far a row's exponentials may exceed 1
 
 template <int NT>
 constexpr int kTreeThreads = NT * 128 + 96;  // softmax groups, MMA warp, K and V producers
 template <int D, int NT>
 constexpr size_t tree_smem_bytes() {
-  return 1024 + (size_t)kTreeStages * 2 * kTreeTile * D * 2 + (size_t)NT * 128 * D * 2;
+  return 1024 + (size_t)kTreeStages<D, NT> * 2 * kTreeTile * D * 2 + (size_t)NT * 128 * D * 2;
 }
 
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
@@ -49,6 +55,24 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]
       "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
       "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+// waits for the loads in flight; the values are not to be used before
+__device__ __forceinline__ void tmem_ld_wait32(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+                 "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]),
+                 "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),
+                 "+r"(v[25]), "+r"(v[26]), "+r"(v[27])
+               :
+               : "memory");
+  asm volatile("" : "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31]) : : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D (tensor memory) += A (tensor memory) B (shared memory)
@@ -78,15 +102,18 @@ template <int D, int NT>
 __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     attend_tree_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const int runs) {
-  constexpr int TILE = kTreeTile, STAGES = kTreeStages, THREADS = kTreeThreads<NT>, ROWS = 128 * NT;
+  constexpr int TILE = kTreeTile, STAGES = kTreeStages<D, NT>, THREADS = kTreeThreads<NT>, ROWS = 128 * NT;
   constexpr int MMA_WARP = NT * 4;
+  constexpr int SB = NT == 1 ? 2 : 1;            // S buffers per group
   constexpr uint32_t kTileBytes = TILE * D * 2;
   constexpr uint32_t kGroup = D * 16;            // bytes of 8 tokens
   constexpr uint32_t kQBytes = 128 * D * 2;      // 128 query rows: [D / 64][128 rows][128 B]
-  constexpr uint32_t kCols = NT == 1 ? 256 : 512;
+  constexpr uint32_t kCols = 512;                // tensor memory: S buffers (128 columns each, 256 in all), then O
   extern __shared__ unsigned char smem_raw[];
   __shared__ AttendRing<TILE, STAGES> ring;
-  __shared__ uint64_t s_full[NT][2], p_ready[NT][2], o_done[NT][2], q_ready[NT], drained;
+  // per group and S buffer: S is there, P is there, P V is over
+  __shared__ uint64_t s_full[NT][SB], p_ready[NT][SB], o_done[NT][SB];
+  __shared__ uint64_t q_ready[NT], drained;
   __shared__ long long red[THREADS / 32];
   __shared__ long long found[2];
   __shared__ uint32_t s_tmem;
@@ -94,12 +121,13 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
   if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&ring.full[s]), 2);   // the K and the V producer
-      mbar_init(smem_u32(&ring.empty[s]), 1);  // the tensor core's commit
-    }
+    for (int s = 0; s < STAGES; ++s)
+      for (int w = 0; w < 2; ++w) {
+        mbar_init(smem_u32(&ring.full[w][s]), 1);
+        mbar_init(smem_u32(&ring.empty[w][s]), 1);  // the tensor core's commit
+      }
     for (int g = 0; g < NT; ++g) {
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < SB; ++x) {
         mbar_init(smem_u32(&s_full[g][x]), 1);
         mbar_init(smem_u32(&p_ready[g][x]), 4);
         mbar_init(smem_u32(&o_done[g][x]), 1);
@@ -133,70 +161,65 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   const uint32_t tmem = s_tmem;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t q_base = base + STAGES * 2 * kTileBytes;
-  const uint32_t o_col = NT * 128;  // S buffers first, 64 columns each, then O
+  const uint32_t v_base = base + STAGES * kTileBytes, q_base = v_base + STAGES * kTileBytes;
+  constexpr uint32_t o_col = 256;
 
   if (wid > MMA_WARP) {
-    attend_produce<D, TILE, STAGES>(p, wid == MMA_WARP + 1 ? &kmap : &vmap, wid - MMA_WARP - 1, c, count, ROWS, base, ring);
+    const int w = wid - MMA_WARP - 1;
+    attend_produce<D, TILE, STAGES>(p, w == 0 ? &kmap : &vmap, w, c, count, ROWS, w == 0 ? base : v_base, kTileBytes,
+                                    ring.full[w], ring.empty[w], ring);
   } else if (wid == MMA_WARP) {
-    // ------------------------------------------------------------------------------------------ MMA issue
+    // ------------------------------------------------------------------------------------------ MMA issue: one thread
+    if (elect_one()) {
     constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 4) << 24);  // fp32 += bf16 bf16, M = 128
     constexpr uint32_t kIdescS = kIdesc | ((uint32_t)(TILE >> 3) << 17);
     constexpr uint32_t kIdescO = kIdesc | ((uint32_t)(D >> 3) << 17) | (1u << 16);         // B: channels contiguous
     bool ok = true;
-    int t_in_piece = 0, piece_no = 0;  // of tile i; of tile i - 1: prev_in_piece
-    int prev_in_piece = 0;
-    int left = min(c.r.tiles - c.t, count);  // tiles of the piece from tile i on
-    auto pv = [&](int i, int in_piece) {
+    int t_in_piece = 0, prev_in_piece = 0, piece_no = 0;  // tile i's place in its piece, tile i - 1's
+    int left = min(c.r.tiles - c.t, count);               // tiles of the piece from tile i on
+    auto issue_s = [&](int i, int g) {
       const int s = i % STAGES;
-      const uint32_t vb = base + (uint32_t)s * 2 * kTileBytes + kTileBytes;
-      const uint64_t dv = umma_desc(vb, 1024u, kGroup);
+      if (g == 0 && !thread_wait(ring.full[0][s], (uint32_t)(i / STAGES) & 1u, &ring.err, p.status)) return false;
+      if (t_in_piece == 0 && !thread_wait(q_ready[g], (uint32_t)piece_no & 1u, &ring.err, p.status)) return false;
+      fence_proxy_async();
+      tc_fence_after();
+      const uint64_t dk = umma_desc(base + (uint32_t)s * kTileBytes, 16u, kGroup), dq = umma_desc(q_base + g * kQBytes, 16u, 1024u);
+      {
 #pragma unroll
-      for (int g = 0; g < NT; ++g) {
-        if (!ring_wait(p_ready[g][i & 1], (uint32_t)(i >> 1) & 1u, &ring.err, p.status)) return false;
-        tc_fence_after();
-        const uint32_t pa = tmem + (uint32_t)(g * 2 + (i & 1)) * 64u;
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)
-            umma_bf16_ts(tmem + o_col + g * D, pa + k * 8, dv + (uint64_t)(k * 2 * kGroup >> 4), kIdescO, in_piece > 0 || k > 0 ? 1u : 0u);
-          umma_commit(smem_u32(&o_done[g][i & 1]));
-          if (g == NT - 1) umma_commit(smem_u32(&ring.empty[s]));
-        }
-        __syncwarp();
+        for (int k = 0; k < D / 16; ++k)
+          umma_bf16(tmem + (uint32_t)(g * SB + i % SB) * 128u, dq + (uint64_t)((k & 3) * 2 + (k >> 2) * (16384 >> 4)),
+                    dk + (uint64_t)((k & 3) * 2 + (k >> 2) * (1024 >> 4)), kIdescS, k ? 1u : 0u);
+        umma_commit(smem_u32(&s_full[g][i % SB]));
+        if (g == NT - 1) umma_commit(smem_u32(&ring.empty[0][s]));
       }
       return true;
     };
-    int i = 0;
-    for (; i < count && ok; ++i) {
+    auto issue_pv = [&](int i, int g, int in_piece) {
       const int s = i % STAGES;
-      ok = ring_wait(ring.full[s], (uint32_t)(i / STAGES) & 1u, &ring.err, p.status);
-      if (!ok) break;
+      if (g == 0 && !thread_wait(ring.full[1][s], (uint32_t)(i / STAGES) & 1u, &ring.err, p.status)) return false;
+      if (!thread_wait(p_ready[g][i % SB], (uint32_t)(i / SB) & 1u, &ring.err, p.status)) return false;
       fence_proxy_async();
       tc_fence_after();
-      // a new segment's query rows are written after the last P V of the one before
-      const bool turn = t_in_piece == 0 && i > 0;
-      if (turn && !(ok = pv(i - 1, prev_in_piece))) break;
-      const uint32_t kb = base + (uint32_t)s * 2 * kTileBytes;
-      const uint64_t dk = umma_desc(kb, 16u, kGroup);
+      const uint32_t pa = tmem + (uint32_t)(g * SB + i % SB) * 128u;
+      const uint64_t dv = umma_desc(v_base + (uint32_t)s * kTileBytes, 1024u, kGroup);
+      {
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k)
+          umma_bf16_ts(tmem + o_col + g * D, pa + k * 8, dv + (uint64_t)((k * 2 * kGroup) >> 4), kIdescO, in_piece > 0 || k > 0 ? 1u : 0u);
+        umma_commit(smem_u32(&o_done[g][i % SB]));
+        if (g == NT - 1) umma_commit(smem_u32(&ring.empty[1][s]));
+      }
+      return true;
+    };
+    for (int i = 0; i < count && ok; ++i) {
+      // a new segment's query rows are written after the last P V of the one before; with one S buffer P V comes first anyway
+      const bool pv_first = i > 0 && (SB == 1 || t_in_piece == 0);
 #pragma unroll
       for (int g = 0; g < NT; ++g) {
-        if (t_in_piece == 0 && ok) {
-          ok = ring_wait(q_ready[g], (uint32_t)piece_no & 1u, &ring.err, p.status);
-          tc_fence_after();
-        }
-        if (!ok) break;
-        const uint64_t dq = umma_desc(q_base + g * kQBytes, 16u, 1024u);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k)
-            umma_bf16(tmem + (uint32_t)(g * 2 + (i & 1)) * 64u, dq + (uint64_t)((k & 3) * 2 + (k >> 2) * (16384 >> 4)),
-                      dk + (uint64_t)((k & 3) * 2 + (k >> 2) * (1024 >> 4)), kIdescS, k ? 1u : 0u);
-          umma_commit(smem_u32(&s_full[g][i & 1]));
-        }
-        __syncwarp();
+        if (ok && pv_first) ok = issue_pv(i - 1, g, prev_in_piece);
+        if (ok) ok = issue_s(i, g);
+        if (ok && i > 0 && !pv_first) ok = issue_pv(i - 1, g, prev_in_piece);
       }
-      if (ok && i > 0 && !turn) ok = pv(i - 1, prev_in_piece);
       prev_in_piece = t_in_piece++;
       if (--left == 0 && i + 1 < count) {
         c.t = c.r.tiles - 1;
@@ -206,12 +229,15 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         left = min(c.r.tiles, count - i - 1);
       }
     }
-    if (ok) ok = pv(count - 1, prev_in_piece);
+#pragma unroll
+    for (int g = 0; g < NT; ++g)
+      if (ok) ok = issue_pv(count - 1, g, prev_in_piece);
     if (!ok) {  // a wait ran out: the operands must outlive what has been issued
-      if (elect_one()) umma_commit(smem_u32(&drained));
-      __syncwarp();
+      umma_commit(smem_u32(&drained));
       mbar_wait_bounded(smem_u32(&drained), 0u);
     }
+    }
+    __syncwarp();
   } else {
     // ------------------------------------------------------------------------------------------ softmax
     const int g = wid >> 2, row = tid & 127;
@@ -223,7 +249,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       const bool there = r < at.r.n * p.g;
       const int i = there ? r / p.g : 0, j = there ? r - i * p.g : 0;
       const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(at.r.q0 + i) * p.q_ts + (long long)(at.h * p.g + j) * p.q_hs);
-      unsigned char* dst = base_ptr + STAGES * 2 * kTileBytes + g * kQBytes + row * 128;
+      unsigned char* dst = base_ptr + (q_base - base) + g * kQBytes + row * 128;
 #pragma unroll
       for (int x = 0; x < D / 8; ++x) {
         const uint4 w = there ? src[x] : make_uint4(0u, 0u, 0u, 0u);
@@ -233,10 +259,10 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&q_ready[g]));
     };
-    // P V of tile k is over.  Asked for k = n - 1 while tile n is in work, and at the end of a piece for its last tile: the
-    // barrier's phase of tile k - 2 is over by then (S of tile n came after that product), and its phase of tile k + 2
-    // needs this thread's P.
-    auto wait_o = [&](int k) { return ring_wait(o_done[g][k & 1], (uint32_t)(k >> 1) & 1u, &ring.err, p.status); };
+    // P V of tile k is over.  Asked for k = n - 1 while tile n is in work (two S buffers; with one, S of tile n came after it) and
+    // for a piece's last tile: the barrier's phase before is over by then, since S of a later tile came after that
+    // product, and its next phase needs this thread's P.
+    auto wait_o = [&](int k) { return ring_wait(o_done[g][k % SB], (uint32_t)(k / SB) & 1u, &ring.err, p.status); };
     load_q(c);
     int piece_no = 0;
     for (int it = 0; it < count && ok; ++piece_no) {
@@ -249,91 +275,109 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       float m = -INFINITY, l = 0.f;
       for (int x = 0; x < piece; ++x) {
         const int n = it + x, s = n % STAGES;
-        const uint32_t t_s = tmem + lanes + (uint32_t)(g * 2 + (n & 1)) * 64u;
-        ok = ring_wait(s_full[g][n & 1], (uint32_t)(n >> 1) & 1u, &ring.err, p.status);
+        const uint32_t t_s = tmem + lanes + (uint32_t)(g * SB + n % SB) * 128u;
+        ok = ring_wait(s_full[g][n % SB], (uint32_t)(n / SB) & 1u, &ring.err, p.status);
         if (!ok) break;
         tc_fence_after();
         // tiles that reach the query's own tokens, the end, or a run of tokens that is not there
+        const int* pos8 = ring.pos[n % kPosRing<TILE>];
         bool edge = false;
         if (p.block_list != nullptr || (t_begin + x + 1) * TILE > ctx || *(volatile int*)&ring.gaps != 0) {
-          // positions and values are read here: wait for the tile itself (it stays until this thread's P has been used)
-          ok = ring_wait(ring.full[s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status);
+          // positions and values are read here: wait for the tile itself (V stays until this thread's P has been used)
+          ok = ring_wait(ring.full[1][s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status);
           if (!ok) break;
           int top_pos = -1, low_pos = 1;
 #pragma unroll
           for (int j = 0; j < TILE / 8; ++j) {
-            const int q8 = ring.pos[n % kPosRing<TILE>][j];
+            const int q8 = pos8[j];
             top_pos = max(top_pos, q8);
             low_pos = min(low_pos, q8);
           }
           edge = low_pos < 0 || top_pos + 8 > ctx;
         }
         if (!idle) {
+          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+          float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
           uint32_t sv[2][32];
           tmem_ld32(t_s, sv[0]);
-          tmem_ld32(t_s + 32, sv[1]);
-          tmem_ld_wait();
-          if (edge) {
 #pragma unroll
-            for (int j = 0; j < TILE; ++j) {
-              const int q8 = ring.pos[n % kPosRing<TILE>][j >> 3], pos = q8 + (j & 7), d = pos - ctx;
-              const bool sees = q8 >= 0 && pos < c.r.T && (d < 0 || ((word >> d) & 1ull));
-              if (!sees) sv[j >> 5][j & 31] = 0xff800000u;  // -inf
+          for (int q = 0; q < TILE / 32; ++q) {
+            uint32_t(&s32)[32] = sv[q & 1];
+            tmem_ld_wait32(s32);
+            if (q + 1 < TILE / 32) tmem_ld32(t_s + (q + 1) * 32, sv[(q + 1) & 1]);
+            if (edge) {  // hidden tokens
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const int q8 = pos8[q * 4 + (j >> 3)], pos = q8 + (j & 7), d = pos - ctx;
+                const bool sees = q8 >= 0 && pos < c.r.T && (d < 0 || ((word >> d) & 1ull));
+                if (!sees) s32[j] = 0xff800000u;
+              }
             }
-          }
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < TILE; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(sv[j >> 5][j & 31]));
-          float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-          mx *= p.scale_log2;
-          const bool raise = mx > m + kTreeSlack || (m == -INFINITY && mx > m);
-          if (__any_sync(0xffffffffu, raise)) {
-            const float mn = raise ? mx : m;
-            const float a = raise ? ex2(m - mn) : 1.f;
-            l *= a;
-            m = mn;
-            if (x > 0) {  // the accumulator exists: wait for P V of the tile before, then rescale this row
-              if (!wait_o(n - 1)) ok = false;
-              tc_fence_after();
+            for (int j = 0; j < 32; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s32[j]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+            const bool raise = mx > m + kTreeSlack;  // (also the first finite one)
+            if (__any_sync(0xffffffffu, raise)) {
+              const float mn = raise ? mx : m;
+              const float f = raise ? ex2(m - mn) : 1.f;
+              l *= f;
+              la.x *= f, la.y *= f, lb.x *= f, lb.y *= f;
+              m = mn;
+              if (q > 0) {  // this tile's P so far
+                for (int y = 0; y < q; ++y) {
+                  uint32_t pv[16];
+                  tmem_ld16(t_s + y * 16, pv);
+                  tmem_ld_wait();
 #pragma unroll
-              for (int q = 0; q < D / 32; ++q) {
-                uint32_t ov[32];
-                tmem_ld32(t_o + q * 32, ov);
-                tmem_ld_wait();
+                  for (int j = 0; j < 16; ++j) {
+                    const float2 e = bf16x2_to_float2(pv[j]);
+                    pv[j] = pack_bf16(e.x * f, e.y * f);
+                  }
+                  tmem_st16(t_s + y * 16, pv);
+                }
+              }
+              if (x > 0) {  // the accumulator, after P V of the tile before
+                if (SB > 1 && !wait_o(n - 1)) ok = false;
+                tc_fence_after();
+                for (int y = 0; y < D / 16; ++y) {
+                  uint32_t ov[16];
+                  tmem_ld16(t_o + y * 16, ov);
+                  tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * a);
-                tmem_st32(t_o + q * 32, ov);
+                  for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
+                  tmem_st16(t_o + y * 16, ov);
+                }
               }
               tmem_st_wait();
             }
-          }
-          const float mbase = m == -INFINITY ? 0.f : m;
-          uint32_t pv[32];
-          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mb2 = make_float2(-mbase, -mbase);
-          float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+            const float mbase = m == -INFINITY ? 0.f : m;
+            const float2 mb2 = make_float2(-mbase, -mbase);
+            uint32_t pv[16];
 #pragma unroll
-          for (int j = 0; j < TILE / 2; ++j) {
-            float2 e = ffma2(make_float2(__uint_as_float(sv[j >> 4][(2 * j) & 31]), __uint_as_float(sv[j >> 4][(2 * j + 1) & 31])), sc2, mb2);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            if (j & 1) lb = fadd2(lb, e);
-            else la = fadd2(la, e);
-            pv[j] = pack_bf16(e.x, e.y);
+            for (int j = 0; j < 16; ++j) {
+              float2 e = ffma2(make_float2(__uint_as_float(s32[2 * j]), __uint_as_float(s32[2 * j + 1])), sc2, mb2);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              if (j & 1) lb = fadd2(lb, e);
+              else la = fadd2(la, e);
+              pv[j] = pack_bf16(e.x, e.y);
+            }
+            tmem_st16(t_s + q * 16, pv);  // columns of logits that have been read
           }
           la = fadd2(la, lb);
           l += la.x + la.y;
-          tmem_st32(t_s, pv);
           tmem_st_wait();
         }
         if (edge && g == 0) {
           // values of tokens that are not there are zero; infinities and NaN in values of the query's own tokens are zero in the
           // product and reach the rows that see them when the piece is written (a hidden one would reach a row as 0 * inf)
-          const int key = row >> 1, q8 = ring.pos[n % kPosRing<TILE>][key >> 3], pos = q8 + (key & 7);
+          const int q8 = pos8[row >> 3], pos = q8 + (row & 7);  // one token per thread
           const bool out = q8 < 0 || pos >= c.r.T;
           if (out || pos >= ctx) {
-#pragma unroll
-            for (int q = 0; q < D / 16; ++q) {
-              uint4* v = reinterpret_cast<uint4*>(base_ptr + (uint32_t)s * 2 * kTileBytes + kTileBytes + swz_off<D>(key, (row & 1) * (D / 16) + q));
+#pragma unroll 4
+            for (int q = 0; q < D / 8; ++q) {
+              uint4* v = reinterpret_cast<uint4*>(base_ptr + (v_base - base) + (uint32_t)s * kTileBytes + swz_off<D>(row, q));
               if (out) {
                 *v = make_uint4(0u, 0u, 0u, 0u);
               } else {
@@ -349,7 +393,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&p_ready[g][n & 1]));
+        if (lane == 0) mbar_arrive(smem_u32(&p_ready[g][n % SB]));
       }
       if (!ok) break;
       ok = wait_o(it + piece - 1);
