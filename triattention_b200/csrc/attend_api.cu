@@ -154,12 +154,25 @@ int launch_attend(const AttendParams& p, const AttendPlan& a, const CUtensorMap&
 
 template <int D>
 int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensorMap& km, const CUtensorMap& vm,
-                      int max_row_tiles, int observe_runs, cudaStream_t st) {
+                      int max_row_tiles, const CUtensorMap* observe_map, int observe_runs, cudaStream_t st) {
   int rc = launch_attend<D>(p, a, km, vm, st);
   if (rc != TRIATTN_OK) return rc;
   rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)(max_row_tiles * ((a.rows + 7) / 8)), (unsigned)p.Hkv, (unsigned)p.B),
                      dim3(kCombineThreads), 0, st, true, p, a.runs, a.tile, a.rows);
   if (rc != TRIATTN_OK || p.sums == nullptr) return rc;
+  if (observe_map != nullptr) {
+    constexpr size_t smem = observe_tiled_smem_bytes<D>();
+    if (!ensure_dynamic_smem<attend_observe_tiled_kernel<D>>(smem)) return TRIATTN_ERR_CUDA;
+    for (int row0 = 0; row0 < p.max_q * p.g; row0 += kObserveTileRows<D>) {
+      AttendParams o = p;
+      for (o.box = kDecodeTile; o.bs % o.box; o.box /= 2) {
+      }
+      rc = launch_kernel(attend_observe_tiled_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kObserveThreads), smem, st,
+                         true, o, *observe_map, observe_runs, row0);
+      if (rc != TRIATTN_OK) return rc;
+    }
+    return TRIATTN_OK;
+  }
   if (!ensure_dynamic_smem<attend_observe_kernel<D>>(observe_smem_bytes<D>())) return TRIATTN_ERR_CUDA;
   return launch_kernel(attend_observe_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kAttendThreads),
                        observe_smem_bytes<D>(), st, true, p, observe_runs);
@@ -221,7 +234,7 @@ int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache
   p.max_q = max_query_len;
   p.box = a.box;
   p.min_tiles = a.min_tiles;
-  p.slots_per_block = a.kind == AttendKind::kGeneral ? 0 : (int)(Y.block_stride / Y.head_stride);
+  p.slots_per_block = tileable(Y) ? (int)(Y.block_stride / Y.head_stride) : 0;
   p.scale_log2 = scale * kLog2e;
   p.out = static_cast<uint16_t*>(out);
   p.o_ts = out_token_stride;
@@ -235,15 +248,24 @@ int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache
   p.status = device_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int row_tiles = (int)(((long long)max_query_len * Y.group_size + a.rows - 1) / a.rows);
-  const int observe_runs = (int)std::min<long long>(attend_max_runs(kSMs * (Y.head_dim > 128 ? 1 : 2), Y.num_kv_heads),
-                                                    attend_max_tiles(Y, 1, num_listed, kAttendTile, 64));
-  CUtensorMap km{}, vm{};
+  CUtensorMap km{}, vm{}, om{};
+  const bool tiled = tileable(Y);
   if (a.kind != AttendKind::kGeneral && (!encode_cache_map(&km, k_cache, Y, a.box) || !encode_cache_map(&vm, v_cache, Y, a.box)))
     return TRIATTN_ERR_CUDA;
+  int observe_runs = 0;
+  if (weight_sums != nullptr) {
+    observe_runs = (int)std::min<long long>(attend_max_runs(tiled || Y.head_dim > 128 ? kSMs : 2 * kSMs, Y.num_kv_heads),
+                                            attend_max_tiles(Y, 1, num_listed, tiled ? kDecodeTile : kAttendTile, 64));
+    int box = kDecodeTile;
+    for (; Y.block_size % box; box /= 2) {
+    }
+    if (tiled && !encode_cache_map(&om, k_cache, Y, box)) return TRIATTN_ERR_CUDA;
+  }
+  const CUtensorMap* observe_map = tiled ? &om : nullptr;
   switch (Y.head_dim) {
-    case 64: return launch_attend_all<64>(p, a, km, vm, row_tiles, observe_runs, st);
-    case 128: return launch_attend_all<128>(p, a, km, vm, row_tiles, observe_runs, st);
-    default: return launch_attend_all<256>(p, a, km, vm, row_tiles, observe_runs, st);
+    case 64: return launch_attend_all<64>(p, a, km, vm, row_tiles, observe_map, observe_runs, st);
+    case 128: return launch_attend_all<128>(p, a, km, vm, row_tiles, observe_map, observe_runs, st);
+    default: return launch_attend_all<256>(p, a, km, vm, row_tiles, observe_map, observe_runs, st);
   }
 }
 

@@ -37,11 +37,13 @@ template <int TILE>
 constexpr int kPosRing = TILE == 32 ? 64 : 16;
 template <int TILE>
 constexpr int kBatch = kPosRing<TILE> / 2;
-template <int TILE, int STAGES>
+template <int TILE, int STAGES, bool BLOCKS = false>
 struct AttendRing {
+  static constexpr bool kBlocks = BLOCKS;
   static_assert(STAGES + kBatch<TILE> + 2 <= kPosRing<TILE>, "positions of tiles still being read would be overwritten");
   uint64_t full[2][STAGES], empty[2][STAGES];  // K and V; the kernel for few rows has one pair for both
   int pos[kPosRing<TILE>][TILE / 8];
+  int blk[BLOCKS ? kPosRing<TILE> : 1][TILE / 8];  // the cache block each run lies in, for who asks
   int gaps;  // not 0: a block outside the cache was met (its tokens are not there)
   int err;
 };
@@ -70,10 +72,10 @@ __device__ __forceinline__ bool thread_wait(uint64_t& bar, uint32_t parity, int*
 // dst + s * stride, its barriers are full[s] and empty[s].
 // Two warps, because a warp spends some 400 cycles on a tile - waiting for the stage, arming its barrier and above all
 // issuing the loads - while the SM's share of the bandwidth moves a 16 KB tile in 700.
-template <int D, int TILE, int STAGES>
+template <int D, int TILE, int STAGES, class Ring>
 __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUtensorMap* map, int which, AttendCursor c,
                                                int count, int rows_per_tile, uint32_t dst, uint32_t stride,
-                                               uint64_t* full, uint64_t* empty, AttendRing<TILE, STAGES>& ring) {
+                                               uint64_t* full, uint64_t* empty, Ring& ring) {
   const int lane = threadIdx.x & 31;
   const int boxes = TILE / p.box;
   const int my_tile = lane / boxes, my_box = lane - my_tile * boxes;
@@ -125,7 +127,10 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
       *(volatile int*)&ring.gaps = 1;
     }
     if (which == 0 && my_tile < u.tiles)
-      for (int i = 0; i < p.box; i += 8) ring.pos[(it + my_tile) % kPosRing<TILE>][(my_box * p.box + i) >> 3] = u.pos < 0 ? -1 : u.pos + i;
+      for (int i = 0; i < p.box; i += 8) {
+        ring.pos[(it + my_tile) % kPosRing<TILE>][(my_box * p.box + i) >> 3] = u.pos < 0 ? -1 : u.pos + i;
+        if constexpr (Ring::kBlocks) ring.blk[(it + my_tile) % kPosRing<TILE>][(my_box * p.box + i) >> 3] = u.blk;
+      }
     __syncwarp();  // before lane 0 arrives for the batch's tiles
     const unsigned live = __ballot_sync(0xffffffffu, u.pos >= 0);
     const int slot = u.blk * p.slots_per_block + u.head, group = u.in >> 3;
@@ -482,6 +487,164 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     it += piece;
     c.t += piece - 1;
     if (it < count) attend_advance(p, c, TILE, ROWS);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ weight sums
+// The second pass of attend_observe_kernel (see attend.cuh for the formula), K tiles from the ring.  S^T = K Q^T: a warp's tile of
+// 32 tokens is the A operand (two 16-row fragments, held in registers), the query rows are the columns, eight at a
+// time from shared memory; a token's sum over the rows stays inside four lanes.  The old sums are requested when the tile arrives.
+// Calls with more than kObserveRows<D> rows run the kernel once per that many (row0): the first pass sets or adds, the
+// others add.
+constexpr int kObserveWarps = 6;
+constexpr int kObserveThreads = (kObserveWarps + 1) * 32;
+template <int D>
+constexpr int kObserveStages = D == 256 ? 6 : 12;
+template <int D>
+constexpr int kObserveTileRows = D == 256 ? 128 : 256;
+template <int D>
+constexpr size_t observe_tiled_smem_bytes() {
+  return 1024 + (size_t)kObserveStages<D> * kDecodeTile * D * 2 + (size_t)kObserveTileRows<D> * D * 2;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kObserveThreads, 1)
+    attend_observe_tiled_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap, const int runs,
+                                const int row0) {
+  constexpr int TILE = kDecodeTile, STAGES = kObserveStages<D>, WARPS = kObserveWarps, THREADS = kObserveThreads;
+  constexpr int RMAX = kObserveTileRows<D>;
+  constexpr int kAll = 1 << 24;  // all rows of a (request, KV head) in one segment
+  static_assert(STAGES % WARPS == 0, "a stage belongs to one warp");
+  constexpr uint32_t kTileBytes = TILE * D * 2;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ AttendRing<TILE, STAGES, true> ring;
+  __shared__ long long red[THREADS / 32];
+  __shared__ long long found[2];
+  __shared__ float lse2[RMAX];
+  __shared__ unsigned long long words[RMAX];
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&ring.full[0][s]), 1);
+      mbar_init(smem_u32(&ring.empty[0][s]), 1);
+    }
+    mbar_fence_init();
+    ring.err = ring.gaps = 0;
+  }
+  grid_dependency_wait();
+  trigger_dependents();
+  unsigned err = 0u;
+  const long long W = attend_work_before<THREADS>(p, p.B, TILE, kAll, err, red);
+  const int J = attend_runs(runs, W, WARPS), run = (int)blockIdx.x / p.Hkv;
+  if (run >= J) return;
+  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
+  AttendCursor c;
+  attend_seek<THREADS>(p, first, TILE, kAll, red, found, c);
+  c.h = (int)blockIdx.x - run * p.Hkv;
+  const int count = (int)(last - first);
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* const q_smem = smem_raw + (base - smem_u32(smem_raw)) + STAGES * kTileBytes;
+  const uint32_t q_base = base + STAGES * kTileBytes;
+  if (wid == WARPS) {
+    attend_produce<D, TILE, STAGES>(p, &kmap, 0, c, count, kAll, base, kTileBytes, ring.full[0], ring.empty[0], ring);
+    return;
+  }
+  auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
+  bool dead = false;
+  for (int it = 0; it < count;) {
+    const int piece = min(c.r.tiles - c.t, count - it);
+    const int R = c.r.n * p.g, ctx = c.r.T - c.r.n;
+    const int live = min(R - row0, RMAX), nt = (max(live, 0) + 7) >> 3;  // 8-row groups of this pass
+    meet();
+    for (int x = tid; x < nt * 8 * (D / 8); x += WARPS * 32) {
+      const int row = x / (D / 8), pc = x % (D / 8), r = row0 + row;
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (r < R) {
+        const int i = r / p.g, j = r - i * p.g;
+        w = *reinterpret_cast<const uint4*>(p.q + (long long)(c.r.q0 + i) * p.q_ts + (long long)(c.h * p.g + j) * p.q_hs + pc * 8);
+      }
+      *reinterpret_cast<uint4*>(q_smem + tile_off<D>(row, pc)) = w;
+    }
+    for (int row = tid; row < nt * 8; row += WARPS * 32) {
+      const int r = row0 + row;
+      float z = INFINITY;  // rows that do not exist, or see nothing, add exp2(-inf) = 0
+      unsigned long long w = 0ull;
+      if (r < R) {
+        const int i = r / p.g, j = r - i * p.g;
+        const float e = p.lse[(long long)(c.r.q0 + i) * (p.Hkv * p.g) + c.h * p.g + j];
+        if (e != -INFINITY) z = e * kLog2e;
+        w = attend_word(p, c.r, i);
+      }
+      lse2[row] = z;
+      words[row] = w;
+    }
+    meet();
+    for (int x0 = (wid + WARPS - it % WARPS) % WARPS; x0 < piece; x0 += WARPS) {
+      const int n = it + x0, s = n % STAGES;
+      if (dead || !ring_wait(ring.full[0][s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status)) {
+        dead = true;
+        break;
+      }
+      const uint32_t kb = base + (uint32_t)s * kTileBytes;
+      // this lane's four tokens: rows lane / 4 + 8 i
+      int pos[4];
+      float old[4] = {0.f, 0.f, 0.f, 0.f};
+      float* at[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int q8 = ring.pos[n % kPosRing<TILE>][i];
+        pos[i] = q8 < 0 ? -1 : q8 + (lane >> 2);
+        if (pos[i] >= c.r.T) pos[i] = -1;
+        at[i] = nullptr;
+        if ((lane & 3) == 0 && pos[i] >= 0) {
+          at[i] = p.sums + ((long long)ring.blk[n % kPosRing<TILE>][i] * p.Hkv + c.h) * p.bs + pos[i] % p.bs;
+          // a query's own token, or sums that start anew: whatever the slot holds is nobody's
+          if (row0 > 0 || (p.reset_sums == 0 && pos[i] < ctx)) old[i] = *at[i];
+        }
+      }
+      uint32_t kf[2][D / 16][4];
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) ldsm_x4(kf[a][k], kb + swz_off<D>(a * 16 + (lane & 15), k * 2 + (lane >> 4)));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ring.empty[0][s]));  // the tile is in registers
+      const bool own = max(max(pos[0], pos[1]), max(pos[2], pos[3])) >= ctx;
+      float w[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < nt; ++j) {
+        float e[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          uint32_t qf[4];
+          ldsm_x4(qf, q_base + tile_off<D>(j * 8 + (lane & 7), k * 4 + (lane >> 3)));
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            mma_bf16(e[a], kf[a][2 * k], qf[0], qf[1]);
+            mma_bf16(e[a], kf[a][2 * k + 1], qf[2], qf[3]);
+          }
+        }
+        const int row = j * 8 + (lane & 3) * 2;
+        const float z0 = lse2[row], z1 = lse2[row + 1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float p0 = ex2(fmaf(e[i >> 1][(i & 1) * 2], p.scale_log2, -z0)), p1 = ex2(fmaf(e[i >> 1][(i & 1) * 2 + 1], p.scale_log2, -z1));
+          if (own && pos[i] >= ctx) {
+            p0 = (words[row] >> (pos[i] - ctx)) & 1ull ? p0 : 0.f;
+            p1 = (words[row + 1] >> (pos[i] - ctx)) & 1ull ? p1 : 0.f;
+          }
+          w[i] += p0 + p1;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
+        w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
+        if (at[i] != nullptr) *at[i] = old[i] + w[i];
+      }
+    }
+    it += piece;
+    c.t += piece - 1;
+    if (it < count) attend_advance(p, c, TILE, kAll);
   }
 }
 
