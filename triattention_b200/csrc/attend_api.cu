@@ -297,7 +297,8 @@ int triattn_update_block_bounds(const triattn_paged_layout* layout, const void* 
   p.status = device_status;
   const long long pairs = (long long)Y.num_layers * Y.num_reqs;
   const long long warps = (long long)Y.max_blocks_per_req * Y.num_kv_heads;
-  const long long gx = std::max<long long>(1, std::min((warps + 7) / 8, (kSMs * 16 + pairs - 1) / pairs));
+  // eight CTAs per SM; a step that touches one block per request gets one CTA per (layer, request)
+  const long long gx = std::max<long long>(1, std::min((warps + 7) / 8, kSMs * 8 / pairs));
   return launch_kernel(block_bounds_kernel, dim3((unsigned)gx, (unsigned)Y.num_reqs, (unsigned)Y.num_layers),
                        dim3(kBoundsThreads), 0, static_cast<cudaStream_t>(stream), true, p);
 }
@@ -322,7 +323,8 @@ int triattn_select_blocks(const triattn_paged_layout* layout, const void* q, int
   const long long own = (max_query_len + Y.block_size - 2) / Y.block_size + 1;
   if (num_selected < sink_blocks + std::max<long long>(recent_blocks, own)) return TRIATTN_ERR_INVALID_ARGUMENT;
   if (num_query_tokens > 0 && !q) return TRIATTN_ERR_INVALID_ARGUMENT;
-  if (!aligned16(bounds) || !aligned16(workspace)) return TRIATTN_ERR_MISALIGNED;
+  if (!aligned16(bounds) || !aligned16(workspace) || !aligned16(q) || q_token_stride % 8 || q_head_stride % 8)
+    return TRIATTN_ERR_MISALIGNED;
   if (workspace_bytes < triattn_select_blocks_workspace_bytes(layout)) return TRIATTN_ERR_WORKSPACE_TOO_SMALL;
   SelectBlocksParams p{};
   p.q = static_cast<const uint16_t*>(q);
@@ -348,12 +350,15 @@ int triattn_select_blocks(const triattn_paged_layout* layout, const void* q, int
   p.status = device_status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long rows = (long long)Y.num_reqs * Y.num_kv_heads;
-  const long long gx = std::max<long long>(1, std::min<long long>((Y.max_blocks_per_req + 7) / 8, (kSMs * 8 + rows - 1) / rows));
-  const dim3 grid((unsigned)gx, (unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs);
+  // up to 32 blocks per warp, fewer while the grid does not hold two CTAs per SM
+  int per_warp = 32;
+  const auto grid_x = [&](int n) { return (Y.max_blocks_per_req + 8ll * n - 1) / (8 * n); };
+  while (per_warp > 4 && grid_x(per_warp) * rows < 2 * kSMs) per_warp /= 2;
+  const dim3 grid((unsigned)grid_x(per_warp), (unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs);
   switch (Y.head_dim) {
-    case 64: rc = launch_kernel(block_scores_kernel<64>, grid, dim3(kScoreThreads), 0, st, true, p); break;
-    case 128: rc = launch_kernel(block_scores_kernel<128>, grid, dim3(kScoreThreads), 0, st, true, p); break;
-    default: rc = launch_kernel(block_scores_kernel<256>, grid, dim3(kScoreThreads), 0, st, true, p); break;
+    case 64: rc = launch_kernel(block_scores_kernel<64>, grid, dim3(kScoreThreads), 0, st, true, p, per_warp); break;
+    case 128: rc = launch_kernel(block_scores_kernel<128>, grid, dim3(kScoreThreads), 0, st, true, p, per_warp); break;
+    default: rc = launch_kernel(block_scores_kernel<256>, grid, dim3(kScoreThreads), 0, st, true, p, per_warp); break;
   }
   if (rc != TRIATTN_OK) return rc;
   const int cap = (int)std::min<long long>(Y.max_blocks_per_req, 32768);

@@ -51,10 +51,12 @@ __global__ void __launch_bounds__(kBoundsThreads) block_bounds_kernel(const __gr
   const int lpr = p.D / 8, rpw = 32 / lpr;  // lanes per row, rows per step
   const int sub = lane / lpr, piece = lane - sub * lpr;
   const int blk0 = max(p.first[b], 0) / p.bs, blk1 = (T + p.bs - 1) / p.bs;
-  const long long items = (long long)max(blk1 - blk0, 0) * p.Hkv;
   const unsigned char* kbase = static_cast<const unsigned char*>(p.k_ptrs[l]);
-  for (long long it = (long long)blockIdx.x * (kBoundsThreads / 32) + wid; it < items; it += (long long)gridDim.x * (kBoundsThreads / 32)) {
-    const int lb = blk0 + (int)(it / p.Hkv), h = (int)(it % p.Hkv);
+  // (block, head) pairs, the head fastest; the warps of the grid's row stride over them
+  const int stride = (int)gridDim.x * (kBoundsThreads / 32), start = (int)blockIdx.x * (kBoundsThreads / 32) + wid;
+  const int d_blk = stride / p.Hkv, d_head = stride - d_blk * p.Hkv;
+  int lb = blk0 + start / p.Hkv, h = start % p.Hkv;
+  for (; lb < blk1; lb += d_blk, h += d_head, lb += h >= p.Hkv ? 1 : 0, h -= h >= p.Hkv ? p.Hkv : 0) {
     const int blk = p.block_table[(long long)b * p.max_blocks + lb];
     if ((unsigned)blk >= (unsigned)p.num_blocks) {
       err |= TRIATTN_DEV_BAD_BLOCK_ID;
@@ -62,19 +64,25 @@ __global__ void __launch_bounds__(kBoundsThreads) block_bounds_kernel(const __gr
     }
     const int n = min(p.bs, T - lb * p.bs);
     const unsigned char* src = kbase + ((long long)blk * p.block_stride + (long long)h * p.head_stride) * 2 + piece * 16;
+    const long long step = (long long)rpw * p.token_stride * 2;
+    src += (long long)sub * p.token_stride * 2;
     uint32_t lo[4] = {0x7f807f80u, 0x7f807f80u, 0x7f807f80u, 0x7f807f80u};
     uint32_t hi[4] = {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
-#pragma unroll 8
-    for (int t = sub; t < n; t += rpw) {
-      const uint4 w = *reinterpret_cast<const uint4*>(src + (long long)t * p.token_stride * 2);
-      lo[0] = min2_nan(lo[0], w.x);
-      lo[1] = min2_nan(lo[1], w.y);
-      lo[2] = min2_nan(lo[2], w.z);
-      lo[3] = min2_nan(lo[3], w.w);
-      hi[0] = max2_nan(hi[0], w.x);
-      hi[1] = max2_nan(hi[1], w.y);
-      hi[2] = max2_nan(hi[2], w.z);
-      hi[3] = max2_nan(hi[3], w.w);
+    for (int t = sub; t < n; t += 8 * rpw, src += 8 * step) {
+      uint4 w[8];  // eight loads in flight; tokens that are not there repeat the first
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = *reinterpret_cast<const uint4*>(src + (t + j * rpw < n ? j * step : 0));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        lo[0] = min2_nan(lo[0], w[j].x);
+        lo[1] = min2_nan(lo[1], w[j].y);
+        lo[2] = min2_nan(lo[2], w[j].z);
+        lo[3] = min2_nan(lo[3], w[j].w);
+        hi[0] = max2_nan(hi[0], w[j].x);
+        hi[1] = max2_nan(hi[1], w[j].y);
+        hi[2] = max2_nan(hi[2], w[j].z);
+        hi[3] = max2_nan(hi[3], w[j].w);
+      }
     }
     for (int s = 16; s >= lpr; s >>= 1) {
 #pragma unroll
@@ -132,71 +140,114 @@ __device__ __forceinline__ BlocksReq blocks_req(const SelectBlocksParams& p, int
   return r;
 }
 
+//
+// A warp takes `per_warp` consecutive blocks of one (request, KV head): its lanes fetch the block ids together, then four
+// blocks' bounds at a time (a lane holds the same 2 D / 32 channels' weights throughout), and the four sums are
+// reduced together.  Bound by the bounds' bytes (4 D per block and KV head), read once.
 template <int D>
-__global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __grid_constant__ SelectBlocksParams p) {
-  __shared__ double qsum[2][D];
+__global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __grid_constant__ SelectBlocksParams p, const int per_warp) {
+  constexpr int WARPS = kScoreThreads / 32, PCS = D / 8, GROUPS = kScoreThreads / PCS;  // 16-byte pieces of a row, rows at a time
+  __shared__ double part[2][GROUPS][D];  // sums of the queries' negative and positive parts
   grid_dependency_wait();
+  trigger_dependents();
   unsigned err = 0u;
   const int h = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const BlocksReq r = blocks_req(p, b, err);
-  if (err && blockIdx.x == 0 && h == 0 && threadIdx.x == 0) flag_status(p.status, err);
+  if (err && blockIdx.x == 0 && h == 0 && tid == 0) flag_status(p.status, err);
   err = 0u;
-  if (r.blocks <= (int)blockIdx.x * (kScoreThreads / 32)) return;
-  for (int d = threadIdx.x; d < D; d += kScoreThreads) {
-    double up = 0.0, down = 0.0;
-    for (int x = 0; x < r.n * p.g; ++x) {
-      const int i = x / p.g, j = x - i * p.g;
-      const float v = bf16_to_float(p.q[(long long)(r.q0 + i) * p.q_ts + (long long)(h * p.g + j) * p.q_hs + d]);
-      up += v > 0.f ? (double)v : 0.0;
-      down += v < 0.f ? (double)v : 0.0;
+  const int lb0 = ((int)blockIdx.x * WARPS + wid) * per_warp, lb1 = min(lb0 + per_warp, r.blocks);
+  if ((int)blockIdx.x * WARPS * per_warp >= r.blocks) return;
+  // ---- block ids of this warp's blocks; -1: always read, or not there
+  int my_blk = -1;
+  if (lb0 + lane < lb1 && lb0 + lane >= p.sink && lb0 + lane < r.forced_from) {
+    my_blk = p.block_table[(long long)b * p.max_blocks + lb0 + lane];
+    if ((unsigned)my_blk >= (unsigned)p.num_blocks) {
+      err |= TRIATTN_DEV_BAD_BLOCK_ID;
+      my_blk = -2;
     }
-    qsum[0][d] = down;
-    qsum[1][d] = up;
+  }
+  // ---- the query rows' sums, eight channels per thread
+  {
+    const int pc = tid % PCS, gr = tid / PCS;
+    double up[8], down[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) up[x] = down[x] = 0.0;
+    for (int row = gr; row < r.n * p.g; row += GROUPS) {
+      const int i = row / p.g, j = row - i * p.g;
+      const uint4 w = *reinterpret_cast<const uint4*>(p.q + (long long)(r.q0 + i) * p.q_ts + (long long)(h * p.g + j) * p.q_hs + pc * 8);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const float2 e = bf16x2_to_float2(u[x]);
+        up[2 * x] += (double)fmaxf(e.x, 0.f);
+        down[2 * x] += (double)fminf(e.x, 0.f);
+        up[2 * x + 1] += (double)fmaxf(e.y, 0.f);
+        down[2 * x + 1] += (double)fminf(e.y, 0.f);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      part[0][gr][pc * 8 + x] = down[x];
+      part[1][gr][pc * 8 + x] = up[x];
+    }
+  }
+  __syncthreads();
+  __shared__ double qsum[2 * D];
+  for (int e = tid; e < 2 * D; e += kScoreThreads) {
+    double s = 0.0;
+    const int live = min(GROUPS, r.n * p.g);
+    for (int gr = 0; gr < live; ++gr) s += part[e / D][gr][e % D];
+    qsum[e] = s;
   }
   __syncthreads();
   constexpr int PER = 2 * D / 32;  // values per lane: 4 at D = 64, 8 at 128, 16 at 256
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   double q[PER];
 #pragma unroll
-  for (int x = 0; x < PER; ++x) q[x] = (&qsum[0][0])[lane * PER + x];
+  for (int x = 0; x < PER; ++x) q[x] = qsum[lane * PER + x];
   const double unscale = __hiloint2double((1023 + 896) << 20, 0);
   float* out = p.scores + ((long long)b * p.Hkv + h) * p.max_blocks;
-  for (int lb = blockIdx.x * (kScoreThreads / 32) + wid; lb < r.blocks; lb += gridDim.x * (kScoreThreads / 32)) {
-    float score;
-    if (lb < p.sink || lb >= r.forced_from) {
-      score = INFINITY;
-    } else {
-      const int blk = p.block_table[(long long)b * p.max_blocks + lb];
-      if ((unsigned)blk >= (unsigned)p.num_blocks) {
-        err |= TRIATTN_DEV_BAD_BLOCK_ID;
-        score = -INFINITY;
-      } else {
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(p.bounds + ((long long)blk * p.Hkv + h) * 2 * D) + lane * (PER / 2);
-        uint32_t w[PER / 2];
+  auto fetch = [&](int j, uint32_t (&w)[PER / 2]) {  // bounds of the warp's block j
+    const int blk = max(__shfl_sync(0xffffffffu, my_blk, j & 31), 0);
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.bounds + ((long long)blk * p.Hkv + h) * 2 * D) + lane * (PER / 2);
 #pragma unroll
-        for (int x = 0; x < PER / 2; x += 2) {
-          const uint2 u = *reinterpret_cast<const uint2*>(src + x);
-          w[x] = u.x;
-          w[x + 1] = u.y;
-        }
-        double s = 0.0;
+    for (int x = 0; x < PER / 2; x += 2) {
+      const uint2 u = *reinterpret_cast<const uint2*>(src + x);
+      w[x] = u.x;
+      w[x + 1] = u.y;
+    }
+  };
+  const int count = lb1 - lb0;
+  for (int j0 = 0; j0 < count; j0 += 4) {
+    uint32_t w[4][PER / 2];
 #pragma unroll
-        for (int x = 0; x < PER / 2; ++x) {
-          const uint32_t a = w[x] << 16, c = w[x] & 0xffff0000u;
-          s = fma(__hiloint2double((int)((a & 0x80000000u) | ((a & 0x7fffffffu) >> 3)), 0), q[2 * x], s);
-          s = fma(__hiloint2double((int)((c & 0x80000000u) | ((c & 0x7fffffffu) >> 3)), 0), q[2 * x + 1], s);
-        }
+    for (int y = 0; y < 4; ++y) fetch(min(j0 + y, count - 1), w[y]);
+    double s[4];
 #pragma unroll
-        for (int k = 16; k; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
-        score = (float)(s * unscale);
+    for (int y = 0; y < 4; ++y) {
+      s[y] = 0.0;
+#pragma unroll
+      for (int x = 0; x < PER / 2; ++x) {
+        const uint32_t a = w[y][x] << 16, c = w[y][x] & 0xffff0000u;
+        s[y] = fma(__hiloint2double((int)((a & 0x80000000u) | ((a & 0x7fffffffu) >> 3)), 0), q[2 * x], s[y]);
+        s[y] = fma(__hiloint2double((int)((c & 0x80000000u) | ((c & 0x7fffffffu) >> 3)), 0), q[2 * x + 1], s[y]);
       }
     }
-    if (lane == 0) out[lb] = score;
+    // lanes 0-15 go on with blocks 0 and 1, 16-31 with 2 and 3; then a quarter of the warp has one block
+    const bool upper = (lane & 16) != 0, odd = (lane & 8) != 0;
+#pragma unroll
+    for (int y = 0; y < 2; ++y) s[y] = (upper ? s[y + 2] : s[y]) + __shfl_xor_sync(0xffffffffu, upper ? s[y] : s[y + 2], 16);
+    s[0] = (odd ? s[1] : s[0]) + __shfl_xor_sync(0xffffffffu, odd ? s[0] : s[1], 8);
+#pragma unroll
+    for (int k = 4; k; k >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], k);
+    const int j = j0 + (upper ? 2 : 0) + (odd ? 1 : 0);
+    const int blk = __shfl_sync(0xffffffffu, my_blk, j & 31);
+    if ((lane & 7) == 0 && j < count) out[lb0 + j] = blk >= 0 ? (float)(s[0] * unscale) : blk == -1 ? INFINITY : -INFINITY;
   }
   if (err) flag_status(p.status, err);
 }
 
-constexpr int kPickThreads = 256;
+constexpr int kPickThreads = 1024;
 __global__ void __launch_bounds__(kPickThreads) pick_blocks_kernel(const __grid_constant__ SelectBlocksParams p, const int cap) {
   extern __shared__ __align__(16) unsigned char pick_smem[];
   __shared__ TopkShared<kPickThreads> sh;
@@ -209,13 +260,15 @@ __global__ void __launch_bounds__(kPickThreads) pick_blocks_kernel(const __grid_
   int32_t* out = p.block_list + ((long long)b * p.Hkv + h) * p.num_selected;
   for (int i = k + threadIdx.x; i < p.num_selected; i += kPickThreads) out[i] = -1;
   topk_row<kPickThreads>(
-      r.blocks, k, reinterpret_cast<unsigned*>(pick_smem), cap, sh,
-      [&](int i) -> unsigned {
-        const float w = x[i];
-        return float_to_ordered(w == w ? w + 0.f : -INFINITY);
+      r.blocks, k, reinterpret_cast<unsigned*>(pick_smem), cap, sh, [&](int i) -> unsigned { return __float_as_uint(x[i]); },
+      [&](unsigned bits, int i) -> unsigned {
+        const float w = __uint_as_float(bits);
+        return float_to_ordered(w == w ? w + 0.f : -INFINITY);  // -0 ranks as 0, NaN last
       },
-      [&](bool sel, int rank, int i) {
-        if (sel) out[rank] = i;
+      [&](const bool(&sel)[4], const int(&rank)[4], const int(&at)[4], const unsigned(&)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (sel[j]) out[rank[j]] = at[j];
       });
 }
 

@@ -2,9 +2,10 @@
 // largest sums survive; the last `window` tokens and the first prefill_lens[b] are ranked above all others.  The
 // sums live beside the cache, [num_blocks, Hkv, block_size] fp32 per layer, and are compacted with it.
 //
-// One CTA per row.  A row's sums are read once through the block table into shared memory (runs of block_size values),
-// the radix passes and the output pass run from there, and the surviving sums move to their new slots in the output
-// pass: rank r <= index i, and a chunk's values are in registers or shared memory before any slot of it is written.
+// One CTA per row.  A row's sums are read once through the block table into shared memory (runs of block_size values);
+// the radix passes and the output pass run from there, and the surviving sums go from there to their new slots.  Rows of more than
+// kEvictCap tokens are read from the cache in every pass; their sums move in the output pass, run by run: rank r <= index
+// i, and a run's values are in registers before any slot of it is written.
 #pragma once
 
 #include "common.cuh"
@@ -56,29 +57,29 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const __gri
     return ((long long)blk * p.Hkv + h) * p.bs + (t - lb * p.bs);
   };
   for (int i = k + threadIdx.x; i < p.pitch; i += kEvictThreads) out[i] = -1;
+  const bool cached = n <= p.cap;
   topk_row<kEvictThreads>(
       n, k, reinterpret_cast<unsigned*>(evict_smem), p.cap, sh,
       [&](int i) -> unsigned {
-        if (i >= recent || i < guard) return float_to_ordered(INFINITY);
         const long long at = slot(i);
-        const float w = at < 0 ? -INFINITY : sums[at];
-        return float_to_ordered(w == w ? w + 0.f : -INFINITY);  // -0 ranks as 0, NaN last
+        return __float_as_uint(at < 0 ? -INFINITY : sums[at]);
       },
-      [&](bool sel, int rank, int i) {
-        // all threads of the CTA come here together; the sums of a run of indices are read before any of its
-        // destinations (at or below the run's indices) is written
-        long long from = -1, to = -1;
-        float w = 0.f;
-        if (sel) {
-          out[rank] = i;
-          if (rank != i) {
-            from = slot(i);
-            to = slot(rank);
-            if (from >= 0) w = sums[from];
+      [&](unsigned bits, int i) -> unsigned {
+        const float w = __uint_as_float(bits);
+        const float rank_by = i >= recent || i < guard ? INFINITY : w == w ? w + 0.f : -INFINITY;  // -0 ranks as 0, NaN last
+        return float_to_ordered(rank_by);
+      },
+      [&](const bool(&sel)[4], const int(&rank)[4], const int(&at)[4], const unsigned(&bits)[4]) {
+        if (!cached) __syncthreads();  // the run's sums are in registers before any of its destinations is written
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (!sel[j]) continue;
+          out[rank[j]] = at[j];
+          if (rank[j] != at[j]) {
+            const long long to = slot(rank[j]);
+            if (to >= 0) sums[to] = __uint_as_float(bits[j]);
           }
         }
-        __syncthreads();
-        if (from >= 0 && to >= 0) sums[to] = w;
       });
   if (err) flag_status(p.status, err);
 }

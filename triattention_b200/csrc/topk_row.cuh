@@ -40,21 +40,43 @@ __device__ __forceinline__ unsigned topk_scan(unsigned v, TopkShared<THREADS>& s
   return before + incl - v;
 }
 
-// load(i) -> key of element i < n (called once per element when n <= cap).  emit(sel, rank, i) is called by all threads
-// together, for runs of THREADS consecutive elements in ascending order: where sel holds, element i is chosen with that
-// rank (0 .. k-1, ascending with i).
-template <int THREADS, class Load, class Emit>
-__device__ __forceinline__ void topk_row(int n, int k, unsigned* keys, int cap, TopkShared<THREADS>& sh, Load load, Emit emit) {
+// load(i) -> the bits of element i < n, key(bits, i) -> what it is ranked by.  emit(sel, rank, i, bits) is called by all threads
+// together for runs of 4 * THREADS consecutive elements in ascending order (four to a thread): where sel holds, element i is
+// chosen with that rank (0 .. k-1, ascending with i).  With n <= cap the row is read once, before the first emit.
+template <int THREADS, class Load, class Key, class Emit>
+__device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, TopkShared<THREADS>& sh, Load load, Key key, Emit emit) {
+  constexpr int VEC = 4;
   const int tid = threadIdx.x;
   const bool cached = n <= cap;
   if (k <= 0) return;
+  if (cached) {
+    // eight loads in flight per thread
+    for (int i0 = tid; i0 < n; i0 += THREADS * 8) {
+      unsigned v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i0 + j * THREADS < n ? load(i0 + j * THREADS) : 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i0 + j * THREADS < n) bits[i0 + j * THREADS] = v[j];
+    }
+  }
+  auto bits_at = [&](int i) { return cached ? bits[i] : load(i); };
   if (k >= n) {
-    for (int i0 = 0; i0 < n; i0 += THREADS) emit(i0 + tid < n, i0 + tid, i0 + tid);
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += THREADS * VEC) {
+      bool sel[VEC];
+      int rank[VEC], at[VEC];
+      unsigned v[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        at[j] = rank[j] = i0 + tid * VEC + j;
+        sel[j] = at[j] < n;
+        v[j] = sel[j] ? bits_at(at[j]) : 0u;
+      }
+      emit(sel, rank, at, v);
+    }
     return;
   }
-  if (cached)
-    for (int i = tid; i < n; i += THREADS) keys[i] = load(i);
-  auto key_at = [&](int i) { return cached ? keys[i] : load(i); };
   if (tid == 0) {
     sh.prefix = 0u;
     sh.remaining = (unsigned)k;
@@ -67,8 +89,8 @@ __device__ __forceinline__ void topk_row(int n, int k, unsigned* keys, int cap, 
     __syncthreads();
     const unsigned prefix = sh.prefix, remaining = sh.remaining;
     for (int i = tid; i < n; i += THREADS) {
-      const unsigned key = key_at(i);
-      if (((key ^ prefix) & himask) == 0u) atomicAdd(&sh.hist[(key >> shift) & (bins - 1u)], 1u);
+      const unsigned x = key(bits_at(i), i);
+      if (((x ^ prefix) & himask) == 0u) atomicAdd(&sh.hist[(x >> shift) & (bins - 1u)], 1u);
     }
     __syncthreads();
     // thread t owns PER consecutive bins, from the top
@@ -95,17 +117,29 @@ __device__ __forceinline__ void topk_row(int n, int k, unsigned* keys, int cap, 
   }
   const unsigned kth = sh.prefix, need_eq = sh.remaining;
   unsigned base_eq = 0u, base_out = 0u;
-  for (int i0 = 0; i0 < n; i0 += THREADS) {
-    const int i = i0 + tid;
-    const unsigned key = i < n ? key_at(i) : 0u;
-    const bool gt = i < n && key > kth, eq = i < n && key == kth;
-    // both prefixes at once: counts of a chunk fit 16 bits each
+  for (int i0 = 0; i0 < n; i0 += THREADS * VEC) {
+    bool sel[VEC], eq[VEC];
+    int rank[VEC], at[VEC];
+    unsigned v[VEC], mine = 0u;  // this thread's counts: above the border, at the border (16 bits each)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      at[j] = i0 + tid * VEC + j;
+      v[j] = at[j] < n ? bits_at(at[j]) : 0u;
+      const unsigned x = at[j] < n ? key(v[j], at[j]) : 0u;
+      sel[j] = at[j] < n && x > kth;
+      eq[j] = at[j] < n && x == kth;
+      mine += (sel[j] ? 1u : 0u) + (eq[j] ? 0x10000u : 0u);
+    }
     unsigned total;
-    const unsigned pre = topk_scan<THREADS>((gt ? 1u : 0u) | (eq ? 0x10000u : 0u), sh, total);
-    const unsigned eq_before = base_eq + (pre >> 16), gt_before = pre & 0xffffu;
-    const bool sel = gt || (eq && eq_before < need_eq);
-    const unsigned rank = base_out + gt_before + (min(eq_before, need_eq) - min(base_eq, need_eq));
-    emit(sel, (int)rank, i);
+    unsigned before = topk_scan<THREADS>(mine, sh, total);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      const unsigned eq_before = base_eq + (before >> 16);
+      rank[j] = (int)(base_out + (before & 0xffffu) + (min(eq_before, need_eq) - min(base_eq, need_eq)));
+      before += (sel[j] ? 1u : 0u) + (eq[j] ? 0x10000u : 0u);
+      sel[j] = sel[j] || (eq[j] && eq_before < need_eq);
+    }
+    emit(sel, rank, at, v);
     const unsigned eq_after = base_eq + (total >> 16);
     base_out += (total & 0xffffu) + (min(eq_after, need_eq) - min(base_eq, need_eq));
     base_eq = eq_after;
