@@ -431,12 +431,17 @@ int triattn_evict_paged(const triattn_paged_layout* layout, void* const* k_layer
   p.bs = Y.block_size;
   p.num_blocks = Y.num_blocks;
   p.max_blocks = Y.max_blocks_per_req;
-  p.cap = (int)std::min<long long>((long long)Y.max_blocks_per_req * Y.block_size, kEvictCap);
+  p.cap = (int)std::min<long long>(((long long)Y.max_blocks_per_req * Y.block_size + 3) / 4 * 4, kEvictCap);
   p.status = device_status;
   const size_t smem = (size_t)p.cap * sizeof(unsigned);
-  if (!ensure_dynamic_smem<evict_select_kernel>(smem)) return TRIATTN_ERR_CUDA;
-  rc = launch_kernel(evict_select_kernel, dim3((unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs, (unsigned)Y.num_layers),
-                     dim3(kEvictThreads), smem, static_cast<cudaStream_t>(stream), true, p);
+  const dim3 grid((unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs, (unsigned)Y.num_layers);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if ((long long)Y.max_blocks_per_req * Y.block_size > kEvictLongRow) {
+    if (!ensure_dynamic_smem<evict_select_kernel<1024>>(smem)) return TRIATTN_ERR_CUDA;
+    rc = launch_kernel(evict_select_kernel<1024>, grid, dim3(1024), smem, st, true, p);
+  } else {
+    rc = launch_kernel(evict_select_kernel<512>, grid, dim3(512), smem, st, true, p);
+  }
   if (rc != TRIATTN_OK) return rc;
   const int64_t hs = keep_pitch, rs = hs * Y.num_kv_heads, ls = rs * Y.num_reqs;
   return compact_common(layout, k_layer_ptrs, v_layer_ptrs, block_table, seq_lens, keep_out, ls, rs, hs, keep_counts,

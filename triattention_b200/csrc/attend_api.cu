@@ -361,7 +361,7 @@ int triattn_select_blocks(const triattn_paged_layout* layout, const void* q, int
     default: rc = launch_kernel(block_scores_kernel<256>, grid, dim3(kScoreThreads), 0, st, true, p, per_warp); break;
   }
   if (rc != TRIATTN_OK) return rc;
-  const int cap = (int)std::min<long long>(Y.max_blocks_per_req, 32768);
+  const int cap = (int)std::min<long long>((Y.max_blocks_per_req + 3ll) / 4 * 4, 32768);
   const size_t smem = (size_t)cap * 4;
   if (!ensure_dynamic_smem<pick_blocks_kernel>(smem)) return TRIATTN_ERR_CUDA;
   return launch_kernel(pick_blocks_kernel, dim3((unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs), dim3(kPickThreads), smem, st,

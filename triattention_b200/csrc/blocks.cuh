@@ -260,7 +260,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_blocks_kernel(const __grid_
   int32_t* out = p.block_list + ((long long)b * p.Hkv + h) * p.num_selected;
   for (int i = k + threadIdx.x; i < p.num_selected; i += kPickThreads) out[i] = -1;
   topk_row<kPickThreads>(
-      r.blocks, k, reinterpret_cast<unsigned*>(pick_smem), cap, sh, [&](int i) -> unsigned { return __float_as_uint(x[i]); },
+      r.blocks, k, reinterpret_cast<unsigned*>(pick_smem), cap, sh, [](int i) -> long long { return i; },
+      [&](long long i) -> unsigned { return __float_as_uint(x[i]); },
       [&](unsigned bits, int i) -> unsigned {
         const float w = __uint_as_float(bits);
         return float_to_ordered(w == w ? w + 0.f : -INFINITY);  // -0 ranks as 0, NaN last

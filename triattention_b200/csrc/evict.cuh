@@ -13,7 +13,7 @@
 
 namespace triattn {
 
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictLongRow = 8192;  // rows that may be longer run 1024 threads, one CTA per SM; others 512, two per SM
 constexpr int kEvictCap = 49152;  // keys of a row kept in shared memory (192 KB)
 
 struct EvictParams {
@@ -28,9 +28,15 @@ struct EvictParams {
   uint32_t* status;
 };
 
-__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const __grid_constant__ EvictParams p) {
+// inverse of float_to_ordered
+__device__ __forceinline__ float ordered_to_float(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ __align__(16) unsigned char evict_smem[];
-  __shared__ TopkShared<kEvictThreads> sh;
+  __shared__ TopkShared<THREADS> sh;
   grid_dependency_wait();
   trigger_dependents();
   const int h = blockIdx.x, b = blockIdx.y, l = blockIdx.z;
@@ -56,18 +62,20 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const __gri
     }
     return ((long long)blk * p.Hkv + h) * p.bs + (t - lb * p.bs);
   };
-  for (int i = k + threadIdx.x; i < p.pitch; i += kEvictThreads) out[i] = -1;
+  for (int i = k + threadIdx.x; i < p.pitch; i += THREADS) out[i] = -1;
   const bool cached = n <= p.cap;
-  topk_row<kEvictThreads>(
+  constexpr unsigned kTop = 0xff800000u;  // float_to_ordered(+inf)
+  topk_row<THREADS>(
       n, k, reinterpret_cast<unsigned*>(evict_smem), p.cap, sh,
-      [&](int i) -> unsigned {
-        const long long at = slot(i);
-        return __float_as_uint(at < 0 ? -INFINITY : sums[at]);
+      slot,
+      [&](long long at) -> unsigned {  // (kept invertible: the sum itself goes to its new slot)
+        const float w = sums[max(at, 0ll)];
+        return float_to_ordered(at < 0 ? -INFINITY : w);
       },
       [&](unsigned bits, int i) -> unsigned {
-        const float w = __uint_as_float(bits);
-        const float rank_by = i >= recent || i < guard ? INFINITY : w == w ? w + 0.f : -INFINITY;  // -0 ranks as 0, NaN last
-        return float_to_ordered(rank_by);
+        if (i >= recent || i < guard) return kTop;
+        if (bits == 0x7fffffffu) return 0x80000000u;  // -0 ranks as 0
+        return bits > kTop ? 0u : bits;               // NaN last
       },
       [&](const bool(&sel)[4], const int(&rank)[4], const int(&at)[4], const unsigned(&bits)[4]) {
         if (!cached) __syncthreads();  // the run's sums are in registers before any of its destinations is written
@@ -75,12 +83,29 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const __gri
         for (int j = 0; j < 4; ++j) {
           if (!sel[j]) continue;
           out[rank[j]] = at[j];
-          if (rank[j] != at[j]) {
+          if (!cached && rank[j] != at[j]) {
             const long long to = slot(rank[j]);
-            if (to >= 0) sums[to] = __uint_as_float(bits[j]);
+            if (to >= 0) sums[to] = ordered_to_float(bits[j]);
           }
         }
       });
+  if (cached) {
+    __syncthreads();  // the CTA's keep list and the row's sums are there for all threads
+    const unsigned* bits = reinterpret_cast<const unsigned*>(evict_smem);
+    for (int r0 = threadIdx.x; r0 < k; r0 += THREADS * 4) {
+      int from[4];
+      long long to[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) from[j] = out[min(r0 + j * THREADS, k - 1)];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[j] = slot(min(r0 + j * THREADS, k - 1));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = r0 + j * THREADS;
+        if (r < k && from[j] != r && to[j] >= 0) sums[to[j]] = ordered_to_float(bits[from[j]]);
+      }
+    }
+  }
   if (err) flag_status(p.status, err);
 }
 

@@ -40,38 +40,52 @@ __device__ __forceinline__ unsigned topk_scan(unsigned v, TopkShared<THREADS>& s
   return before + incl - v;
 }
 
-// load(i) -> the bits of element i < n, key(bits, i) -> what it is ranked by.  emit(sel, rank, i, bits) is called by all threads
+// where(i) -> the address index of element i < n, fetch(index) -> its bits, key(bits, i) -> what it is ranked by.  emit(sel, rank, i, bits) is called by all threads
 // together for runs of 4 * THREADS consecutive elements in ascending order (four to a thread): where sel holds, element i is
-// chosen with that rank (0 .. k-1, ascending with i).  With n <= cap the row is read once, before the first emit.
-template <int THREADS, class Load, class Key, class Emit>
-__device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, TopkShared<THREADS>& sh, Load load, Key key, Emit emit) {
+// chosen with that rank (0 .. k-1, ascending with i).  With n <= cap (a multiple of 4; bits 16-byte aligned)
+// the row is read once, before the first emit.
+template <int THREADS, class Where, class Fetch, class Key, class Emit>
+__device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, TopkShared<THREADS>& sh, Where where,
+                                         Fetch fetch, Key key, Emit emit) {
   constexpr int VEC = 4;
   const int tid = threadIdx.x;
   const bool cached = n <= cap;
   if (k <= 0) return;
   if (cached) {
-    // eight loads in flight per thread
-    for (int i0 = tid; i0 < n; i0 += THREADS * 8) {
+    for (int i0 = tid; i0 < n; i0 += THREADS * 8) {  // eight look-ups, then eight loads in flight per thread
+      long long at[8];
       unsigned v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = i0 + j * THREADS < n ? load(i0 + j * THREADS) : 0u;
+      for (int j = 0; j < 8; ++j) at[j] = where(min(i0 + j * THREADS, n - 1));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = fetch(at[j]);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         if (i0 + j * THREADS < n) bits[i0 + j * THREADS] = v[j];
     }
   }
-  auto bits_at = [&](int i) { return cached ? bits[i] : load(i); };
+  auto bits_at = [&](int i) { return cached ? bits[i] : fetch(where(i)); };
+  // four consecutive elements (those at or behind n are not used)
+  auto four_at = [&](int i, unsigned(&v)[VEC]) {
+    if (cached) {
+      const uint4 w = *reinterpret_cast<const uint4*>(bits + i);
+      v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = i + j < n ? bits_at(i + j) : 0u;
+    }
+  };
   if (k >= n) {
     __syncthreads();
     for (int i0 = 0; i0 < n; i0 += THREADS * VEC) {
       bool sel[VEC];
       int rank[VEC], at[VEC];
-      unsigned v[VEC];
+      unsigned v[VEC] = {0u, 0u, 0u, 0u};
+      if (i0 + tid * VEC < n) four_at(i0 + tid * VEC, v);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         at[j] = rank[j] = i0 + tid * VEC + j;
         sel[j] = at[j] < n;
-        v[j] = sel[j] ? bits_at(at[j]) : 0u;
       }
       emit(sel, rank, at, v);
     }
@@ -88,9 +102,14 @@ __device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, 
     for (int i = tid; i < kTopkBins; i += THREADS) sh.hist[i] = 0u;
     __syncthreads();
     const unsigned prefix = sh.prefix, remaining = sh.remaining;
-    for (int i = tid; i < n; i += THREADS) {
-      const unsigned x = key(bits_at(i), i);
-      if (((x ^ prefix) & himask) == 0u) atomicAdd(&sh.hist[(x >> shift) & (bins - 1u)], 1u);
+    for (int i = tid * VEC; i < n; i += THREADS * VEC) {
+      unsigned v[VEC];
+      four_at(i, v);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const unsigned x = key(v[j], i + j);
+        if (i + j < n && ((x ^ prefix) & himask) == 0u) atomicAdd(&sh.hist[(x >> shift) & (bins - 1u)], 1u);
+      }
     }
     __syncthreads();
     // thread t owns PER consecutive bins, from the top
@@ -120,11 +139,11 @@ __device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, 
   for (int i0 = 0; i0 < n; i0 += THREADS * VEC) {
     bool sel[VEC], eq[VEC];
     int rank[VEC], at[VEC];
-    unsigned v[VEC], mine = 0u;  // this thread's counts: above the border, at the border (16 bits each)
+    unsigned v[VEC] = {0u, 0u, 0u, 0u}, mine = 0u;  // this thread's counts: above the border, at the border (16 bits each)
+    if (i0 + tid * VEC < n) four_at(i0 + tid * VEC, v);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       at[j] = i0 + tid * VEC + j;
-      v[j] = at[j] < n ? bits_at(at[j]) : 0u;
       const unsigned x = at[j] < n ? key(v[j], at[j]) : 0u;
       sel[j] = at[j] < n && x > kth;
       eq[j] = at[j] < n && x == kth;
