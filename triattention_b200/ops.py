@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional, Sequence
@@ -395,32 +396,88 @@ def rewrite_block_tables(block_table: torch.Tensor, blocks_before: torch.Tensor,
 
 
 # ------------------------------------------------------------------------------------------ attention over the cache
+# These run once per layer and decode step, so their checks avoid creating tensor views and device objects.
 _NO_GUARD = contextlib.nullcontext()
 
 
-def _on_device(dev: torch.device):
-    """Makes ``dev`` current for the launches inside (nothing to do when it already is)."""
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _on_device(index: int):
+    """Makes the device current for the launches inside (nothing to do when it already is)."""
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _expect(t: torch.Tensor, name: str, dtype: torch.dtype, dev: torch.device, shape: tuple) -> None:
-    """``t`` is a contiguous ``dtype`` tensor of ``shape`` on ``dev`` (-1: any extent)."""
-    if t.dtype != dtype or t.device != dev or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor on {dev}, got {t.dtype} on {t.device}")
-    if t.dim() != len(shape) or any(s not in (-1, d) for s, d in zip(shape, t.shape)):
-        raise ValueError(f"{name} must have shape {list(shape)} (-1: any), got {list(t.shape)}")
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _expect(t: torch.Tensor, name: str, dtype: torch.dtype, index: int, shape: tuple) -> int:
+    """Address of ``t``, a contiguous ``dtype`` tensor of ``shape`` on CUDA device ``index``."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on cuda:{index}, "
+                         f"got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _status_ptr(status: Optional[torch.Tensor], index: int):
+    if status is None:
+        return None
+    if status.dtype is not torch.int32 or status.get_device() != index or status.numel() < 1 or not status.is_contiguous():
+        raise ValueError(f"status must be an int32 tensor on cuda:{index}")
+    return status.data_ptr()
+
+
+def _workspace(t: Optional[torch.Tensor], nbytes: int, like: torch.Tensor):
+    """(tensor, address, bytes) of the caller's workspace or a new one."""
+    if t is None:
+        t = like.new_empty(max(nbytes, 16), dtype=torch.uint8)
+    elif t.get_device() != like.get_device() or not t.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {like.device}")
+    return t, t.data_ptr(), t.numel() * t.element_size()
+
+
+def _cache_geometry(kv_cache: torch.Tensor, kv_axis: Optional[int]):
+    """(K address, V address, blocks, block size, KV heads, head_dim, block / token / head stride) of one layer's
+    5-D tensor, the K/V axis found as in :func:`split_kv_axes`."""
+    shape, st = kv_cache.shape, kv_cache.stride()
+    if len(shape) != 5:
+        raise ValueError(f"Unsupported kv_cache ndim={len(shape)}, expect 5")
+    first, second = shape[0] == 2, shape[1] == 2
+    if first and second:
+        if kv_axis not in (0, 1):
+            raise ValueError("Ambiguous KV layout: both dim0 and dim1 have size 2; pass kv_axis")
+        first = kv_axis == 0
+    elif not (first or second):
+        raise ValueError("Unsupported KV layout: expected a dimension with size 2")
+    if kv_cache.dtype is not torch.bfloat16 or st[4] != 1:
+        raise ValueError("kv_cache must be a bf16 tensor with a contiguous head_dim axis")
+    k = kv_cache.data_ptr()
+    if first:
+        return k, k + 2 * st[0], shape[1], shape[2], shape[3], shape[4], st[1], st[2], st[3]
+    return k, k + 2 * st[1], shape[0], shape[2], shape[3], shape[4], st[0], st[2], st[3]
 
 
 def _check_queries(q: torch.Tensor, num_kv_heads: int, head_dim: int) -> int:
     """Query heads per KV head of ``q`` [N, Hq, D]."""
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(2) != 1:
+    if q.dtype is not torch.bfloat16 or q.dim() != 3 or q.stride(2) != 1:
         raise ValueError("q must be a bf16 [N, Hq, D] tensor with a contiguous last axis")
-    if int(q.shape[2]) != head_dim:
-        raise ValueError(f"q has head_dim {int(q.shape[2])}, the cache has {head_dim}")
-    g, rem = divmod(int(q.shape[1]), num_kv_heads)
+    if q.shape[2] != head_dim:
+        raise ValueError(f"q has head_dim {q.shape[2]}, the cache has {head_dim}")
+    g, rem = divmod(q.shape[1], num_kv_heads)
     if rem or g <= 0:
-        raise ValueError(f"q has {int(q.shape[1])} heads, not a multiple of the cache's {num_kv_heads} KV heads")
+        raise ValueError(f"q has {q.shape[1]} heads, not a multiple of the cache's {num_kv_heads} KV heads")
     return g
+
+
+@functools.lru_cache(maxsize=1024)
+def _layer_layout(B, H, g, D, bs, nb, width, block_stride, token_stride, head_stride):
+    """One layer's geometry as the library takes it (kept alive by the reference next to it)."""
+    layout = PagedLayout(1, B, H, g, D, bs, nb, width, block_stride, token_stride, head_stride, 0, 0)
+    return ctypes.byref(layout), layout
+
+
+@functools.lru_cache(maxsize=1024)
+def _attend_bytes(B, H, g, D, bs, nb, width, block_stride, token_stride, head_stride, max_query_len, num_listed):
+    ref, _ = _layer_layout(B, H, g, D, bs, nb, width, block_stride, token_stride, head_stride)
+    return int(_native.load().triattn_attend_workspace_bytes(ref, max_query_len, num_listed))
 
 
 def attend_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -446,51 +503,46 @@ def attend_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     """
     lib = _native.load()
     _require_cuda(q, "q")
-    k, v = split_kv_axes(kv_cache, kv_axis)
-    dev = q.device
-    if k.dtype != torch.bfloat16 or k.device != dev or k.stride(3) != 1:
-        raise ValueError(f"kv_cache must be a bf16 tensor on {dev} with a contiguous head_dim axis")
-    nb, bs, H, D = k.shape
+    index = q.get_device()
+    k, v, nb, bs, H, D, s0, s1, s2 = _cache_geometry(kv_cache, kv_axis)
+    if kv_cache.get_device() != index:
+        raise ValueError(f"kv_cache is on {kv_cache.device}, q on {q.device}")
     g = _check_queries(q, H, D)
-    B = int(seq_lens.shape[0])
-    N = int(q.shape[0])
-    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
-    _expect(block_table, "block_table", torch.int32, dev, (B, -1))
-    _expect(query_start_loc, "query_start_loc", torch.int32, dev, (B + 1,))
-    if B == 0 or int(block_table.shape[1]) == 0:
+    B, N, S = seq_lens.numel(), q.shape[0], 0
+    width = block_table.shape[1] if block_table.dim() == 2 else -1
+    if B == 0 or width == 0:
         raise ValueError("seq_lens and block_table must not be empty")
-    S = 0
-    if tree_mask is not None:
-        _expect(tree_mask, "tree_mask", torch.int64, dev, (N,))
+    p_lens = _expect(seq_lens, "seq_lens", torch.int32, index, (B,))
+    p_table = _expect(block_table, "block_table", torch.int32, index, (B, width))
+    p_start = _expect(query_start_loc, "query_start_loc", torch.int32, index, (B + 1,))
+    p_tree = None if tree_mask is None else _expect(tree_mask, "tree_mask", torch.int64, index, (N,))
+    p_list = None
     if block_list is not None:
-        _expect(block_list, "block_list", torch.int32, dev, (B, H, -1))
-        S = int(block_list.shape[2])
+        S = block_list.shape[-1] if block_list.dim() == 3 else 0
         if S == 0:
-            raise ValueError("block_list must not be empty")
-    if weight_sums is not None:
-        _expect(weight_sums, "weight_sums", torch.float32, dev, (nb, H, bs))
-    if status is not None:
-        _expect(status, "status", torch.int32, dev, (-1,))
-    st = k.stride()
-    layout = PagedLayout(1, B, H, g, D, bs, nb, int(block_table.shape[1]), st[0], st[1], st[2], 0, 0)
-    with _on_device(dev):
+            raise ValueError("block_list must be a [B, Hkv, S] tensor with S > 0")
+        p_list = _expect(block_list, "block_list", torch.int32, index, (B, H, S))
+    p_sums = None if weight_sums is None else _expect(weight_sums, "weight_sums", torch.float32, index, (nb, H, bs))
+    p_status = _status_ptr(status, index)
+    geometry = (B, H, g, D, bs, nb, width, s0, s1, s2)
+    with _on_device(index):
         if out is None:
-            out = torch.empty((N, H * g, D), dtype=torch.bfloat16, device=dev)
-        elif out.dtype != torch.bfloat16 or out.device != dev or out.shape != q.shape or out.stride(2) != 1:
+            out = q.new_empty(q.shape)
+        elif out.dtype is not torch.bfloat16 or out.get_device() != index or out.shape != q.shape or out.stride(2) != 1:
             raise ValueError("out must be a bf16 tensor of q's shape on q's device with a contiguous last axis")
         if lse is None:
-            lse = torch.empty((N, H * g), dtype=torch.float32, device=dev)
+            lse = q.new_empty((N, H * g), dtype=torch.float32)
+            p_lse = lse.data_ptr()
         else:
-            _expect(lse, "lse", torch.float32, dev, (N, H * g))
-        if workspace is None:
-            workspace = torch.empty(max(lib.triattn_attend_workspace_bytes(ctypes.byref(layout), max_query_len, S), 16),
-                                    dtype=torch.uint8, device=dev)
+            p_lse = _expect(lse, "lse", torch.float32, index, (N, H * g))
+        if N == 0:
+            return out, lse
+        workspace, p_ws, ws_bytes = _workspace(workspace, _attend_bytes(*geometry, max_query_len, S), q)
         _native.check(lib.triattn_attend_paged(
-            ctypes.byref(layout), k.data_ptr(), v.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-            query_start_loc.data_ptr(), q.data_ptr(), q.stride(0), q.stride(1), N, max_query_len,
-            1.0 / math.sqrt(D) if scale is None else scale, _ptr(tree_mask), _ptr(block_list), S, _ptr(weight_sums),
-            1 if reset_weight_sums else 0, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _ptr(status), _stream()), "attend_paged")
+            _layer_layout(*geometry)[0], k, v, p_table, p_lens, p_start, q.data_ptr(), q.stride(0), q.stride(1), N,
+            max_query_len, 1.0 / math.sqrt(D) if scale is None else scale, p_tree, p_list, S, p_sums,
+            1 if reset_weight_sums else 0, out.data_ptr(), out.stride(0), out.stride(1), p_lse, p_ws, ws_bytes, p_status,
+            _raw_stream(index)), "attend_paged")
     return out, lse
 
 
@@ -511,25 +563,23 @@ def evict_paged(view: PagedCacheView, layout: PagedLayout, weight_sums: torch.Te
     """
     lib = _native.load()
     _require_cuda(weight_sums, "weight_sums")
-    dev = view.device
+    index = weight_sums.get_device()
     L, B, H = view.num_layers, layout.num_reqs, view.num_kv_heads
-    _expect(weight_sums, "weight_sums", torch.float32, dev, (L, view.num_blocks, H, view.block_size))
-    _expect(block_table, "block_table", torch.int32, dev, (B, layout.max_blocks_per_req))
-    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
-    _expect(keep_counts, "keep_counts", torch.int32, dev, (B,))
-    if prefill_lens is not None:
-        _expect(prefill_lens, "prefill_lens", torch.int32, dev, (B,))
-    if status is not None:
-        _expect(status, "status", torch.int32, dev, (-1,))
-    with _on_device(dev):
+    if view.k_ptrs.get_device() != index:
+        raise ValueError(f"weight_sums is on {weight_sums.device}, the cache on {view.device}")
+    p_sums = _expect(weight_sums, "weight_sums", torch.float32, index, (L, view.num_blocks, H, view.block_size))
+    p_table = _expect(block_table, "block_table", torch.int32, index, (B, layout.max_blocks_per_req))
+    p_lens = _expect(seq_lens, "seq_lens", torch.int32, index, (B,))
+    p_counts = _expect(keep_counts, "keep_counts", torch.int32, index, (B,))
+    p_prefill = None if prefill_lens is None else _expect(prefill_lens, "prefill_lens", torch.int32, index, (B,))
+    p_status = _status_ptr(status, index)
+    with _on_device(index):
         if keep_out is None:
-            keep_out = torch.empty((L, B, H, keep_pitch), dtype=torch.int32, device=dev)
-        else:
-            _expect(keep_out, "keep_out", torch.int32, dev, (L, B, H, keep_pitch))
+            keep_out = weight_sums.new_empty((L, B, H, keep_pitch), dtype=torch.int32)
+        p_keep = _expect(keep_out, "keep_out", torch.int32, index, (L, B, H, keep_pitch))
         _native.check(lib.triattn_evict_paged(
-            ctypes.byref(layout), view.k_ptrs.data_ptr(), view.v_ptrs.data_ptr(), weight_sums.data_ptr(),
-            block_table.data_ptr(), seq_lens.data_ptr(), keep_counts.data_ptr(), _ptr(prefill_lens), int(window),
-            keep_out.data_ptr(), int(keep_pitch), _ptr(status), _stream()), "evict_paged")
+            ctypes.byref(layout), view.k_ptrs.data_ptr(), view.v_ptrs.data_ptr(), p_sums, p_table, p_lens, p_counts,
+            p_prefill, int(window), p_keep, int(keep_pitch), p_status, _raw_stream(index)), "evict_paged")
     return keep_out
 
 
@@ -539,17 +589,19 @@ def update_block_bounds(view: PagedCacheView, layout: PagedLayout, bounds: torch
     (``triattn_update_block_bounds``); ``bounds`` ``[L, num_blocks, Hkv, 2, D]`` bf16 (smallest, largest)."""
     lib = _native.load()
     _require_cuda(bounds, "bounds")
-    dev, B = view.device, layout.num_reqs
-    _expect(bounds, "bounds", torch.bfloat16, dev, (view.num_layers, view.num_blocks, view.num_kv_heads, 2, view.head_dim))
-    _expect(block_table, "block_table", torch.int32, dev, (B, layout.max_blocks_per_req))
-    _expect(first_tokens, "first_tokens", torch.int32, dev, (B,))
-    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
-    if status is not None:
-        _expect(status, "status", torch.int32, dev, (-1,))
-    with _on_device(dev):
+    index, B = bounds.get_device(), layout.num_reqs
+    if view.k_ptrs.get_device() != index:
+        raise ValueError(f"bounds is on {bounds.device}, the cache on {view.device}")
+    p_bounds = _expect(bounds, "bounds", torch.bfloat16, index,
+                       (view.num_layers, view.num_blocks, view.num_kv_heads, 2, view.head_dim))
+    p_table = _expect(block_table, "block_table", torch.int32, index, (B, layout.max_blocks_per_req))
+    p_first = _expect(first_tokens, "first_tokens", torch.int32, index, (B,))
+    p_lens = _expect(seq_lens, "seq_lens", torch.int32, index, (B,))
+    p_status = _status_ptr(status, index)
+    with _on_device(index):
         _native.check(lib.triattn_update_block_bounds(
-            ctypes.byref(layout), view.k_ptrs.data_ptr(), block_table.data_ptr(), first_tokens.data_ptr(),
-            seq_lens.data_ptr(), bounds.data_ptr(), _ptr(status), _stream()), "update_block_bounds")
+            ctypes.byref(layout), view.k_ptrs.data_ptr(), p_table, p_first, p_lens, p_bounds, p_status,
+            _raw_stream(index)), "update_block_bounds")
 
 
 def select_blocks(q: torch.Tensor, bounds: torch.Tensor, seq_lens: torch.Tensor, query_start_loc: torch.Tensor,
@@ -565,34 +617,37 @@ def select_blocks(q: torch.Tensor, bounds: torch.Tensor, seq_lens: torch.Tensor,
     """
     lib = _native.load()
     _require_cuda(q, "q")
-    dev = q.device
-    _expect(bounds, "bounds", torch.bfloat16, dev, (-1, -1, 2, -1))
+    index = q.get_device()
+    if bounds.dim() != 4:
+        raise ValueError("bounds must be a [num_blocks, Hkv, 2, D] tensor")
     nb, H, _, D = bounds.shape
     g = _check_queries(q, H, D)
-    B, width = int(seq_lens.shape[0]), int(block_table.shape[1])
-    _expect(seq_lens, "seq_lens", torch.int32, dev, (B,))
-    _expect(block_table, "block_table", torch.int32, dev, (B, -1))
-    _expect(query_start_loc, "query_start_loc", torch.int32, dev, (B + 1,))
+    B, width = seq_lens.numel(), block_table.shape[1] if block_table.dim() == 2 else -1
     if B == 0 or width == 0:
         raise ValueError("seq_lens and block_table must not be empty")
+    p_bounds = _expect(bounds, "bounds", torch.bfloat16, index, (nb, H, 2, D))
+    p_lens = _expect(seq_lens, "seq_lens", torch.int32, index, (B,))
+    p_table = _expect(block_table, "block_table", torch.int32, index, (B, width))
+    p_start = _expect(query_start_loc, "query_start_loc", torch.int32, index, (B + 1,))
+    if block_size <= 0:
+        raise ValueError(f"block_size must be positive, got {block_size}")
     own = (max_query_len + block_size - 2) // block_size + 1
     if num_selected < sink_blocks + max(recent_blocks, own):
         raise ValueError(f"num_selected={num_selected} cannot hold {sink_blocks} sink and {max(recent_blocks, own)} recent blocks")
-    if status is not None:
-        _expect(status, "status", torch.int32, dev, (-1,))
+    p_status = _status_ptr(status, index)
     # strides play no part in the choice: any that pass the layout check
-    layout = PagedLayout(1, B, H, g, D, block_size, nb, width, block_size * H * D, H * D, D, 0, 0)
-    with _on_device(dev):
+    ref, _ = _layer_layout(B, H, g, D, block_size, nb, width, block_size * H * D, H * D, D)
+    with _on_device(index):
         if block_list is None:
-            block_list = torch.empty((B, H, num_selected), dtype=torch.int32, device=dev)
-        else:
-            _expect(block_list, "block_list", torch.int32, dev, (B, H, num_selected))
-        if workspace is None:
-            workspace = torch.empty(max(lib.triattn_select_blocks_workspace_bytes(ctypes.byref(layout)), 16),
-                                    dtype=torch.uint8, device=dev)
+            block_list = q.new_empty((B, H, num_selected), dtype=torch.int32)
+        p_list = _expect(block_list, "block_list", torch.int32, index, (B, H, num_selected))
+        workspace, p_ws, ws_bytes = _workspace(workspace, (B * H * width * 4 + 255) // 256 * 256, q)
         _native.check(lib.triattn_select_blocks(
-            ctypes.byref(layout), q.data_ptr(), q.stride(0), q.stride(1), int(q.shape[0]), max_query_len,
-            query_start_loc.data_ptr(), bounds.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), num_selected,
-            sink_blocks, recent_blocks, block_list.data_ptr(), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _ptr(status), _stream()), "select_blocks")
+            ref, q.data_ptr(), q.stride(0), q.stride(1), q.shape[0], max_query_len, p_start, p_bounds, p_table, p_lens,
+            num_selected, sink_blocks, recent_blocks, p_list, p_ws, ws_bytes, p_status, _raw_stream(index)), "select_blocks")
     return block_list
+
+
+def select_blocks_workspace_bytes(layout: PagedLayout) -> int:
+    """Bytes of workspace :func:`select_blocks` needs."""
+    return int(_native.load().triattn_select_blocks_workspace_bytes(ctypes.byref(layout)))
