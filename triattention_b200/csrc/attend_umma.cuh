@@ -3,19 +3,19 @@
 // A row tile is NT x 128 query rows of one KV head; token tiles of 128 come in through the producers of attend_tma.cuh, K and
 // V in rings of their own (K is left earlier).  Per token tile and 128 rows:
 //   S = Q K^T      tcgen05.mma M 128, N 128, both operands K-major in shared memory, S in tensor memory,
-//   softmax        one thread per row: 128 logits from tensor memory, running maximum and sum, P = exp2(..) as bf16
-//                  back into the columns of S,
+//   softmax        two threads per row, 64 logits each from tensor memory; P = exp2(..) as bf16 back into the columns of S
+//                  (each thread the first half of its own),
 //   O += P V       A operand P from tensor memory, B operand V as it lies in the cache (channels contiguous), O in
 //                  tensor memory for the whole segment.
 // N = 128 because the A operand is read again for every product: at N = 64 the reads of Q, 4 KB per product, take longer than the
 // product (measured: the issuing warp spent 65 cycles on each of 16 products a tile).
 // NT = 2 (more than 128 rows): two groups of softmax threads share every K/V tile and take turns with the tensor cores,
-// P V and the next S of one group running while the other group is at its exponentials.  NT = 1: S has two buffers, and S of tile i
+// P V and the next S of one group running while the other group is at its exponentials.  (One thread per row: a group took 2500
+// cycles for a tile's softmax, two and a half times what its exponentials cost, and the turns did not overlap.)  NT = 1: S has two buffers, and S of tile i
 // is issued before P V of tile i - 1.
 // A row's exponentials are taken against the maximum of the first logits it saw, which is raised only when a logit exceeds
 // it by more than 2^64: P, the sums and O stay inside the range of bf16 and fp32 (2^127), and their precision is relative, so a
-// stale reference costs no accuracy.  That leaves one pass over a tile's logits; the rare raise rescales what the
-// row has accumulated, in its own thread.
+// stale reference costs no accuracy.  The rare raise rescales what the row has accumulated, in its own threads.
 #pragma once
 
 #include "attend_tma.cuh"
@@ -25,11 +25,11 @@ namespace triattn {
 
 constexpr int kTreeTile = 128;
 template <int D, int NT>
-constexpr int kTreeStages = (NT == 1 ? 3 : 2) * (128 / D);  // of K and of V: 96 or 64 KB each
+constexpr int kTreeStages = 2 * (128 / D);  // of K and of V: 64 KB each
 constexpr float kTreeSlack = 64.f;  // log2 of how far a row's exponentials may exceed 1
 
 template <int NT>
-constexpr int kTreeThreads = NT * 128 + 96;  // softmax groups, MMA warp, K and V producers
+constexpr int kTreeThreads = NT * 256 + 96;  // softmax groups, MMA warp, K and V producers
 template <int D, int NT>
 constexpr size_t tree_smem_bytes() {
   return 1024 + (size_t)kTreeStages<D, NT> * 2 * kTreeTile * D * 2 + (size_t)NT * 128 * D * 2;
@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     attend_tree_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,
                        const __grid_constant__ CUtensorMap vmap, const int runs) {
   constexpr int TILE = kTreeTile, STAGES = kTreeStages<D, NT>, THREADS = kTreeThreads<NT>, ROWS = 128 * NT;
-  constexpr int MMA_WARP = NT * 4;
+  constexpr int MMA_WARP = NT * 8;
   constexpr int SB = NT == 1 ? 2 : 1;            // S buffers per group
   constexpr uint32_t kTileBytes = TILE * D * 2;
   constexpr uint32_t kGroup = D * 16;            // bytes of 8 tokens
@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   __shared__ long long red[THREADS / 32];
   __shared__ long long found[2];
   __shared__ uint32_t s_tmem;
+  __shared__ float pair_val[2][NT][2][128];  // what the two threads of a row tell each other (tiles in turn)
   __shared__ int odd_piece;  // the last piece in which a query token's value held an infinity or NaN
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
@@ -129,10 +130,10 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     for (int g = 0; g < NT; ++g) {
       for (int x = 0; x < SB; ++x) {
         mbar_init(smem_u32(&s_full[g][x]), 1);
-        mbar_init(smem_u32(&p_ready[g][x]), 4);
+        mbar_init(smem_u32(&p_ready[g][x]), 8);
         mbar_init(smem_u32(&o_done[g][x]), 1);
       }
-      mbar_init(smem_u32(&q_ready[g]), 4);
+      mbar_init(smem_u32(&q_ready[g]), 8);
     }
     mbar_init(smem_u32(&drained), 1);
     mbar_fence_init();
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       {
 #pragma unroll
         for (int k = 0; k < TILE / 16; ++k)
-          umma_bf16_ts(tmem + o_col + g * D, pa + k * 8, dv + (uint64_t)((k * 2 * kGroup) >> 4), kIdescO, in_piece > 0 || k > 0 ? 1u : 0u);
+          umma_bf16_ts(tmem + o_col + g * D, pa + (k & 3) * 8 + (k >> 2) * 64, dv + (uint64_t)((k * 2 * kGroup) >> 4), kIdescO, in_piece > 0 || k > 0 ? 1u : 0u);
         umma_commit(smem_u32(&o_done[g][i % SB]));
         if (g == NT - 1) umma_commit(smem_u32(&ring.empty[1][s]));
       }
@@ -240,18 +241,21 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------------------------------------ softmax
-    const int g = wid >> 2, row = tid & 127;
+    const int g = wid >> 3, half = (wid >> 2) & 1, row = tid & 127;
     const uint32_t lanes = (uint32_t)((wid & 3) * 32) << 16;
     const uint32_t t_o = tmem + lanes + o_col + g * D;
+    // the two warps that share these 32 rows
+    auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + g * 4 + (wid & 3)) : "memory"); };
     bool ok = true;
-    auto load_q = [&](const AttendCursor& at) {  // this thread's row of the operand
+    auto load_q = [&](const AttendCursor& at) {  // this thread's half row of the operand
       const int r = at.rt * ROWS + g * 128 + row;
       const bool there = r < at.r.n * p.g;
       const int i = there ? r / p.g : 0, j = there ? r - i * p.g : 0;
       const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(at.r.q0 + i) * p.q_ts + (long long)(at.h * p.g + j) * p.q_hs);
       unsigned char* dst = base_ptr + (q_base - base) + g * kQBytes + row * 128;
 #pragma unroll
-      for (int x = 0; x < D / 8; ++x) {
+      for (int y = 0; y < D / 16; ++y) {
+        const int x = half * (D / 16) + y;
         const uint4 w = there ? src[x] : make_uint4(0u, 0u, 0u, 0u);
         *reinterpret_cast<uint4*>(dst + (x >> 3) * 16384 + (((x & 7) ^ (row & 7)) << 4)) = w;
       }
@@ -296,64 +300,62 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
           edge = low_pos < 0 || top_pos + 8 > ctx;
         }
         if (!idle) {
-          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
-          float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
-          uint32_t sv[2][32];
-          tmem_ld32(t_s, sv[0]);
-#pragma unroll
-          for (int q = 0; q < TILE / 32; ++q) {
-            uint32_t(&s32)[32] = sv[q & 1];
-            tmem_ld_wait32(s32);
-            if (q + 1 < TILE / 32) tmem_ld32(t_s + (q + 1) * 32, sv[(q + 1) & 1]);
-            if (edge) {  // hidden tokens
+          // 32 of this thread's 64 logits; hidden tokens are -inf
+          auto logits = [&](int q, uint32_t (&sv)[32]) {
+            tmem_ld32(t_s + half * 64 + q * 32, sv);
+            tmem_ld_wait32(sv);
+            if (edge) {
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
-                const int q8 = pos8[q * 4 + (j >> 3)], pos = q8 + (j & 7), d = pos - ctx;
+                const int q8 = pos8[half * 8 + q * 4 + (j >> 3)], pos = q8 + (j & 7), d = pos - ctx;
                 const bool sees = q8 >= 0 && pos < c.r.T && (d < 0 || ((word >> d) & 1ull));
-                if (!sees) s32[j] = 0xff800000u;
+                if (!sees) sv[j] = 0xff800000u;
               }
             }
-            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          };
+          auto maximum = [](const uint32_t (&sv)[32]) {
+            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(s32[j]));
-            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
-            const bool raise = mx > m + kTreeSlack;  // (also the first finite one)
-            if (__any_sync(0xffffffffu, raise)) {
-              const float mn = raise ? mx : m;
-              const float f = raise ? ex2(m - mn) : 1.f;
-              l *= f;
-              la.x *= f, la.y *= f, lb.x *= f, lb.y *= f;
-              m = mn;
-              if (q > 0) {  // this tile's P so far
-                for (int y = 0; y < q; ++y) {
-                  uint32_t pv[16];
-                  tmem_ld16(t_s + y * 16, pv);
-                  tmem_ld_wait();
+            for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(sv[j]));
+            return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          };
+          // (96 registers per thread with two groups: the logits are read again for the exponentials)
+          uint32_t sv[NT == 1 ? 2 : 1][32];
+          logits(0, sv[0]);
+          float mx = maximum(sv[0]);
+          logits(1, sv[NT == 1 ? 1 : 0]);
+          mx = fmaxf(mx, maximum(sv[NT == 1 ? 1 : 0]));
+          pair_val[n & 1][g][half][row] = mx;
+          pair_sync();
+          mx = fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]) * p.scale_log2;
+          const bool raise = mx > m + kTreeSlack;  // (also the first finite one); the same for both threads
+          if (__any_sync(0xffffffffu, raise)) {
+            const float mn = raise ? mx : m;
+            const float f = raise ? ex2(m - mn) : 1.f;
+            l *= f;
+            m = mn;
+            if (x > 0) {  // the accumulator, after P V of the tile before; each thread half of the channels
+              if (SB > 1 && !wait_o(n - 1)) ok = false;
+              tc_fence_after();
+              for (int y = 0; y < D / 32; ++y) {
+                uint32_t ov[16];
+                tmem_ld16(t_o + half * (D / 2) + y * 16, ov);
+                tmem_ld_wait();
 #pragma unroll
-                  for (int j = 0; j < 16; ++j) {
-                    const float2 e = bf16x2_to_float2(pv[j]);
-                    pv[j] = pack_bf16(e.x * f, e.y * f);
-                  }
-                  tmem_st16(t_s + y * 16, pv);
-                }
-              }
-              if (x > 0) {  // the accumulator, after P V of the tile before
-                if (SB > 1 && !wait_o(n - 1)) ok = false;
-                tc_fence_after();
-                for (int y = 0; y < D / 16; ++y) {
-                  uint32_t ov[16];
-                  tmem_ld16(t_o + y * 16, ov);
-                  tmem_ld_wait();
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
-                  tmem_st16(t_o + y * 16, ov);
-                }
+                for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
+                tmem_st16(t_o + half * (D / 2) + y * 16, ov);
               }
               tmem_st_wait();
             }
-            const float mbase = m == -INFINITY ? 0.f : m;
-            const float2 mb2 = make_float2(-mbase, -mbase);
+          }
+          const float mbase = m == -INFINITY ? 0.f : m;
+          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mb2 = make_float2(-mbase, -mbase);
+          float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
             uint32_t pv[16];
+            uint32_t(&s32)[32] = sv[NT == 1 ? q : 0];
+            if (NT > 1) logits(q, s32);
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               float2 e = ffma2(make_float2(__uint_as_float(s32[2 * j]), __uint_as_float(s32[2 * j + 1])), sc2, mb2);
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
               else la = fadd2(la, e);
               pv[j] = pack_bf16(e.x, e.y);
             }
-            tmem_st16(t_s + q * 16, pv);  // columns of logits that have been read
+            tmem_st16(t_s + half * 64 + q * 16, pv);  // columns of its own logits, which have been read
           }
           la = fadd2(la, lb);
           l += la.x + la.y;
@@ -372,11 +374,11 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         if (edge && g == 0) {
           // values of tokens that are not there are zero; infinities and NaN in values of the query's own tokens are zero in the
           // product and reach the rows that see them when the piece is written (a hidden one would reach a row as 0 * inf)
-          const int q8 = pos8[row >> 3], pos = q8 + (row & 7);  // one token per thread
+          const int q8 = pos8[row >> 3], pos = q8 + (row & 7);  // half a token per thread
           const bool out = q8 < 0 || pos >= c.r.T;
           if (out || pos >= ctx) {
 #pragma unroll 4
-            for (int q = 0; q < D / 8; ++q) {
+            for (int q = half * (D / 16); q < (half + 1) * (D / 16); ++q) {
               uint4* v = reinterpret_cast<uint4*>(base_ptr + (v_base - base) + (uint32_t)s * kTileBytes + swz_off<D>(row, q));
               if (out) {
                 *v = make_uint4(0u, 0u, 0u, 0u);
@@ -408,6 +410,11 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         load_q(c);
       }
       if (idle) continue;
+      pair_sync();  // the last exchange has been read
+      pair_val[0][g][half][row] = l;
+      pair_sync();
+      l += pair_val[0][g][half ^ 1][row];
+      pair_sync();  // read before the next one
       const bool whole = t_begin == 0 && piece == done.r.tiles;
       const int slot = 2 * (int)blockIdx.x + (t_begin > 0 ? 0 : 1);
       const int i = there ? r / p.g : 0, hq = done.h * p.g + (there ? r - i * p.g : 0);
@@ -416,10 +423,11 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       uint16_t* dst = p.out + (long long)(done.r.q0 + i) * p.o_ts + (long long)hq * p.o_hs;
       float* part = p.part_o + ((long long)slot * ROWS + g * 128 + row) * D;
 #pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
+      for (int y = 0; y < D / 64; ++y) {  // this thread's half of the channels
+        const int q = half * (D / 64) + y;
         uint32_t ov[32];
         tmem_ld32(t_o + q * 32, ov);
-        tmem_ld_wait();
+        tmem_ld_wait32(ov);
         if (odd && there) {
           const int lo = t_begin * TILE, hi = min((t_begin + piece) * TILE, done.r.vlen);
           for (int vp = p.block_list == nullptr ? max(lo, ctx) : lo; vp < hi; ++vp) {
@@ -449,8 +457,8 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
             *reinterpret_cast<uint4*>(part + q * 32 + j) = make_uint4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
         }
       }
-      if (there && whole) p.lse[(long long)(done.r.q0 + i) * (p.Hkv * p.g) + hq] = (m + log2f(l)) * kLn2;
-      if (there && !whole)
+      if (there && whole && half == 0) p.lse[(long long)(done.r.q0 + i) * (p.Hkv * p.g) + hq] = (m + log2f(l)) * kLn2;
+      if (there && !whole && half == 0)
         *reinterpret_cast<float2*>(p.part_ml + ((long long)slot * ROWS + g * 128 + row) * 2) = make_float2(m, l);
       tc_fence_before();  // the accumulator has been read: the next piece's first P V (after this warp's next arrival) may overwrite it
     }
