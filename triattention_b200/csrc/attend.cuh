@@ -107,8 +107,14 @@ __device__ __forceinline__ long long attend_work_before(const AttendParams& p, i
 __device__ __forceinline__ int attend_runs(int runs, long long W, int min_tiles) {
   return (int)min((long long)runs, (W + min_tiles - 1) / min_tiles);
 }
-// first tile of run j of J over W >= J tiles (every run has one at least), and the run that owns a tile
-__device__ __forceinline__ long long attend_first_tile(long long W, int J, int j) { return W * j / J; }
+// first tile of run j of J over W >= J tiles, floor(W j / J) (every run has one at least), and the run that owns a tile
+__device__ __forceinline__ long long attend_first_tile(long long W, int J, int j) {
+  if (W < (1ll << 31)) {  // 32-bit divisions
+    const unsigned w = (unsigned)W, q = w / (unsigned)J, r = w - q * (unsigned)J;
+    return (long long)q * j + (r * (unsigned)j) / (unsigned)J;  // r j < J^2
+  }
+  return W * j / J;
+}
 __device__ __forceinline__ int attend_owner(long long W, int J, long long tile) {
   return (int)(((tile + 1) * J - 1) / W);
 }
@@ -119,19 +125,29 @@ struct AttendCursor {
   int b, h, rt, t;
 };
 
-// The cursor (but for its head) of tile `at`.  All threads call it; `found` and `red` are shared memory.
+// Shared memory of attend_plan_run.
 template <int THREADS>
-__device__ __forceinline__ void attend_seek(const AttendParams& p, long long at, int tile, int rows_per_tile,
-                                            long long* red, long long* found, AttendCursor& c) {
+struct AttendPlanShared {
+  long long warp_sum[THREADS / 32], at;
+  AttendReq req;
+  int b;
+};
+
+// Where run `run` (at most `runs`) of the call starts, and how many tiles it has; false: there is no such run.  All threads
+// call it; bad metadata is reported by run 0 of head 0.  A request per thread and pass; up to THREADS requests are read once.
+template <int THREADS>
+__device__ __forceinline__ bool attend_plan_run(const AttendParams& p, int runs, int min_tiles, int run, int tile,
+                                                int rows_per_tile, AttendPlanShared<THREADS>& sh, AttendCursor& c, int& count) {
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   unsigned err = 0u;
-  long long base = 0;
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
-    const int b = b0 + threadIdx.x;
+  AttendReq mine{};
+  long long before = 0, W = 0;  // tiles before this thread's request of the pass, tiles of all passes
+  auto pass = [&](int b0) {
     long long w = 0;
-    if (b < p.B) {
-      const AttendReq r = attend_req(p, b, tile, rows_per_tile, err);
-      w = (long long)r.tiles * r.row_tiles;
+    mine.tiles = mine.row_tiles = 0;
+    if (b0 + tid < p.B) {
+      mine = attend_req(p, b0 + tid, tile, rows_per_tile, err);
+      w = (long long)mine.tiles * mine.row_tiles;
     }
     long long incl = w;
 #pragma unroll
@@ -139,28 +155,47 @@ __device__ __forceinline__ void attend_seek(const AttendParams& p, long long at,
       const long long u = __shfl_up_sync(0xffffffffu, incl, s);
       if (lane >= s) incl += u;
     }
-    if (lane == 31) red[wid] = incl;
+    if (lane == 31) sh.warp_sum[wid] = incl;
     __syncthreads();
-    long long before = base, total = 0;
+    before = incl - w;
+    long long total = 0;
 #pragma unroll
     for (int x = 0; x < THREADS / 32; ++x) {
-      if (x < wid) before += red[x];
-      total += red[x];
+      const long long u = sh.warp_sum[x];
+      if (x < wid) before += u;
+      total += u;
     }
-    before += incl - w;
-    if (at >= before && at < before + w) {
-      found[0] = b;
-      found[1] = at - before;
+    return total;
+  };
+  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+    if (b0 > 0) __syncthreads();
+    W += pass(b0);
+  }
+  if (blockIdx.x == 0 && err) flag_status(p.status, err);
+  const int J = attend_runs(runs, W, min_tiles);
+  if (run >= J) return false;
+  const long long first = attend_first_tile(W, J, run);
+  count = (int)(attend_first_tile(W, J, run + 1) - first);
+  long long base = 0;
+  for (int b0 = 0; b0 < p.B; b0 += THREADS) {
+    if (p.B > THREADS) {
+      __syncthreads();
+      const long long total = pass(b0);
+      before += base;
+      base += total;
     }
-    __syncthreads();
-    if (at < base + total) break;
-    base += total;
+    if (first >= before && first < before + (long long)mine.tiles * mine.row_tiles) {
+      sh.at = first - before;
+      sh.req = mine;
+      sh.b = b0 + tid;
+    }
   }
   __syncthreads();
-  c.b = (int)found[0];
-  c.r = attend_req(p, c.b, tile, rows_per_tile, err);
-  c.rt = (int)(found[1] / c.r.tiles);
-  c.t = (int)(found[1] - (long long)c.rt * c.r.tiles);
+  c.r = sh.req;
+  c.b = sh.b;
+  c.rt = (int)((unsigned long long)sh.at / (unsigned)c.r.tiles);
+  c.t = (int)(sh.at - (long long)c.rt * c.r.tiles);
+  return true;
 }
 
 __device__ __forceinline__ void attend_advance(const AttendParams& p, AttendCursor& c, int tile, int rows_per_tile) {
@@ -304,8 +339,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int kpos[kStages][kAttendTile];
   __shared__ int bad_tile[kStages];
-  __shared__ long long red[kAttendThreads / 32];
-  __shared__ long long found[2];
+  __shared__ AttendPlanShared<kAttendThreads> plan;
   __shared__ float join_ml[4][16][2];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   const int wr = wid % MT, wk = wid / MT;
@@ -313,18 +347,13 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
   grid_dependency_wait();
   trigger_dependents();
   unsigned err = 0u;
-  const long long W = attend_work_before<kAttendThreads>(p, p.B, kAttendTile, ROWS, err, red);
-  if (blockIdx.x == 0 && err) flag_status(p.status, err);
-  err = 0u;
-  const int J = attend_runs(runs, W, p.min_tiles), run = (int)blockIdx.x / p.Hkv;
-  if (run >= J) return;
-  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
-  if (tid < kStages) bad_tile[tid] = -1;
+  const int run = (int)blockIdx.x / p.Hkv;
   AttendCursor lc;  // loads
-  attend_seek<kAttendThreads>(p, first, kAttendTile, ROWS, red, found, lc);
+  int count;
+  if (tid < kStages) bad_tile[tid] = -1;
+  if (!attend_plan_run<kAttendThreads>(p, runs, p.min_tiles, run, kAttendTile, ROWS, plan, lc, count)) return;
   lc.h = (int)blockIdx.x - run * p.Hkv;
   AttendCursor c = lc;  // arithmetic
-  const int count = (int)(last - first);
 
   const uint32_t stage0 = smem_u32(smem);
   constexpr uint32_t kStage = kAttendStageBytes<D>;
@@ -766,22 +795,18 @@ __global__ void __launch_bounds__(kAttendThreads) attend_observe_kernel(const __
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int kpos[kStages][kAttendTile];
   __shared__ long long kadr[kStages][kAttendTile];  // index of the token's sum
-  __shared__ long long red[kAttendThreads / 32];
-  __shared__ long long found[2];
+  __shared__ AttendPlanShared<kAttendThreads> plan;
   __shared__ float lse2[kObserveRows];
   __shared__ unsigned long long words[kObserveRows];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
   grid_dependency_wait();
   unsigned err = 0u;
-  const long long W = attend_work_before<kAttendThreads>(p, p.B, kAttendTile, kAll, err, red);
-  const int J = attend_runs(runs, W, 1), run = (int)blockIdx.x / p.Hkv;
-  if (run >= J) return;
-  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
+  const int run = (int)blockIdx.x / p.Hkv;
   AttendCursor lc;
-  attend_seek<kAttendThreads>(p, first, kAttendTile, kAll, red, found, lc);
+  int count;
+  if (!attend_plan_run<kAttendThreads>(p, runs, 1, run, kAttendTile, kAll, plan, lc, count)) return;
   lc.h = (int)blockIdx.x - run * p.Hkv;
   AttendCursor c = lc;
-  const int count = (int)(last - first);
   const uint32_t stage0 = smem_u32(smem);
   constexpr uint32_t kStage = kAttendStageBytes<D>;
   unsigned char* q_smem = smem + kStages * kStage;

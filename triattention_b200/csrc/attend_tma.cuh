@@ -183,8 +183,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   constexpr bool kAllAtOnce = SPLIT_P && D <= 128;  // join scratch for every warp, or one shared and taken in turn
   extern __shared__ unsigned char smem_raw[];
   __shared__ AttendRing<TILE, STAGES> ring;
-  __shared__ long long red[kDecodeThreads / 32];
-  __shared__ long long found[2];
+  __shared__ AttendPlanShared<kDecodeThreads> plan;
   __shared__ float join_ml[WARPS][16][2];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
@@ -198,16 +197,11 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   }
   grid_dependency_wait();
   trigger_dependents();
-  unsigned err = 0u;
-  const long long W = attend_work_before<kDecodeThreads>(p, p.B, TILE, ROWS, err, red);
-  if (blockIdx.x == 0 && err) flag_status(p.status, err);
-  const int J = attend_runs(runs, W, p.min_tiles), run = (int)blockIdx.x / p.Hkv;
-  if (run >= J) return;
-  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
+  const int run = (int)blockIdx.x / p.Hkv;
   AttendCursor c;
-  attend_seek<kDecodeThreads>(p, first, TILE, ROWS, red, found, c);
+  int count;
+  if (!attend_plan_run<kDecodeThreads>(p, runs, p.min_tiles, run, TILE, ROWS, plan, c, count)) return;
   c.h = (int)blockIdx.x - run * p.Hkv;
-  const int count = (int)(last - first);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* const base_ptr = smem_raw + (base - smem_u32(smem_raw));
   float* const join = reinterpret_cast<float*>(base_ptr + STAGES * 2 * kTileBytes);
@@ -518,8 +512,7 @@ __global__ void __launch_bounds__(kObserveThreads, 1)
   constexpr uint32_t kTileBytes = TILE * D * 2;
   extern __shared__ unsigned char smem_raw[];
   __shared__ AttendRing<TILE, STAGES, true> ring;
-  __shared__ long long red[THREADS / 32];
-  __shared__ long long found[2];
+  __shared__ AttendPlanShared<THREADS> plan;
   __shared__ float lse2[RMAX];
   __shared__ unsigned long long words[RMAX];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
@@ -533,15 +526,11 @@ __global__ void __launch_bounds__(kObserveThreads, 1)
   }
   grid_dependency_wait();
   trigger_dependents();
-  unsigned err = 0u;
-  const long long W = attend_work_before<THREADS>(p, p.B, TILE, kAll, err, red);
-  const int J = attend_runs(runs, W, WARPS), run = (int)blockIdx.x / p.Hkv;
-  if (run >= J) return;
-  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
+  const int run = (int)blockIdx.x / p.Hkv;
   AttendCursor c;
-  attend_seek<THREADS>(p, first, TILE, kAll, red, found, c);
+  int count;
+  if (!attend_plan_run<THREADS>(p, runs, WARPS, run, TILE, kAll, plan, c, count)) return;
   c.h = (int)blockIdx.x - run * p.Hkv;
-  const int count = (int)(last - first);
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* const q_smem = smem_raw + (base - smem_u32(smem_raw)) + STAGES * kTileBytes;
   const uint32_t q_base = base + STAGES * kTileBytes;

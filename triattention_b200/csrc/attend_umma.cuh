@@ -114,8 +114,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   // per group and S buffer: S is there, P is there, P V is over
   __shared__ uint64_t s_full[NT][SB], p_ready[NT][SB], o_done[NT][SB];
   __shared__ uint64_t q_ready[NT], drained;
-  __shared__ long long red[THREADS / 32];
-  __shared__ long long found[2];
+  __shared__ AttendPlanShared<THREADS> plan;
   __shared__ uint32_t s_tmem;
   __shared__ float pair_val[2][NT][2][128];  // what the two threads of a row tell each other (tiles in turn)
   __shared__ int odd_piece;  // the last piece in which a query token's value held an infinity or NaN
@@ -143,19 +142,15 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   grid_dependency_wait();
   trigger_dependents();
   unsigned err = 0u;
-  const long long W = attend_work_before<THREADS>(p, p.B, TILE, ROWS, err, red);
-  if (blockIdx.x == 0 && err) flag_status(p.status, err);
-  const int J = attend_runs(runs, W, p.min_tiles), run = (int)blockIdx.x / p.Hkv;
-  if (run >= J) return;  // nothing allocated yet
-  const long long first = attend_first_tile(W, J, run), last = attend_first_tile(W, J, run + 1);
+  const int run = (int)blockIdx.x / p.Hkv;
   AttendCursor c;
+  int count;
+  if (!attend_plan_run<THREADS>(p, runs, p.min_tiles, run, TILE, ROWS, plan, c, count)) return;  // nothing allocated yet
+  c.h = (int)blockIdx.x - run * p.Hkv;
   if (wid == MMA_WARP) {
     tmem_alloc(smem_u32(&s_tmem), kCols);
     tmem_relinquish();
   }
-  attend_seek<THREADS>(p, first, TILE, ROWS, red, found, c);
-  c.h = (int)blockIdx.x - run * p.Hkv;
-  const int count = (int)(last - first);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -246,18 +241,21 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     const uint32_t t_o = tmem + lanes + o_col + g * D;
     // the two warps that share these 32 rows
     auto pair_sync = [&]() { asm volatile("bar.sync %0, 64;" ::"r"(2 + g * 4 + (wid & 3)) : "memory"); };
-    bool ok = true;
-    auto load_q = [&](const AttendCursor& at) {  // this thread's half row of the operand
-      const int r = at.rt * ROWS + g * 128 + row;
-      const bool there = r < at.r.n * p.g;
-      const int i = there ? r / p.g : 0, j = there ? r - i * p.g : 0;
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + (long long)(at.r.q0 + i) * p.q_ts + (long long)(at.h * p.g + j) * p.q_hs);
-      unsigned char* dst = base_ptr + (q_base - base) + g * kQBytes + row * 128;
-#pragma unroll
-      for (int y = 0; y < D / 16; ++y) {
-        const int x = half * (D / 16) + y;
-        const uint4 w = there ? src[x] : make_uint4(0u, 0u, 0u, 0u);
-        *reinterpret_cast<uint4*>(dst + (x >> 3) * 16384 + (((x & 7) ^ (row & 7)) << 4)) = w;
+    // A wait that runs out ends the work but not the control flow: a warp that left would strand its partner at a barrier.
+    bool dead = false;
+    auto load_q = [&](const AttendCursor& at) {  // the pair's 32 rows of the operand, half of them per warp; D / 8 lanes to a row
+      const int rows0 = at.rt * ROWS + g * 128, pc = lane % (D / 8);
+      unsigned char* dst = base_ptr + (q_base - base) + g * kQBytes;
+#pragma unroll 4
+      for (int y = 0; y < D / 16; ++y) {  // 256 / D rows at a time
+        const int rr = (wid & 3) * 32 + half * 16 + y * (256 / D) + lane / (D / 8);
+        const int r = rows0 + rr;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (r < at.r.n * p.g) {
+          const int i = r / p.g, j = r - i * p.g;
+          w = *reinterpret_cast<const uint4*>(p.q + (long long)(at.r.q0 + i) * p.q_ts + (long long)(at.h * p.g + j) * p.q_hs + pc * 8);
+        }
+        *reinterpret_cast<uint4*>(dst + rr * 128 + (pc >> 3) * 16384 + (((pc & 7) ^ (rr & 7)) << 4)) = w;
       }
       fence_proxy_async();
       __syncwarp();
@@ -269,7 +267,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     auto wait_o = [&](int k) { return ring_wait(o_done[g][k % SB], (uint32_t)(k / SB) & 1u, &ring.err, p.status); };
     load_q(c);
     int piece_no = 0;
-    for (int it = 0; it < count && ok; ++piece_no) {
+    for (int it = 0; it < count; ++piece_no) {
       const int t_begin = c.t, piece = min(c.r.tiles - c.t, count - it);
       const int R = c.r.n * p.g, ctx = c.r.T - c.r.n;
       const int r = c.rt * ROWS + g * 128 + row;
@@ -280,16 +278,14 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       for (int x = 0; x < piece; ++x) {
         const int n = it + x, s = n % STAGES;
         const uint32_t t_s = tmem + lanes + (uint32_t)(g * SB + n % SB) * 128u;
-        ok = ring_wait(s_full[g][n % SB], (uint32_t)(n / SB) & 1u, &ring.err, p.status);
-        if (!ok) break;
+        dead = dead || !ring_wait(s_full[g][n % SB], (uint32_t)(n / SB) & 1u, &ring.err, p.status);
         tc_fence_after();
         // tiles that reach the query's own tokens, the end, or a run of tokens that is not there
         const int* pos8 = ring.pos[n % kPosRing<TILE>];
         bool edge = false;
-        if (p.block_list != nullptr || (t_begin + x + 1) * TILE > ctx || *(volatile int*)&ring.gaps != 0) {
+        if (!dead && (p.block_list != nullptr || (t_begin + x + 1) * TILE > ctx || *(volatile int*)&ring.gaps != 0)) {
           // positions and values are read here: wait for the tile itself (V stays until this thread's P has been used)
-          ok = ring_wait(ring.full[1][s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status);
-          if (!ok) break;
+          dead = !ring_wait(ring.full[1][s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status);
           int top_pos = -1, low_pos = 1;
 #pragma unroll
           for (int j = 0; j < TILE / 8; ++j) {
@@ -299,18 +295,37 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
           }
           edge = low_pos < 0 || top_pos + 8 > ctx;
         }
+        if (dead) {
+          if (!idle) pair_sync();
+          continue;
+        }
         if (!idle) {
-          // 32 of this thread's 64 logits; hidden tokens are -inf
+          // which of this thread's 64 tokens its row sees (the code of the loop is kept small: with the tests spelled out per logit
+          // the instruction cache missed, and a tile took a tenth longer)
+          uint32_t sees[2] = {0xffffffffu, 0xffffffffu};
+          if (edge) {
+#pragma unroll 1
+            for (int j = 0; j < 8; ++j) {
+              const int q8 = pos8[half * 8 + j];
+              uint32_t bits = 0u;  // of a run of 8 tokens
+              if (q8 >= 0) {
+                const int d = q8 - ctx;  // its first token's place among the query's own
+                const unsigned long long own = d >= 0 ? word >> d : (word << -max(d, -8)) | ((1ull << -max(d, -8)) - 1ull);
+                bits = (uint32_t)own & (q8 + 8 <= c.r.T ? 0xffu : (1u << (c.r.T - q8 > 0 ? c.r.T - q8 : 0)) - 1u);
+              }
+              const uint32_t at = (uint32_t)(j & 3) * 8u;
+              if (j < 4) sees[0] = (sees[0] & ~(0xffu << at)) | (bits & 0xffu) << at;
+              else sees[1] = (sees[1] & ~(0xffu << at)) | (bits & 0xffu) << at;
+            }
+          }
+          // 32 of the logits; hidden tokens are -inf
           auto logits = [&](int q, uint32_t (&sv)[32]) {
             tmem_ld32(t_s + half * 64 + q * 32, sv);
             tmem_ld_wait32(sv);
             if (edge) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                const int q8 = pos8[half * 8 + q * 4 + (j >> 3)], pos = q8 + (j & 7), d = pos - ctx;
-                const bool sees = q8 >= 0 && pos < c.r.T && (d < 0 || ((word >> d) & 1ull));
-                if (!sees) sv[j] = 0xff800000u;
-              }
+              for (int j = 0; j < 32; ++j)
+                if (!((sees[q] >> j) & 1u)) sv[j] = 0xff800000u;
             }
           };
           auto maximum = [](const uint32_t (&sv)[32]) {
@@ -335,8 +350,9 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
             l *= f;
             m = mn;
             if (x > 0) {  // the accumulator, after P V of the tile before; each thread half of the channels
-              if (SB > 1 && !wait_o(n - 1)) ok = false;
+              if (SB > 1) dead = !wait_o(n - 1);
               tc_fence_after();
+#pragma unroll 1
               for (int y = 0; y < D / 32; ++y) {
                 uint32_t ov[16];
                 tmem_ld16(t_o + half * (D / 2) + y * 16, ov);
@@ -377,7 +393,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
           const int q8 = pos8[row >> 3], pos = q8 + (row & 7);  // half a token per thread
           const bool out = q8 < 0 || pos >= c.r.T;
           if (out || pos >= ctx) {
-#pragma unroll 4
+#pragma unroll 1
             for (int q = half * (D / 16); q < (half + 1) * (D / 16); ++q) {
               uint4* v = reinterpret_cast<uint4*>(base_ptr + (v_base - base) + (uint32_t)s * kTileBytes + swz_off<D>(row, q));
               if (out) {
@@ -397,69 +413,81 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_ready[g][n % SB]));
       }
-      if (!ok) break;
-      ok = wait_o(it + piece - 1);
-      if (!ok) break;
+      dead = dead || !wait_o(it + piece - 1);
       tc_fence_after();
-      // the next segment's query rows first: S of its first tile does not wait for what follows
-      const AttendCursor done = c;
+      // ---- the piece is written; each thread holds half of the channels of its row.  A warp's 32 rows x 32 channels pass through
+      // the place of the (used) query operand, so that eight lanes write 128 consecutive bytes of a row
+      const bool whole = t_begin == 0 && piece == c.r.tiles;
+      if (!idle) {
+        pair_sync();  // the last exchange has been read
+        pair_val[0][g][half][row] = l;
+        pair_sync();
+        l += pair_val[0][g][half ^ 1][row];
+        pair_sync();  // read before the next one
+        const int slot = 2 * (int)blockIdx.x + (t_begin > 0 ? 0 : 1);
+        const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : l;  // a NaN sum stays one
+        const bool odd = *(volatile int*)&odd_piece == piece_no;
+        unsigned char* stage = base_ptr + (q_base - base) + wid * (16 * D * 2);  // 16 rows of the operand: 4 KB (D = 128)
+#pragma unroll 1
+        for (int y = 0; y < (dead ? 0 : D / 64); ++y) {
+          const int q = half * (D / 64) + y;
+          uint32_t ov[32];
+          tmem_ld32(t_o + q * 32, ov);
+          tmem_ld_wait32(ov);
+          if (odd && there) {
+            const int lo = t_begin * TILE, hi = min((t_begin + piece) * TILE, c.r.vlen);
+            for (int vp = p.block_list == nullptr ? max(lo, ctx) : lo; vp < hi; ++vp) {
+              const TokenAt at = attend_token(p, c, vp, err);
+              if (at.pos < ctx || !((word >> (at.pos - ctx)) & 1ull)) continue;
+              const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v + at.off) + q * 32;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float e = bf16_to_float(v[j]);
+                ov[j] = __float_as_uint(__uint_as_float(ov[j]) + (isfinite(e) ? 0.f : e));
+              }
+            }
+          }
+          // 2 KB at a time (16 channels per row): both head dimensions have room for that
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              *reinterpret_cast<float4*>(stage + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+                  make_float4(__uint_as_float(ov[z * 16 + 4 * j]) * inv, __uint_as_float(ov[z * 16 + 4 * j + 1]) * inv,
+                              __uint_as_float(ov[z * 16 + 4 * j + 2]) * inv, __uint_as_float(ov[z * 16 + 4 * j + 3]) * inv);
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {  // eight rows at a time, four lanes to a row
+              const int rr = k * 8 + (lane >> 2), at = c.rt * ROWS + g * 128 + (wid & 3) * 32 + rr;
+              const float4 e = *reinterpret_cast<const float4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+              const int col = q * 32 + z * 16 + (lane & 3) * 4;
+              if (at < R) {
+                if (whole) {
+                  const int i = at / p.g, hq = c.h * p.g + (at - i * p.g);
+                  *reinterpret_cast<uint2*>(p.out + (long long)(c.r.q0 + i) * p.o_ts + (long long)hq * p.o_hs + col) =
+                      make_uint2(pack_bf16(e.x, e.y), pack_bf16(e.z, e.w));
+                } else {
+                  *reinterpret_cast<float4*>(p.part_o + ((long long)slot * ROWS + at - c.rt * ROWS) * D + col) = e;
+                }
+              }
+            }
+            __syncwarp();
+          }
+        }
+        if (there && half == 0 && !dead) {
+          const int i = r / p.g, hq = c.h * p.g + (r - i * p.g);
+          if (whole) p.lse[(long long)(c.r.q0 + i) * (p.Hkv * p.g) + hq] = (m + log2f(l)) * kLn2;
+          else *reinterpret_cast<float2*>(p.part_ml + ((long long)slot * ROWS + g * 128 + row) * 2) = make_float2(m, l);
+        }
+      }
       it += piece;
       c.t += piece - 1;
       if (it < count) {
         attend_advance(p, c, TILE, ROWS);
+        // the group's warps share the operand's place: all of them are done staging
+        asm volatile("bar.sync %0, 256;" ::"r"(10 + g) : "memory");
         load_q(c);
       }
-      if (idle) continue;
-      pair_sync();  // the last exchange has been read
-      pair_val[0][g][half][row] = l;
-      pair_sync();
-      l += pair_val[0][g][half ^ 1][row];
-      pair_sync();  // read before the next one
-      const bool whole = t_begin == 0 && piece == done.r.tiles;
-      const int slot = 2 * (int)blockIdx.x + (t_begin > 0 ? 0 : 1);
-      const int i = there ? r / p.g : 0, hq = done.h * p.g + (there ? r - i * p.g : 0);
-      const float inv = l > 0.f ? 1.f / l : l;  // a NaN sum stays one
-      const bool odd = *(volatile int*)&odd_piece == piece_no;
-      uint16_t* dst = p.out + (long long)(done.r.q0 + i) * p.o_ts + (long long)hq * p.o_hs;
-      float* part = p.part_o + ((long long)slot * ROWS + g * 128 + row) * D;
-#pragma unroll
-      for (int y = 0; y < D / 64; ++y) {  // this thread's half of the channels
-        const int q = half * (D / 64) + y;
-        uint32_t ov[32];
-        tmem_ld32(t_o + q * 32, ov);
-        tmem_ld_wait32(ov);
-        if (odd && there) {
-          const int lo = t_begin * TILE, hi = min((t_begin + piece) * TILE, done.r.vlen);
-          for (int vp = p.block_list == nullptr ? max(lo, ctx) : lo; vp < hi; ++vp) {
-            const TokenAt at = attend_token(p, done, vp, err);
-            if (at.pos < ctx || !((word >> (at.pos - ctx)) & 1ull)) continue;
-            const uint16_t* v = reinterpret_cast<const uint16_t*>(p.v + at.off) + q * 32;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float e = bf16_to_float(v[j]);
-              if (!isfinite(e)) ov[j] = __float_as_uint(__uint_as_float(ov[j]) + e);
-            }
-          }
-        }
-        if (there && whole) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 8) {
-            uint4 w;
-            w.x = pack_bf16(__uint_as_float(ov[j]) * inv, __uint_as_float(ov[j + 1]) * inv);
-            w.y = pack_bf16(__uint_as_float(ov[j + 2]) * inv, __uint_as_float(ov[j + 3]) * inv);
-            w.z = pack_bf16(__uint_as_float(ov[j + 4]) * inv, __uint_as_float(ov[j + 5]) * inv);
-            w.w = pack_bf16(__uint_as_float(ov[j + 6]) * inv, __uint_as_float(ov[j + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + q * 32 + j) = w;
-          }
-        } else if (there) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<uint4*>(part + q * 32 + j) = make_uint4(ov[j], ov[j + 1], ov[j + 2], ov[j + 3]);
-        }
-      }
-      if (there && whole && half == 0) p.lse[(long long)(done.r.q0 + i) * (p.Hkv * p.g) + hq] = (m + log2f(l)) * kLn2;
-      if (there && !whole && half == 0)
-        *reinterpret_cast<float2*>(p.part_ml + ((long long)slot * ROWS + g * 128 + row) * 2) = make_float2(m, l);
       tc_fence_before();  // the accumulator has been read: the next piece's first P V (after this warp's next arrival) may overwrite it
     }
   }
