@@ -13,9 +13,11 @@
 // P V and the next S of one group running while the other group is at its exponentials.  (One thread per row: a group took 2500
 // cycles for a tile's softmax, two and a half times what its exponentials cost, and the turns did not overlap.)  NT = 1: S has two buffers, and S of tile i
 // is issued before P V of tile i - 1.
-// A row's exponentials are taken against the maximum of the first logits it saw, which is raised only when a logit exceeds
-// it by more than 2^64: P, the sums and O stay inside the range of bf16 and fp32 (2^127), and their precision is relative, so a
-// stale reference costs no accuracy.  The rare raise rescales what the row has accumulated, in its own threads.
+// A row's exponentials are taken against the maximum of the first tile it saw, which is raised only when the exponentials of
+// a later tile add up to more than 2^64: P, the sums and O stay inside the range of bf16 and fp32 (2^127), and their
+// precision is relative, so a stale reference costs no accuracy - and no tile's maximum is needed.  P goes to tensor memory, over
+// the logits, only when it is known to be in range; the rare raise starts from the logits again and rescales what the row has
+// accumulated, in its own threads.
 #pragma once
 
 #include "attend_tma.cuh"
@@ -26,7 +28,7 @@ namespace triattn {
 constexpr int kTreeTile = 128;
 template <int D, int NT>
 constexpr int kTreeStages = 2 * (128 / D);  // of K and of V: 64 KB each
-constexpr float kTreeSlack = 64.f;  // log2 of how far a row's exponentials may exceed 1
+constexpr float kTreeSlack = 18446744073709551616.f;  // 2^64: what a thread's exponentials of a tile may add up to
 
 template <int NT>
 constexpr int kTreeThreads = NT * 256 + 96;  // softmax groups, MMA warp, K and V producers
@@ -117,6 +119,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   __shared__ AttendPlanShared<THREADS> plan;
   __shared__ uint32_t s_tmem;
   __shared__ float pair_val[2][NT][2][128];  // what the two threads of a row tell each other (tiles in turn)
+  __shared__ bool pair_over[2][NT][2][4];
   __shared__ int odd_piece;  // the last piece in which a query token's value held an infinity or NaN
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
@@ -177,7 +180,6 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       const int s = i % STAGES;
       if (g == 0 && !thread_wait(ring.full[0][s], (uint32_t)(i / STAGES) & 1u, &ring.err, p.status)) return false;
       if (t_in_piece == 0 && !thread_wait(q_ready[g], (uint32_t)piece_no & 1u, &ring.err, p.status)) return false;
-      fence_proxy_async();
       tc_fence_after();
       const uint64_t dk = umma_desc(base + (uint32_t)s * kTileBytes, 16u, kGroup), dq = umma_desc(q_base + g * kQBytes, 16u, 1024u);
       {
@@ -194,7 +196,6 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       const int s = i % STAGES;
       if (g == 0 && !thread_wait(ring.full[1][s], (uint32_t)(i / STAGES) & 1u, &ring.err, p.status)) return false;
       if (!thread_wait(p_ready[g][i % SB], (uint32_t)(i / SB) & 1u, &ring.err, p.status)) return false;
-      fence_proxy_async();
       tc_fence_after();
       const uint32_t pa = tmem + (uint32_t)(g * SB + i % SB) * 128u;
       const uint64_t dv = umma_desc(v_base + (uint32_t)s * kTileBytes, 1024u, kGroup);
@@ -328,63 +329,70 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
                 if (!((sees[q] >> j) & 1u)) sv[j] = 0xff800000u;
             }
           };
-          auto maximum = [](const uint32_t (&sv)[32]) {
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(sv[j]));
-            return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-          };
-          // (96 registers per thread with two groups: the logits are read again for the exponentials)
-          uint32_t sv[NT == 1 ? 2 : 1][32];
-          logits(0, sv[0]);
-          float mx = maximum(sv[0]);
-          logits(1, sv[NT == 1 ? 1 : 0]);
-          mx = fmaxf(mx, maximum(sv[NT == 1 ? 1 : 0]));
-          pair_val[n & 1][g][half][row] = mx;
-          pair_sync();
-          mx = fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]) * p.scale_log2;
-          const bool raise = mx > m + kTreeSlack;  // (also the first finite one); the same for both threads
-          if (__any_sync(0xffffffffu, raise)) {
-            const float mn = raise ? mx : m;
-            const float f = raise ? ex2(m - mn) : 1.f;
-            l *= f;
-            m = mn;
-            if (x > 0) {  // the accumulator, after P V of the tile before; each thread half of the channels
-              if (SB > 1) dead = !wait_o(n - 1);
-              tc_fence_after();
+          uint32_t pv[2][16];  // P, kept until it is known to be in range: the logits stay where they are until then
+          float sum;
+          for (bool raise = x == 0;;) {
+            if (raise) {
+              // the reference becomes the maximum so far (of both threads); what the row has accumulated is rescaled
+              float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-              for (int y = 0; y < D / 32; ++y) {
-                uint32_t ov[16];
-                tmem_ld16(t_o + half * (D / 2) + y * 16, ov);
-                tmem_ld_wait();
+              for (int q = 0; q < 2; ++q) {
+                uint32_t sv[32];
+                logits(q, sv);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
-                tmem_st16(t_o + half * (D / 2) + y * 16, ov);
+                for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(sv[j]));
               }
-              tmem_st_wait();
-            }
-          }
-          const float mbase = m == -INFINITY ? 0.f : m;
-          const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mb2 = make_float2(-mbase, -mbase);
-          float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+              float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+              pair_val[n & 1][g][half][row] = mx;
+              pair_sync();
+              mx = fmaxf(m, fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]) * p.scale_log2);
+              const float f = mx > m ? ex2(m - mx) : 1.f;
+              l *= f;
+              m = mx;
+              if (x > 0) {  // the accumulator, after P V of the tile before; each thread half of the channels
+                if (SB > 1) dead = !wait_o(n - 1);
+                tc_fence_after();
+#pragma unroll 1
+                for (int y = 0; y < D / 32; ++y) {
+                  uint32_t ov[16];
+                  tmem_ld16(t_o + half * (D / 2) + y * 16, ov);
+                  tmem_ld_wait();
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t pv[16];
-            uint32_t(&s32)[32] = sv[NT == 1 ? q : 0];
-            if (NT > 1) logits(q, s32);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              float2 e = ffma2(make_float2(__uint_as_float(s32[2 * j]), __uint_as_float(s32[2 * j + 1])), sc2, mb2);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              if (j & 1) lb = fadd2(lb, e);
-              else la = fadd2(la, e);
-              pv[j] = pack_bf16(e.x, e.y);
+                  for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * f);
+                  tmem_st16(t_o + half * (D / 2) + y * 16, ov);
+                }
+                tmem_st_wait();
+              }
             }
-            tmem_st16(t_s + half * 64 + q * 16, pv);  // columns of its own logits, which have been read
+            const float mbase = m == -INFINITY ? 0.f : m;
+            const float2 sc2 = make_float2(p.scale_log2, p.scale_log2), mb2 = make_float2(-mbase, -mbase);
+            float2 la = make_float2(0.f, 0.f), lb = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t sv[32];
+              logits(q, sv);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                float2 e = ffma2(make_float2(__uint_as_float(sv[2 * j]), __uint_as_float(sv[2 * j + 1])), sc2, mb2);
+                e.x = ex2(e.x);
+                e.y = ex2(e.y);
+                if (j & 1) lb = fadd2(lb, e);
+                else la = fadd2(la, e);
+                pv[q][j] = pack_bf16(e.x, e.y);
+              }
+            }
+            la = fadd2(la, lb);
+            sum = la.x + la.y;
+            if (raise) break;  // nothing exceeds 1
+            const bool over = __any_sync(0xffffffffu, !(sum < kTreeSlack) || m == -INFINITY);
+            if (lane == 0) pair_over[n & 1][g][half][wid & 3] = over;
+            pair_sync();
+            if (!over && !pair_over[n & 1][g][half ^ 1][wid & 3]) break;
+            raise = true;
           }
-          la = fadd2(la, lb);
-          l += la.x + la.y;
+          l += sum;
+#pragma unroll
+          for (int q = 0; q < 2; ++q) tmem_st16(t_s + half * 64 + q * 16, pv[q]);  // columns of its own logits
           tmem_st_wait();
         }
         if (edge && g == 0) {
