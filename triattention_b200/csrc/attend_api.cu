@@ -66,7 +66,7 @@ AttendPlan attend_plan(const triattn_paged_layout& Y, int max_q, int num_listed)
   int ctas = kSMs;
   if (R <= 16 && tileable(Y)) {
     a.kind = AttendKind::kDecode;
-    a.tile = kDecodeTile;
+    a.tile = Y.head_dim == 64 ? kDecodeTile<64> : Y.head_dim == 128 ? kDecodeTile<128> : kDecodeTile<256>;
     a.rows = a.split_p ? 8 : 16;
     a.min_tiles = kDecodeWarps;
   } else if (tileable(Y) && Y.head_dim <= 128) {
@@ -165,7 +165,7 @@ int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensor
     if (!ensure_dynamic_smem<attend_observe_tiled_kernel<D>>(smem)) return TRIATTN_ERR_CUDA;
     for (int row0 = 0; row0 < p.max_q * p.g; row0 += kObserveTileRows<D>) {
       AttendParams o = p;
-      for (o.box = kDecodeTile; o.bs % o.box; o.box /= 2) {
+      for (o.box = kObserveTile<D>; o.bs % o.box; o.box /= 2) {
       }
       rc = launch_kernel(attend_observe_tiled_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kObserveThreads), smem, st,
                          true, o, *observe_map, observe_runs, row0);
@@ -255,8 +255,8 @@ int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache
   int observe_runs = 0;
   if (weight_sums != nullptr) {
     observe_runs = (int)std::min<long long>(attend_max_runs(tiled || Y.head_dim > 128 ? kSMs : 2 * kSMs, Y.num_kv_heads),
-                                            attend_max_tiles(Y, 1, num_listed, tiled ? kDecodeTile : kAttendTile, 64));
-    int box = kDecodeTile;
+                                            attend_max_tiles(Y, 1, num_listed, tiled ? 32 : kAttendTile, 64));
+    int box = Y.head_dim == 64 ? kObserveTile<64> : Y.head_dim == 128 ? kObserveTile<128> : kObserveTile<256>;
     for (; Y.block_size % box; box /= 2) {
     }
     if (tiled && !encode_cache_map(&om, k_cache, Y, box)) return TRIATTN_ERR_CUDA;

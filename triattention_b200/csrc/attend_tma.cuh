@@ -34,7 +34,7 @@ __device__ __forceinline__ uint32_t swz_off(int row, int piece) {
 // are not loaded.  The positions are written a batch of up to kBatch tiles at a time, so their ring is deeper: at most
 // STAGES + kBatch + 1 tiles are between the last one read and the last one written.
 template <int TILE>
-constexpr int kPosRing = TILE == 32 ? 64 : 16;
+constexpr int kPosRing = TILE == 128 ? 16 : TILE == 64 ? 32 : 64;
 template <int TILE>
 constexpr int kBatch = kPosRing<TILE> / 2;
 template <int TILE, int STAGES, bool BLOCKS = false>
@@ -69,13 +69,15 @@ __device__ __forceinline__ bool thread_wait(uint64_t& bar, uint32_t parity, int*
 }
 
 // A producer warp: K (which = 0) or V (1) of tiles 0 .. count - 1 of the run that starts at `c`; stage s is at
-// dst + s * stride, its barriers are full[s] and empty[s].
+// dst + s * stride, its barriers are full[s] and empty[s].  Of `turns` warps that share the work, warp `turn` loads every
+// turns-th tile.
 // Two warps, because a warp spends some 400 cycles on a tile - waiting for the stage, arming its barrier and above all
 // issuing the loads - while the SM's share of the bandwidth moves a 16 KB tile in 700.
 template <int D, int TILE, int STAGES, class Ring>
 __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUtensorMap* map, int which, AttendCursor c,
                                                int count, int rows_per_tile, uint32_t dst, uint32_t stride,
-                                               uint64_t* full, uint64_t* empty, Ring& ring) {
+                                               uint64_t* full, uint64_t* empty, Ring& ring, int turn = 0,
+                                               int turns = 1) {
   const int lane = threadIdx.x & 31;
   const int boxes = TILE / p.box;
   const int my_tile = lane / boxes, my_box = lane - my_tile * boxes;
@@ -126,7 +128,7 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
       u.pos = -1;
       *(volatile int*)&ring.gaps = 1;
     }
-    if (which == 0 && my_tile < u.tiles)
+    if (which == 0 && my_tile < u.tiles && (it + my_tile) % turns == turn)
       for (int i = 0; i < p.box; i += 8) {
         ring.pos[(it + my_tile) % kPosRing<TILE>][(my_box * p.box + i) >> 3] = u.pos < 0 ? -1 : u.pos + i;
         if constexpr (Ring::kBlocks) ring.blk[(it + my_tile) % kPosRing<TILE>][(my_box * p.box + i) >> 3] = u.blk;
@@ -136,16 +138,18 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
     const int slot = u.blk * p.slots_per_block + u.head, group = u.in >> 3;
     const uint32_t at = dst + (uint32_t)my_box * box_bytes;
     for (int j = 0; j < u.tiles; ++j, ++it) {
-      if (it >= STAGES && !ring_wait(empty[s], phase, &ring.err, p.status)) {
-        stop = true;
-        break;
+      if (turns == 1 || it % turns == turn) {
+        if (it >= STAGES && !ring_wait(empty[s], phase, &ring.err, p.status)) {
+          stop = true;
+          break;
+        }
+        fence_proxy_async();  // the readers' accesses (acquired above) before the refill
+        const uint32_t bar = smem_u32(&full[s]);
+        if (lane == 0)
+          mbar_arrive_expect_tx(bar, (uint32_t)__popc((live >> (j * boxes)) & ((1u << boxes) - 1u)) * box_bytes + kTestExtraTxBytes);
+        __syncwarp();
+        if (my_tile == j && u.pos >= 0) tma_load_tokens(at + (uint32_t)s * stride, map, bar, group, slot);
       }
-      fence_proxy_async();  // the readers' accesses (acquired above) before the refill
-      const uint32_t bar = smem_u32(&full[s]);
-      if (lane == 0)
-        mbar_arrive_expect_tx(bar, (uint32_t)__popc((live >> (j * boxes)) & ((1u << boxes) - 1u)) * box_bytes + kTestExtraTxBytes);
-      __syncwarp();
-      if (my_tile == j && u.pos >= 0) tma_load_tokens(at + (uint32_t)s * stride, map, bar, group, slot);
       if (++s == STAGES) {
         s = 0;
         phase ^= 1u;
@@ -155,18 +159,20 @@ __device__ __forceinline__ void attend_produce(const AttendParams& p, const CUte
   if (err) flag_status(p.status, err);
   // after a timeout: nothing may still be landing when the CTA retires
   if (*(volatile int*)&ring.err != 0)
-    for (int j = max(0, it - STAGES); j < it; ++j) mbar_wait_bounded(smem_u32(&full[j % STAGES]), (uint32_t)(j / STAGES) & 1u);
+    for (int j = max(0, it - STAGES); j < it; ++j)
+      if (j % turns == turn) mbar_wait_bounded(smem_u32(&full[j % STAGES]), (uint32_t)(j / STAGES) & 1u);
 }
 
 // ------------------------------------------------------------------------------------------ few query rows
 constexpr int kDecodeWarps = 6;   // consumer warps; a stage always belongs to the same warp (STAGES is a multiple)
 constexpr int kDecodeThreads = (kDecodeWarps + 2) * 32;
-constexpr int kDecodeTile = 32;
 template <int D>
-constexpr int kDecodeStages = D == 64 ? 24 : D == 128 ? 12 : 6;  // 192 KB
+constexpr int kDecodeTile = D == 64 ? 64 : 32;  // 16 KB (D = 256: 32 KB) of K and V
+template <int D>
+constexpr int kDecodeStages = D == 256 ? 6 : 12;  // 192 KB
 template <int D, bool SPLIT_P>
 constexpr size_t decode_smem_bytes() {
-  return 1024 + (size_t)kDecodeStages<D> * 2 * kDecodeTile * D * 2 + (size_t)(SPLIT_P && D <= 128 ? kDecodeWarps : 1) * (SPLIT_P ? 8 : 16) * D * 4;
+  return 1024 + (size_t)kDecodeStages<D> * 2 * kDecodeTile<D> * D * 2 + (size_t)(SPLIT_P && D <= 128 ? kDecodeWarps : 1) * (SPLIT_P ? 8 : 16) * D * 4;
 }
 
 // Rows are padded to the 16 of mma.sync; a tile is one warp's business from arrival to release, so tiles of different
@@ -176,7 +182,7 @@ template <int D, bool SPLIT_P>
 __global__ void __launch_bounds__(kDecodeThreads, 1)
     attend_decode_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,
                          const __grid_constant__ CUtensorMap vmap, const int runs) {
-  constexpr int TILE = kDecodeTile, STAGES = kDecodeStages<D>, WARPS = kDecodeWarps;
+  constexpr int TILE = kDecodeTile<D>, STAGES = kDecodeStages<D>, WARPS = kDecodeWarps;
   static_assert(STAGES % WARPS == 0, "a stage belongs to one warp: its barriers are never more than a phase ahead");
   constexpr int ROWS = SPLIT_P ? 8 : 16;
   constexpr uint32_t kTileBytes = TILE * D * 2;
@@ -485,27 +491,31 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
 }
 
 // ------------------------------------------------------------------------------------------ weight sums
-// The second pass of attend_observe_kernel (see attend.cuh for the formula), K tiles from the ring.  S^T = K Q^T: a warp's tile of
-// 32 tokens is the A operand (two 16-row fragments, held in registers), the query rows are the columns, eight at a
-// time from shared memory; a token's sum over the rows stays inside four lanes.  The old sums are requested when the tile arrives.
+// The second pass of attend_observe_kernel (see attend.cuh for the formula), K tiles from the ring.  S^T = K Q^T: 32 tokens of a
+// warp's tile are the A operand (two 16-row fragments, held in registers), the query rows are the columns, eight at a
+// time from shared memory; a token's sum over the rows stays inside four lanes.  The old sums are requested when the
+// tokens are taken up.  Two warps load, tile by tile in turn: a warp issues a load every 80 cycles or so, and a box is only
+// 16 D bytes per 8 tokens.
 // Calls with more than kObserveRows<D> rows run the kernel once per that many (row0): the first pass sets or adds, the
 // others add.
 constexpr int kObserveWarps = 6;
-constexpr int kObserveThreads = (kObserveWarps + 1) * 32;
+constexpr int kObserveThreads = (kObserveWarps + 2) * 32;
+template <int D>
+constexpr int kObserveTile = D == 64 ? 64 : 32;  // tokens: 8 KB (D = 256: 16 KB)
 template <int D>
 constexpr int kObserveStages = D == 256 ? 6 : 12;
 template <int D>
 constexpr int kObserveTileRows = D == 256 ? 128 : 256;
 template <int D>
 constexpr size_t observe_tiled_smem_bytes() {
-  return 1024 + (size_t)kObserveStages<D> * kDecodeTile * D * 2 + (size_t)kObserveTileRows<D> * D * 2;
+  return 1024 + (size_t)kObserveStages<D> * kObserveTile<D> * D * 2 + (size_t)kObserveTileRows<D> * D * 2;
 }
 
 template <int D>
 __global__ void __launch_bounds__(kObserveThreads, 1)
     attend_observe_tiled_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap, const int runs,
                                 const int row0) {
-  constexpr int TILE = kDecodeTile, STAGES = kObserveStages<D>, WARPS = kObserveWarps, THREADS = kObserveThreads;
+  constexpr int TILE = kObserveTile<D>, STAGES = kObserveStages<D>, WARPS = kObserveWarps, THREADS = kObserveThreads;
   constexpr int RMAX = kObserveTileRows<D>;
   constexpr int kAll = 1 << 24;  // all rows of a (request, KV head) in one segment
   static_assert(STAGES % WARPS == 0, "a stage belongs to one warp");
@@ -534,8 +544,8 @@ __global__ void __launch_bounds__(kObserveThreads, 1)
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* const q_smem = smem_raw + (base - smem_u32(smem_raw)) + STAGES * kTileBytes;
   const uint32_t q_base = base + STAGES * kTileBytes;
-  if (wid == WARPS) {
-    attend_produce<D, TILE, STAGES>(p, &kmap, 0, c, count, kAll, base, kTileBytes, ring.full[0], ring.empty[0], ring);
+  if (wid >= WARPS) {
+    attend_produce<D, TILE, STAGES>(p, &kmap, 0, c, count, kAll, base, kTileBytes, ring.full[0], ring.empty[0], ring, wid - WARPS, 2);
     return;
   }
   auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
@@ -575,60 +585,65 @@ __global__ void __launch_bounds__(kObserveThreads, 1)
         break;
       }
       const uint32_t kb = base + (uint32_t)s * kTileBytes;
-      // this lane's four tokens: rows lane / 4 + 8 i
-      int pos[4];
-      float old[4] = {0.f, 0.f, 0.f, 0.f};
-      float* at[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int q8 = ring.pos[n % kPosRing<TILE>][i];
-        pos[i] = q8 < 0 ? -1 : q8 + (lane >> 2);
-        if (pos[i] >= c.r.T) pos[i] = -1;
-        at[i] = nullptr;
-        if ((lane & 3) == 0 && pos[i] >= 0) {
-          at[i] = p.sums + ((long long)ring.blk[n % kPosRing<TILE>][i] * p.Hkv + c.h) * p.bs + pos[i] % p.bs;
-          // a query's own token, or sums that start anew: whatever the slot holds is nobody's
-          if (row0 > 0 || (p.reset_sums == 0 && pos[i] < ctx)) old[i] = *at[i];
-        }
-      }
-      uint32_t kf[2][D / 16][4];
-#pragma unroll
-      for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) ldsm_x4(kf[a][k], kb + swz_off<D>(a * 16 + (lane & 15), k * 2 + (lane >> 4)));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ring.empty[0][s]));  // the tile is in registers
-      const bool own = max(max(pos[0], pos[1]), max(pos[2], pos[3])) >= ctx;
-      float w[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int j = 0; j < nt; ++j) {
-        float e[2][4] = {};
-#pragma unroll
-        for (int k = 0; k < D / 32; ++k) {
-          uint32_t qf[4];
-          ldsm_x4(qf, q_base + tile_off<D>(j * 8 + (lane & 7), k * 4 + (lane >> 3)));
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            mma_bf16(e[a], kf[a][2 * k], qf[0], qf[1]);
-            mma_bf16(e[a], kf[a][2 * k + 1], qf[2], qf[3]);
-          }
-        }
-        const int row = j * 8 + (lane & 3) * 2;
-        const float z0 = lse2[row], z1 = lse2[row + 1];
-#pragma unroll
+#pragma unroll 1
+      for (int sub = 0; sub < TILE; sub += 32) {
+        // this lane's four tokens: rows lane / 4 + 8 i
+        int pos[4];
+        float old[4] = {0.f, 0.f, 0.f, 0.f};
+        float* at[4];
+  #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float p0 = ex2(fmaf(e[i >> 1][(i & 1) * 2], p.scale_log2, -z0)), p1 = ex2(fmaf(e[i >> 1][(i & 1) * 2 + 1], p.scale_log2, -z1));
-          if (own && pos[i] >= ctx) {
-            p0 = (words[row] >> (pos[i] - ctx)) & 1ull ? p0 : 0.f;
-            p1 = (words[row + 1] >> (pos[i] - ctx)) & 1ull ? p1 : 0.f;
+          const int q8 = ring.pos[n % kPosRing<TILE>][(sub >> 3) + i];
+          pos[i] = q8 < 0 ? -1 : q8 + (lane >> 2);
+          if (pos[i] >= c.r.T) pos[i] = -1;
+          at[i] = nullptr;
+          if ((lane & 3) == 0 && pos[i] >= 0) {
+            at[i] = p.sums + ((long long)ring.blk[n % kPosRing<TILE>][(sub >> 3) + i] * p.Hkv + c.h) * p.bs + pos[i] % p.bs;
+            // a query's own token, or sums that start anew: whatever the slot holds is nobody's
+            if (row0 > 0 || (p.reset_sums == 0 && pos[i] < ctx)) old[i] = *at[i];
           }
-          w[i] += p0 + p1;
         }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
-        w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
-        if (at[i] != nullptr) *at[i] = old[i] + w[i];
+        uint32_t kf[2][D / 16][4];
+  #pragma unroll
+        for (int a = 0; a < 2; ++a)
+  #pragma unroll
+          for (int k = 0; k < D / 16; ++k) ldsm_x4(kf[a][k], kb + swz_off<D>(sub + a * 16 + (lane & 15), k * 2 + (lane >> 4)));
+        if (sub + 32 == TILE) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&ring.empty[0][s]));  // the rest of the tile is in registers
+        }
+        const bool own = max(max(pos[0], pos[1]), max(pos[2], pos[3])) >= ctx;
+        float w[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < nt; ++j) {
+          float e[2][4] = {};
+  #pragma unroll
+          for (int k = 0; k < D / 32; ++k) {
+            uint32_t qf[4];
+            ldsm_x4(qf, q_base + tile_off<D>(j * 8 + (lane & 7), k * 4 + (lane >> 3)));
+  #pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              mma_bf16(e[a], kf[a][2 * k], qf[0], qf[1]);
+              mma_bf16(e[a], kf[a][2 * k + 1], qf[2], qf[3]);
+            }
+          }
+          const int row = j * 8 + (lane & 3) * 2;
+          const float z0 = lse2[row], z1 = lse2[row + 1];
+  #pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float p0 = ex2(fmaf(e[i >> 1][(i & 1) * 2], p.scale_log2, -z0)), p1 = ex2(fmaf(e[i >> 1][(i & 1) * 2 + 1], p.scale_log2, -z1));
+            if (own && pos[i] >= ctx) {
+              p0 = (words[row] >> (pos[i] - ctx)) & 1ull ? p0 : 0.f;
+              p1 = (words[row + 1] >> (pos[i] - ctx)) & 1ull ? p1 : 0.f;
+            }
+            w[i] += p0 + p1;
+          }
+        }
+  #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
+          w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
+          if (at[i] != nullptr) *at[i] = old[i] + w[i];
+        }
       }
     }
     it += piece;
