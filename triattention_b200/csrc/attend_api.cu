@@ -167,7 +167,7 @@ int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensor
       AttendParams o = p;
       for (o.box = kObserveTile<D>; o.bs % o.box; o.box /= 2) {
       }
-      rc = launch_kernel(attend_observe_tiled_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kObserveThreads), smem, st,
+      rc = launch_kernel(attend_observe_tiled_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kObserveThreads<D>), smem, st,
                          true, o, *observe_map, observe_runs, row0);
       if (rc != TRIATTN_OK) return rc;
     }

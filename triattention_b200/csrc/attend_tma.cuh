@@ -12,6 +12,8 @@
 
 #include <cuda.h>  // CUtensorMap
 
+#include <type_traits>
+
 #include "attend.cuh"
 
 namespace triattn {
@@ -34,7 +36,7 @@ __device__ __forceinline__ uint32_t swz_off(int row, int piece) {
 // are not loaded.  The positions are written a batch of up to kBatch tiles at a time, so their ring is deeper: at most
 // STAGES + kBatch + 1 tiles are between the last one read and the last one written.
 template <int TILE>
-constexpr int kPosRing = TILE == 128 ? 16 : TILE == 64 ? 32 : 64;
+constexpr int kPosRing = TILE == 128 ? 16 : 64;
 template <int TILE>
 constexpr int kBatch = kPosRing<TILE> / 2;
 template <int TILE, int STAGES, bool BLOCKS = false>
@@ -498,12 +500,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
 // 16 D bytes per 8 tokens.
 // Calls with more than kObserveRows<D> rows run the kernel once per that many (row0): the first pass sets or adds, the
 // others add.
-constexpr int kObserveWarps = 6;
-constexpr int kObserveThreads = (kObserveWarps + 2) * 32;
+template <int D>
+constexpr int kObserveWarps = D == 256 ? 6 : 8;
+template <int D>
+constexpr int kObserveThreads = (kObserveWarps<D> + 2) * 32;
 template <int D>
 constexpr int kObserveTile = D == 64 ? 64 : 32;  // tokens: 8 KB (D = 256: 16 KB)
 template <int D>
-constexpr int kObserveStages = D == 256 ? 6 : 12;
+constexpr int kObserveStages = D == 256 ? 6 : 16;
 template <int D>
 constexpr int kObserveTileRows = D == 256 ? 128 : 256;
 template <int D>
@@ -512,10 +516,10 @@ constexpr size_t observe_tiled_smem_bytes() {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kObserveThreads, 1)
+__global__ void __launch_bounds__(kObserveThreads<D>, 1)
     attend_observe_tiled_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap, const int runs,
                                 const int row0) {
-  constexpr int TILE = kObserveTile<D>, STAGES = kObserveStages<D>, WARPS = kObserveWarps, THREADS = kObserveThreads;
+  constexpr int TILE = kObserveTile<D>, STAGES = kObserveStages<D>, WARPS = kObserveWarps<D>, THREADS = kObserveThreads<D>;
   constexpr int RMAX = kObserveTileRows<D>;
   constexpr int kAll = 1 << 24;  // all rows of a (request, KV head) in one segment
   static_assert(STAGES % WARPS == 0, "a stage belongs to one warp");
@@ -585,66 +589,80 @@ __global__ void __launch_bounds__(kObserveThreads, 1)
         break;
       }
       const uint32_t kb = base + (uint32_t)s * kTileBytes;
-#pragma unroll 1
-      for (int sub = 0; sub < TILE; sub += 32) {
-        // this lane's four tokens: rows lane / 4 + 8 i
-        int pos[4];
-        float old[4] = {0.f, 0.f, 0.f, 0.f};
-        float* at[4];
-  #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int q8 = ring.pos[n % kPosRing<TILE>][(sub >> 3) + i];
-          pos[i] = q8 < 0 ? -1 : q8 + (lane >> 2);
-          if (pos[i] >= c.r.T) pos[i] = -1;
-          at[i] = nullptr;
-          if ((lane & 3) == 0 && pos[i] >= 0) {
-            at[i] = p.sums + ((long long)ring.blk[n % kPosRing<TILE>][(sub >> 3) + i] * p.Hkv + c.h) * p.bs + pos[i] % p.bs;
-            // a query's own token, or sums that start anew: whatever the slot holds is nobody's
-            if (row0 > 0 || (p.reset_sums == 0 && pos[i] < ctx)) old[i] = *at[i];
-          }
+      // In the products a lane has tokens lane / 4 + 8 i of 32; of the sums it keeps one token's, i = lane % 4.
+      int pos[TILE / 8];
+      float old[TILE / 32];
+      float* at[TILE / 32];
+#pragma unroll
+      for (int i = 0; i < TILE / 8; ++i) {
+        const int q8 = ring.pos[n % kPosRing<TILE>][i];
+        pos[i] = q8 < 0 || q8 + (lane >> 2) >= c.r.T ? -1 : q8 + (lane >> 2);
+      }
+#pragma unroll
+      for (int y = 0; y < TILE / 32; ++y) {
+        const int run8 = y * 4 + (lane & 3), q8 = ring.pos[n % kPosRing<TILE>][run8], t = q8 + (lane >> 2);
+        old[y] = 0.f;
+        at[y] = nullptr;
+        if (q8 >= 0 && t < c.r.T) {
+          at[y] = p.sums + ((long long)ring.blk[n % kPosRing<TILE>][run8] * p.Hkv + c.h) * p.bs + t % p.bs;
+          // a query's own token, or sums that start anew: whatever the slot holds is nobody's
+          if (row0 > 0 || (p.reset_sums == 0 && t < ctx)) old[y] = *at[y];
         }
+      }
+#pragma unroll
+      for (int sub = 0; sub < TILE; sub += 32) {
         uint32_t kf[2][D / 16][4];
   #pragma unroll
         for (int a = 0; a < 2; ++a)
   #pragma unroll
           for (int k = 0; k < D / 16; ++k) ldsm_x4(kf[a][k], kb + swz_off<D>(sub + a * 16 + (lane & 15), k * 2 + (lane >> 4)));
-        if (sub + 32 == TILE) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&ring.empty[0][s]));  // the rest of the tile is in registers
-        }
-        const bool own = max(max(pos[0], pos[1]), max(pos[2], pos[3])) >= ctx;
+        const int* ps = pos + (sub >> 3);
+        const bool own = max(max(ps[0], ps[1]), max(ps[2], ps[3])) >= ctx;
         float w[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int j = 0; j < nt; ++j) {
-          float e[2][4] = {};
-  #pragma unroll
+        auto rows8 = [&](int j, auto pair) {  // 8 query rows, or 16: the products of two groups overlap
+          constexpr int G = decltype(pair)::value;
+          float e[G][2][4] = {};
+#pragma unroll
           for (int k = 0; k < D / 32; ++k) {
-            uint32_t qf[4];
-            ldsm_x4(qf, q_base + tile_off<D>(j * 8 + (lane & 7), k * 4 + (lane >> 3)));
-  #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-              mma_bf16(e[a], kf[a][2 * k], qf[0], qf[1]);
-              mma_bf16(e[a], kf[a][2 * k + 1], qf[2], qf[3]);
+#pragma unroll
+            for (int y = 0; y < G; ++y) {
+              uint32_t qf[4];
+              ldsm_x4(qf, q_base + tile_off<D>((j + y) * 8 + (lane & 7), k * 4 + (lane >> 3)));
+#pragma unroll
+              for (int a = 0; a < 2; ++a) {
+                mma_bf16(e[y][a], kf[a][2 * k], qf[0], qf[1]);
+                mma_bf16(e[y][a], kf[a][2 * k + 1], qf[2], qf[3]);
+              }
             }
           }
-          const int row = j * 8 + (lane & 3) * 2;
-          const float z0 = lse2[row], z1 = lse2[row + 1];
-  #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float p0 = ex2(fmaf(e[i >> 1][(i & 1) * 2], p.scale_log2, -z0)), p1 = ex2(fmaf(e[i >> 1][(i & 1) * 2 + 1], p.scale_log2, -z1));
-            if (own && pos[i] >= ctx) {
-              p0 = (words[row] >> (pos[i] - ctx)) & 1ull ? p0 : 0.f;
-              p1 = (words[row + 1] >> (pos[i] - ctx)) & 1ull ? p1 : 0.f;
+#pragma unroll
+          for (int y = 0; y < G; ++y) {
+            const int row = (j + y) * 8 + (lane & 3) * 2;
+            const float z0 = lse2[row], z1 = lse2[row + 1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float p0 = ex2(fmaf(e[y][i >> 1][(i & 1) * 2], p.scale_log2, -z0)), p1 = ex2(fmaf(e[y][i >> 1][(i & 1) * 2 + 1], p.scale_log2, -z1));
+              if (own && ps[i] >= ctx) {
+                p0 = (words[row] >> (ps[i] - ctx)) & 1ull ? p0 : 0.f;
+                p1 = (words[row + 1] >> (ps[i] - ctx)) & 1ull ? p1 : 0.f;
+              }
+              w[i] += p0 + p1;
             }
-            w[i] += p0 + p1;
           }
-        }
-  #pragma unroll
+        };
+        int j = 0;
+        for (; j + 1 < nt; j += 2) rows8(j, std::integral_constant<int, 2>{});
+        if (j < nt) rows8(j, std::integral_constant<int, 1>{});
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
           w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
           w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
-          if (at[i] != nullptr) *at[i] = old[i] + w[i];
         }
+        const float w01 = lane & 1 ? w[1] : w[0], w23 = lane & 1 ? w[3] : w[2];
+        if (at[sub / 32] != nullptr) *at[sub / 32] = old[sub / 32] + (lane & 2 ? w23 : w01);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ring.empty[0][s]));
     }
     it += piece;
     c.t += piece - 1;
