@@ -178,6 +178,12 @@ int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensor
                        observe_smem_bytes<D>(), st, true, p, observe_runs);
 }
 
+template <int D>
+int launch_scores(const SelectBlocksParams& p, dim3 grid, int per_warp, cudaStream_t st) {
+  if (!ensure_dynamic_smem<block_scores_kernel<D>>(score_smem_bytes<D>())) return TRIATTN_ERR_CUDA;
+  return launch_kernel(block_scores_kernel<D>, grid, dim3(kScoreThreads), score_smem_bytes<D>(), st, true, p, per_warp);
+}
+
 }  // namespace
 
 extern "C" {
@@ -356,9 +362,9 @@ int triattn_select_blocks(const triattn_paged_layout* layout, const void* q, int
   while (per_warp > 4 && grid_x(per_warp) * rows < 2 * kSMs) per_warp /= 2;
   const dim3 grid((unsigned)grid_x(per_warp), (unsigned)Y.num_kv_heads, (unsigned)Y.num_reqs);
   switch (Y.head_dim) {
-    case 64: rc = launch_kernel(block_scores_kernel<64>, grid, dim3(kScoreThreads), 0, st, true, p, per_warp); break;
-    case 128: rc = launch_kernel(block_scores_kernel<128>, grid, dim3(kScoreThreads), 0, st, true, p, per_warp); break;
-    default: rc = launch_kernel(block_scores_kernel<256>, grid, dim3(kScoreThreads), 0, st, true, p, per_warp); break;
+    case 64: rc = launch_scores<64>(p, grid, per_warp, st); break;
+    case 128: rc = launch_scores<128>(p, grid, per_warp, st); break;
+    default: rc = launch_scores<256>(p, grid, per_warp, st); break;
   }
   if (rc != TRIATTN_OK) return rc;
   const int cap = (int)std::min<long long>((Y.max_blocks_per_req + 3ll) / 4 * 4, 32768);

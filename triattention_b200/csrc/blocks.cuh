@@ -141,13 +141,21 @@ __device__ __forceinline__ BlocksReq blocks_req(const SelectBlocksParams& p, int
 }
 
 //
-// A warp takes `per_warp` consecutive blocks of one (request, KV head): its lanes fetch the block ids together, then four
-// blocks' bounds at a time (a lane holds the same 2 D / 32 channels' weights throughout), and the four sums are
-// reduced together.  Bound by the bounds' bytes (4 D per block and KV head), read once.
+// A warp takes `per_warp` consecutive blocks of one (request, KV head): its lanes fetch the block ids together, the bounds come
+// in through a ring of eight rows per warp (cp.async: in registers the loads in flight cost occupancy, and with either too few
+// loads or too few warps the kernel took half as long again), and four blocks' sums are reduced together; a lane holds the same
+// 2 D / 32 channels' weights throughout.  Bound by the bounds' bytes (4 D per block and KV head), read once.
+constexpr int kScoreRing = 8;  // rows
+template <int D>
+constexpr size_t score_smem_bytes() { return (size_t)(kScoreThreads / 32) * kScoreRing * D * 4 + 2 * (kScoreThreads / 32) * D * sizeof(double); }
 template <int D>
 __global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __grid_constant__ SelectBlocksParams p, const int per_warp) {
   constexpr int WARPS = kScoreThreads / 32, PCS = D / 8, GROUPS = kScoreThreads / PCS;  // 16-byte pieces of a row, rows at a time
-  __shared__ double part[2][GROUPS][D];  // sums of the queries' negative and positive parts
+  constexpr int PER = 2 * D / 32;  // values per lane: 4 at D = 64, 8 at 128, 16 at 256
+  extern __shared__ __align__(16) unsigned char score_smem[];
+  __shared__ double qsum[2 * D];
+  unsigned char* ring = score_smem + (threadIdx.x >> 5) * (kScoreRing * D * 4);
+  double(*part)[WARPS][D] = reinterpret_cast<double(*)[WARPS][D]>(score_smem + WARPS * kScoreRing * D * 4);  // by sign and warp
   grid_dependency_wait();
   trigger_dependents();
   unsigned err = 0u;
@@ -166,6 +174,21 @@ __global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __gri
       err |= TRIATTN_DEV_BAD_BLOCK_ID;
       my_blk = -2;
     }
+  }
+  const int count = lb1 - lb0;
+  auto fetch = [&](int j) {  // bounds of the warp's block j
+    const int blk = __shfl_sync(0xffffffffu, my_blk, j & 31);
+    if (j < count && blk >= 0) {
+      const unsigned char* src = reinterpret_cast<const unsigned char*>(p.bounds + ((long long)blk * p.Hkv + h) * 2 * D);
+      const uint32_t dst = smem_u32(ring + (j % kScoreRing) * (D * 4));
+#pragma unroll
+      for (int x = lane; x < D / 4; x += 32) cp_async16(dst + x * 16, src + x * 16, true);
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < kScoreRing; ++j) {
+    fetch(j);
+    if (j % 4 == 3) cp_async_commit();
   }
   // ---- the query rows' sums, eight channels per thread
   {
@@ -188,40 +211,46 @@ __global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __gri
     }
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      part[0][gr][pc * 8 + x] = down[x];
-      part[1][gr][pc * 8 + x] = up[x];
+#pragma unroll
+      for (int k = PCS; k < 32; k <<= 1) {
+        up[x] += __shfl_xor_sync(0xffffffffu, up[x], k);
+        down[x] += __shfl_xor_sync(0xffffffffu, down[x], k);
+      }
+      if (lane < PCS) {
+        part[0][wid][pc * 8 + x] = down[x];
+        part[1][wid][pc * 8 + x] = up[x];
+      }
     }
   }
   __syncthreads();
-  __shared__ double qsum[2 * D];
   for (int e = tid; e < 2 * D; e += kScoreThreads) {
     double s = 0.0;
-    const int live = min(GROUPS, r.n * p.g);
-    for (int gr = 0; gr < live; ++gr) s += part[e / D][gr][e % D];
+    for (int w = 0; w < WARPS; ++w) s += part[e / D][w][e % D];
     qsum[e] = s;
   }
   __syncthreads();
-  constexpr int PER = 2 * D / 32;  // values per lane: 4 at D = 64, 8 at 128, 16 at 256
   double q[PER];
 #pragma unroll
   for (int x = 0; x < PER; ++x) q[x] = qsum[lane * PER + x];
   const double unscale = __hiloint2double((1023 + 896) << 20, 0);
   float* out = p.scores + ((long long)b * p.Hkv + h) * p.max_blocks;
-  auto fetch = [&](int j, uint32_t (&w)[PER / 2]) {  // bounds of the warp's block j
-    const int blk = max(__shfl_sync(0xffffffffu, my_blk, j & 31), 0);
-    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.bounds + ((long long)blk * p.Hkv + h) * 2 * D) + lane * (PER / 2);
-#pragma unroll
-    for (int x = 0; x < PER / 2; x += 2) {
-      const uint2 u = *reinterpret_cast<const uint2*>(src + x);
-      w[x] = u.x;
-      w[x + 1] = u.y;
-    }
-  };
-  const int count = lb1 - lb0;
   for (int j0 = 0; j0 < count; j0 += 4) {
+    cp_async_wait<kScoreRing / 4 - 1>();
+    __syncwarp();
     uint32_t w[4][PER / 2];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) fetch(min(j0 + y, count - 1), w[y]);
+    for (int y = 0; y < 4; ++y) {  // (rows that were not fetched hold anything: their sums are not used)
+#pragma unroll
+      for (int x = 0; x < PER / 2; x += 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(ring + ((j0 + y) % kScoreRing) * (D * 4) + (lane * (PER / 2) + x) * 4);
+        w[y][x] = u.x;
+        w[y][x + 1] = u.y;
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int y = 0; y < 4; ++y) fetch(j0 + kScoreRing + y);
+    cp_async_commit();
     double s[4];
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
