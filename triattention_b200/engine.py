@@ -194,6 +194,79 @@ class PagedCompressor:
                               device_status=status, h2d_bytes=n_ints * 4, d2h_bytes=4)
 
 
+@dataclass
+class AttentionEvictor:
+    """Eviction by accumulated attention weight for a batch of requests of one KV-cache group.
+
+    The counterpart of :class:`PagedCompressor` for engines whose attention runs through ``ops.attend_paged`` with
+    ``weight_sums``: no calibrated statistics are needed, and every layer keeps token sets of its own.  One pinned
+    staging buffer, one copy, two launches, one read of the status word; block tables are truncated on the host like
+    :meth:`PagedCompressor.compress` does.
+    """
+
+    window: int = 128
+    _staging: Optional[torch.Tensor] = field(default=None, repr=False)
+    _status_host: Optional[torch.Tensor] = field(default=None, repr=False)
+
+    def evict(
+        self,
+        view: ops.PagedCacheView,
+        weight_sums: torch.Tensor,
+        block_ids: Sequence[Sequence[int]],
+        seq_lens: Sequence[int],
+        budgets: Sequence[int],
+        prefill_lens: Optional[Sequence[int]] = None,
+    ) -> CompressResult:
+        """Keep ``min(budgets[b], seq_lens[b])`` tokens of every listed request, in place.
+
+        ``weight_sums`` ``[L, num_blocks, Hkv, block_size]`` fp32 is compacted with K and V.  Returns keep
+        ``[L, B, Hkv, keep_pitch]`` (as ``CompressResult.keep``) and the truncated block tables.
+        """
+        B = len(block_ids)
+        if not (B == len(seq_lens) == len(budgets)) or B == 0:
+            raise ValueError("block_ids, seq_lens and budgets must be non-empty and of equal length")
+        if prefill_lens is not None and len(prefill_lens) != B:
+            raise ValueError("prefill_lens must have one entry per request")
+        bs = view.block_size
+        lens = [int(n) for n in seq_lens]
+        need = [num_required_blocks(n, bs) for n in lens]
+        for ids, n in zip(block_ids, need):
+            if n > len(ids):
+                raise IndexError(f"token indices require block_idx={n - 1}, but only {len(ids)} blocks exist")
+        keep_counts = [max(0, min(int(k), n)) for k, n in zip(budgets, lens)]
+        keep_pitch, width = max(max(keep_counts), 1), max(max(need), 1)
+        n_ints = B * width + 3 * B + 1
+        if self._staging is None or self._staging.numel() < n_ints:
+            self._staging = torch.empty(n_ints, dtype=torch.int32).pin_memory()
+        if self._status_host is None:
+            self._status_host = torch.zeros(1, dtype=torch.int32).pin_memory()
+        st = self._staging[:n_ints]
+        sn = st.numpy()
+        table = sn[: B * width].reshape(B, width)
+        table[:] = 0
+        for b, (ids, n) in enumerate(zip(block_ids, need)):
+            table[b, :n] = ids[:n]
+        rest = sn[B * width :]
+        rest[:B], rest[B : 2 * B] = lens, keep_counts
+        rest[2 * B : 3 * B] = prefill_lens if prefill_lens is not None else 0
+        rest[3 * B] = 0
+        with torch.cuda.device(view.device):
+            dm = st.to(view.device, non_blocking=True)
+            off = B * width
+            d_status = dm[off + 3 * B : off + 3 * B + 1]
+            keep = ops.evict_paged(
+                view, view.layout(B, 1, width), weight_sums, dm[:off].view(B, width), dm[off : off + B],
+                dm[off + B : off + 2 * B], keep_pitch, self.window,
+                dm[off + 2 * B : off + 3 * B] if prefill_lens is not None else None, status=d_status)
+            self._status_host.copy_(d_status, non_blocking=True)
+            torch.cuda.current_stream().synchronize()
+        after = [num_required_blocks(k, bs) for k in keep_counts]
+        kept = [ids[:r] if isinstance(ids, np.ndarray) else [int(x) for x in ids[:r]] for ids, r in zip(block_ids, after)]
+        removed = [ids[r:] if isinstance(ids, np.ndarray) else [int(x) for x in ids[r:]] for ids, r in zip(block_ids, after)]
+        return CompressResult(keep=keep, keep_counts=keep_counts, kept_block_ids=kept, removed_block_ids=removed,
+                              device_status=int(self._status_host[0]), h2d_bytes=n_ints * 4, d2h_bytes=4)
+
+
 def compress_layer_shared(
     view: ops.PagedCacheView,
     stats: ops.DeviceStats,
