@@ -133,8 +133,29 @@ struct AttendPlanShared {
   int b;
 };
 
+// The tiles of up to 32 requests, one per lane: this lane's request, the tiles before it, the tiles of all.
+__device__ __forceinline__ long long attend_scan32(const AttendParams& p, int tile, int rows_per_tile, AttendReq& mine,
+                                                   long long& before, unsigned& err) {
+  const int lane = threadIdx.x & 31;
+  mine.tiles = mine.row_tiles = 0;
+  long long w = 0;
+  if (lane < p.B) {
+    mine = attend_req(p, lane, tile, rows_per_tile, err);
+    w = (long long)mine.tiles * mine.row_tiles;
+  }
+  long long incl = w;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const long long u = __shfl_up_sync(0xffffffffu, incl, s);
+    if (lane >= s) incl += u;
+  }
+  before = incl - w;
+  return __shfl_sync(0xffffffffu, incl, 31);
+}
+
 // Where run `run` (at most `runs`) of the call starts, and how many tiles it has; false: there is no such run.  All threads
-// call it; bad metadata is reported by run 0 of head 0.  A request per thread and pass; up to THREADS requests are read once.
+// call it; bad metadata is reported by run 0 of head 0.  Up to 32 requests every warp finds out for itself, without a
+// barrier (with one, planning took three times as long); more take a request per thread and pass.
 template <int THREADS>
 __device__ __forceinline__ bool attend_plan_run(const AttendParams& p, int runs, int min_tiles, int run, int tile,
                                                 int rows_per_tile, AttendPlanShared<THREADS>& sh, AttendCursor& c, int& count) {
@@ -142,6 +163,28 @@ __device__ __forceinline__ bool attend_plan_run(const AttendParams& p, int runs,
   unsigned err = 0u;
   AttendReq mine{};
   long long before = 0, W = 0;  // tiles before this thread's request of the pass, tiles of all passes
+  if (p.B <= 32) {
+    W = attend_scan32(p, tile, rows_per_tile, mine, before, err);
+    if (blockIdx.x == 0 && wid == 0 && err) flag_status(p.status, err);
+    const int J = attend_runs(runs, W, min_tiles);
+    if (run >= J) return false;
+    const long long first = attend_first_tile(W, J, run);
+    count = (int)(attend_first_tile(W, J, run + 1) - first);
+    const bool here = first >= before && first < before + (long long)mine.tiles * mine.row_tiles;
+    const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+    const int at = (int)__shfl_sync(0xffffffffu, first - before, from);  // inside one request's tiles: 32 bits
+    c.b = from;
+    c.r.T = __shfl_sync(0xffffffffu, mine.T, from);
+    c.r.n = __shfl_sync(0xffffffffu, mine.n, from);
+    c.r.q0 = __shfl_sync(0xffffffffu, mine.q0, from);
+    c.r.vlen = __shfl_sync(0xffffffffu, mine.vlen, from);
+    c.r.tiles = __shfl_sync(0xffffffffu, mine.tiles, from);
+    c.r.row_tiles = __shfl_sync(0xffffffffu, mine.row_tiles, from);
+    c.rt = at / c.r.tiles;
+    c.t = at - c.rt * c.r.tiles;
+    __syncthreads();  // what the CTA has set up meanwhile
+    return true;
+  }
   auto pass = [&](int b0) {
     long long w = 0;
     mine.tiles = mine.row_tiles = 0;
@@ -694,8 +737,15 @@ __global__ void __launch_bounds__(kCombineThreads) attend_combine_kernel(const _
   const AttendReq r = attend_req(p, b, tile, rows, err);
   int i0 = 0, i1 = 0;
   if (rt < r.row_tiles) {
-    const long long before = attend_work_before<kCombineThreads>(p, b, tile, rows, err, red);
-    const long long W = attend_work_before<kCombineThreads>(p, p.B, tile, rows, err, red);
+    long long before, W;
+    if (p.B <= 32) {
+      AttendReq mine{};
+      W = attend_scan32(p, tile, rows, mine, before, err);
+      before = __shfl_sync(0xffffffffu, before, b);
+    } else {
+      before = attend_work_before<kCombineThreads>(p, b, tile, rows, err, red);
+      W = attend_work_before<kCombineThreads>(p, p.B, tile, rows, err, red);
+    }
     const long long s0 = before + (long long)rt * r.tiles;
     const int J = attend_runs(runs, W, p.min_tiles);
     i0 = attend_owner(W, J, s0);

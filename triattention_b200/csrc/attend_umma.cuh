@@ -245,18 +245,22 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     // A wait that runs out ends the work but not the control flow: a warp that left would strand its partner at a barrier.
     bool dead = false;
     auto load_q = [&](const AttendCursor& at) {  // the pair's 32 rows of the operand, half of them per warp; D / 8 lanes to a row
-      const int rows0 = at.rt * ROWS + g * 128, pc = lane % (D / 8);
+      const int pc = lane % (D / 8), rr0 = (wid & 3) * 32 + half * 16 + lane / (D / 8);
+      constexpr int STEP = 256 / D;  // rows at a time
       unsigned char* dst = base_ptr + (q_base - base) + g * kQBytes;
-#pragma unroll 4
-      for (int y = 0; y < D / 16; ++y) {  // 256 / D rows at a time
-        const int rr = (wid & 3) * 32 + half * 16 + y * (256 / D) + lane / (D / 8);
-        const int r = rows0 + rr;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (r < at.r.n * p.g) {
-          const int i = r / p.g, j = r - i * p.g;
-          w = *reinterpret_cast<const uint4*>(p.q + (long long)(at.r.q0 + i) * p.q_ts + (long long)(at.h * p.g + j) * p.q_hs + pc * 8);
-        }
-        *reinterpret_cast<uint4*>(dst + rr * 128 + (pc >> 3) * 16384 + (((pc & 7) ^ (rr & 7)) << 4)) = w;
+      int r = at.rt * ROWS + g * 128 + rr0, i = r / p.g, j = r - i * p.g;
+      uint4 w[D / 16];  // all loads in flight
+#pragma unroll
+      for (int y = 0; y < D / 16; ++y) {
+        w[y] = make_uint4(0u, 0u, 0u, 0u);
+        if (i < at.r.n)
+          w[y] = *reinterpret_cast<const uint4*>(p.q + (long long)(at.r.q0 + i) * p.q_ts + (long long)(at.h * p.g + j) * p.q_hs + pc * 8);
+        for (j += STEP; j >= p.g; j -= p.g) ++i;
+      }
+#pragma unroll
+      for (int y = 0; y < D / 16; ++y) {
+        const int rr = rr0 + y * STEP;
+        *reinterpret_cast<uint4*>(dst + rr * 128 + (pc >> 3) * 16384 + (((pc & 7) ^ (rr & 7)) << 4)) = w[y];
       }
       fence_proxy_async();
       __syncwarp();
@@ -435,6 +439,16 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         const int slot = 2 * (int)blockIdx.x + (t_begin > 0 ? 0 : 1);
         const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : l;  // a NaN sum stays one
         const bool odd = *(volatile int*)&odd_piece == piece_no;
+        // the four rows this lane writes pieces of: where they go (null: they do not exist)
+        unsigned char* to[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int at = c.rt * ROWS + g * 128 + (wid & 3) * 32 + k * 8 + (lane >> 2);
+          const int i = at / p.g, hq = c.h * p.g + (at - i * p.g);
+          to[k] = at >= R ? nullptr
+                          : whole ? reinterpret_cast<unsigned char*>(p.out + (long long)(c.r.q0 + i) * p.o_ts + (long long)hq * p.o_hs)
+                                  : reinterpret_cast<unsigned char*>(p.part_o + ((long long)slot * ROWS + at - c.rt * ROWS) * D);
+        }
         unsigned char* stage = base_ptr + (q_base - base) + wid * (16 * D * 2);  // 16 rows of the operand: 4 KB (D = 128)
 #pragma unroll 1
         for (int y = 0; y < (dead ? 0 : D / 64); ++y) {
@@ -466,18 +480,12 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
             __syncwarp();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {  // eight rows at a time, four lanes to a row
-              const int rr = k * 8 + (lane >> 2), at = c.rt * ROWS + g * 128 + (wid & 3) * 32 + rr;
+              const int rr = k * 8 + (lane >> 2);
               const float4 e = *reinterpret_cast<const float4*>(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
               const int col = q * 32 + z * 16 + (lane & 3) * 4;
-              if (at < R) {
-                if (whole) {
-                  const int i = at / p.g, hq = c.h * p.g + (at - i * p.g);
-                  *reinterpret_cast<uint2*>(p.out + (long long)(c.r.q0 + i) * p.o_ts + (long long)hq * p.o_hs + col) =
-                      make_uint2(pack_bf16(e.x, e.y), pack_bf16(e.z, e.w));
-                } else {
-                  *reinterpret_cast<float4*>(p.part_o + ((long long)slot * ROWS + at - c.rt * ROWS) * D + col) = e;
-                }
-              }
+              if (to[k] == nullptr) continue;
+              if (whole) *reinterpret_cast<uint2*>(to[k] + col * 2) = make_uint2(pack_bf16(e.x, e.y), pack_bf16(e.z, e.w));
+              else *reinterpret_cast<float4*>(to[k] + col * 4) = e;
             }
             __syncwarp();
           }
