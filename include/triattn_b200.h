@@ -376,7 +376,8 @@ size_t triattn_attend_workspace_bytes(const triattn_paged_layout* layout /* host
  * ties go to the lowest index, NaN ranks last.  K, V and weight_sums of the kept tokens are compacted in place to the
  * front of the request's blocks; slots behind them are left as they are.
  *   weight_sums [num_layers, num_blocks, num_kv_heads, block_size] fp32
- *   keep_out    [num_layers, num_reqs, num_kv_heads, keep_pitch] int32, ascending, tail filled with -1
+ *   keep_out    [num_layers, num_reqs, num_kv_heads, keep_pitch] int32, ascending, tail filled with -1; a keep count above
+ *               keep_pitch is cut to it (TRIATTN_DEV_BAD_LENGTH)
  * Head dimension: any multiple of 8 the compaction takes.  Stands beside triattn_compress_paged, whose scores come
  * from calibrated statistics (triattention/vllm/runtime/selector_hf.py:749-1033).
  */

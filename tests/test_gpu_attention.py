@@ -497,3 +497,188 @@ def test_two_streams_and_graph_replay():
         g.replay()
         want = run(a, weight_sums=eager)
         assert torch.equal(out, want[0]) and torch.equal(sums, eager)
+
+
+# ------------------------------------------------------------------------------------------ every kernel variant
+# (D, block size, rows): decode with split and plain probabilities, tree with one and two row tiles, the gathered general kernel
+VARIANTS = [(64, 16, 4, 2), (128, 16, 4, 4), (128, 16, 7, 5), (64, 8, 3, 12), (128, 16, 9, 20), (64, 32, 4, 40),
+            (256, 16, 4, 2), (256, 16, 2, 8), (256, 16, 8, 7), (128, 5, 4, 2), (128, 5, 2, 8), (64, 5, 4, 12), (64, 24, 8, 30)]
+
+
+@pytest.mark.parametrize("D,bs,g,n", VARIANTS)
+def test_hidden_drafts_do_not_leak_in_any_variant(D, bs, g, n):
+    """The last draft is hidden from all other rows; its key is NaN, its value holds infinities and NaN."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(800 + D + bs + n)
+    T = 140
+    bt = Batch([T], [n], 2, g, D, bs, gen, tree=True)
+    for i in range(n - 1):
+        assert not (bt.words[i] >> (n - 1)) & 1
+    run = lambda: ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, n, tree_mask=bt.d_words, kv_axis=0)  # noqa: E731
+    bt.dev()
+    want, wlse = run()
+    check_rows(bt, want, wlse, n, 1 / math.sqrt(D))
+    blk, off = oa.token_slots(bt.table[0].tolist(), bs, T)
+    k, v = split(bt.cache[0], 0)
+    clean = bt.cache.clone()
+    v[blk[-1], off[-1], :, 3] = float("inf")
+    v[blk[-1], off[-1], :, D - 1] = float("-inf")
+    bt.dev()
+    out, lse = run()
+    assert torch.equal(out[: n - 1], want[: n - 1]) and torch.equal(lse, wlse)
+    assert (out[n - 1, :, 3] == float("inf")).all() and (out[n - 1, :, D - 1] == float("-inf")).all()
+    rest = [d for d in range(D) if d not in (3, D - 1)]
+    assert torch.equal(out[n - 1][:, rest], want[n - 1][:, rest])
+    k[blk[-1], off[-1]] = float("nan")
+    v[blk[-1], off[-1], :, :5] = float("nan")
+    bt.dev()
+    out, lse = run()
+    assert torch.equal(out[: n - 1], want[: n - 1]) and torch.equal(lse[: n - 1], wlse[: n - 1])
+    assert torch.isnan(out[n - 1].float()).all() and torch.isnan(lse[n - 1]).all()
+    bt.cache = clean
+
+
+@pytest.mark.parametrize("g,n,D", [(4, 1, 128), (4, 4, 64), (8, 6, 128), (4, 40, 128), (4, 64, 64), (2, 3, 256)])
+def test_logits_that_grow_by_orders_of_magnitude(g, n, D):
+    """Keys whose logits climb from -300 to 300 along the sequence: the running reference is raised again and again (2^64 steps
+    included), and the first tiles vanish; then the same falling, and all equal."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(900 + n)
+    T = 700
+    for shape in ("climb", "fall", "jump"):
+        bt = Batch([T], [n], 1, g, D, 16, gen, tree=n > 1)
+        bt.q[:] = 0
+        bt.q[:, :, 0] = 16.0                       # logits are 16 k_0 scale
+        bt.q[:, :, 1:9] = torch.randn((n, g, 8), generator=gen).to(torch.bfloat16)
+        blk, off = oa.token_slots(bt.table[0].tolist(), 16, T)
+        x = torch.linspace(-300, 300, T) if shape == "climb" else torch.linspace(300, -300, T)
+        if shape == "jump":
+            x = torch.where(torch.arange(T) == 400, 500.0, -200.0)
+        bt.cache[0][0][blk, off, 0, 0] = (x / 16).to(torch.bfloat16)
+        bt.dev()
+        out, lse = ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, n, tree_mask=bt.d_words, kv_axis=0, scale=1.0)
+        check_rows(bt, out, lse, n, 1.0)
+
+
+def test_caches_that_no_tensor_map_describes():
+    """Block strides that are no multiple of the head stride: the gathered kernels serve, weight sums included."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1000)
+    for n in (1, 6, 30):
+        bt = Batch([75, 50], [n, max(1, n - 2)], 2, 4, 64, 16, gen, tree=n > 1).dev()
+        flat = torch.zeros(2 * bt.nb * (16 * 2 * 64 + 8), dtype=torch.bfloat16, device=DEV)
+        odd = flat.as_strided((2, bt.nb, 16, 2, 64), (bt.nb * (16 * 2 * 64 + 8), 16 * 2 * 64 + 8, 128, 64, 1))
+        odd.copy_(bt.d_cache[0])
+        sums, want = (torch.zeros((bt.nb, 2, 16), device=DEV) for _ in range(2))
+        args = (bt.d_table, bt.d_lens, bt.d_start, n)
+        out, lse = ops.attend_paged(bt.d_q, odd, *args, tree_mask=bt.d_words, kv_axis=0, weight_sums=sums)
+        check_rows(bt, out, lse, n, 1 / 8)
+        ops.attend_paged(bt.d_q, bt.d_cache[0], *args, tree_mask=bt.d_words, kv_axis=0, weight_sums=want)
+        assert torch.allclose(sums, want, rtol=1e-4, atol=1e-7)
+
+
+@pytest.mark.parametrize("B,H,n", [(40, 3, 1), (700, 1, 1), (400, 1, 5), (3, 40, 1), (2, 160, 2), (33, 2, 9)])
+def test_many_requests_and_many_heads(B, H, n):
+    """Batches that are planned in several passes, head counts that do not divide the device."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1100 + B)
+    lens = torch.randint(n, 60, (B,), generator=gen).tolist()
+    lens[B // 2] = 500
+    counts = [0 if b % 7 == 3 else n for b in range(B)]
+    bt = Batch(lens, counts, H, 2, 64, 16, gen, tree=n > 1).dev()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    sums = torch.zeros((bt.nb, H, 16), device=DEV)
+    out, lse = ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, n, tree_mask=bt.d_words, kv_axis=0,
+                                weight_sums=sums, status=status)
+    assert int(status) == 0
+    # all requests at once, dense over padded lengths in 64 bits (the oracle's loops would take minutes)
+    T = max(lens)
+    pos = torch.arange(T)
+    blk = bt.table.long()[:, : (T + 15) // 16].repeat_interleave(16, 1)[:, :T]
+    k, v = (x[blk, pos % 16].double() for x in split(bt.cache[0], 0))           # [B, T, H, D]
+    worst, total = 0.0, 0.0
+    for b in range(B):
+        c = counts[b]
+        if c == 0:
+            continue
+        see = oa.visible(lens[b], c, None if bt.words is None else bt.words[bt.rows(b)])
+        q = bt.q[bt.rows(b)].double().view(c, H, 2, 64)
+        s = torch.einsum("nhgd,thd->nhgt", q, k[b, : lens[b]]) / 8
+        s = s.masked_fill(~see[:, None, None, :], -math.inf)
+        p = torch.softmax(s, -1)
+        o = torch.einsum("nhgt,thd->nhgd", p, v[b, : lens[b]]).reshape(c, H * 2, 64)
+        a = torch.einsum("nhgt,thd->nhgd", p, v[b, : lens[b]].abs()).reshape(c, H * 2, 64)
+        err = (out[bt.rows(b)].cpu().double() - o).abs() - 2.0 ** -8 * o.abs() - 2.0 ** -7.9 * a
+        worst = max(worst, float(err.max()))
+        assert torch.allclose(lse[bt.rows(b)].cpu().double(), torch.logsumexp(s, -1).reshape(c, H * 2), atol=1e-4)
+        total += c * H * 2
+    assert worst <= 0 and abs(float(sums.double().sum()) - total) < 1e-3 * total
+
+
+def test_weight_sums_of_many_rows_go_in_passes():
+    """512 rows to a KV head: two passes over the keys."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1200)
+    bt = Batch([200, 90], [64, 20], 1, 8, 128, 16, gen, tree=True).dev()
+    sums = torch.full((bt.nb, 1, 16), 0.25, device=DEV)
+    ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, 64, tree_mask=bt.d_words, kv_axis=0, weight_sums=sums)
+    for b in range(2):
+        e = bt.expect(b, 1 / math.sqrt(128))
+        blk, off = oa.token_slots(bt.table[b].tolist(), 16, bt.lens[b])
+        got = sums.cpu()[blk, 0, off].double()
+        got[: bt.lens[b] - bt.counts[b]] -= 0.25
+        rel = (2 * 132 * 2.0 ** -23 * e["logit"]).max() + 2.0 ** -20 + 512 * 2.0 ** -24
+        assert ((got - e["weight"][0]).abs() <= rel * e["weight"][0] + 2.0 ** -22 * (0.25 + e["weight"][0])).all()
+
+
+def test_eviction_with_counts_beyond_the_keep_rows():
+    from triattention_b200 import _native, ops
+    gen = torch.Generator().manual_seed(1300)
+    bt = Batch([90, 30], [0, 0], 2, 1, 64, 16, gen).dev()
+    view = ops.PagedCacheView.from_layers([bt.d_cache[0]], kv_axis=0)
+    sums = torch.rand((1, bt.nb, 2, 16), generator=gen).to(DEV)
+    a, b = sums.clone(), sums.clone()
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    other = bt.d_cache.clone()
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    keep = ops.evict_paged(view, view.layout(2, 1, bt.width), a, bt.d_table, bt.d_lens, i32([80, 20]), 33, 4, status=status)
+    assert int(status) == _native.DEV_BAD_LENGTH
+    view2 = ops.PagedCacheView.from_layers([other[0]], kv_axis=0)
+    want = ops.evict_paged(view2, view2.layout(2, 1, bt.width), b, bt.d_table, bt.d_lens, i32([33, 20]), 33, 4)
+    assert torch.equal(keep, want) and torch.equal(a, b) and torch.equal(bt.d_cache, other)
+
+
+def test_wait_timeout_in_the_attention_kernels_reports_status_and_returns():
+    """The test-only library build (waits of about a millisecond, barriers that expect 16 bytes more than ever arrive): the
+    attention kernels set TRIATTN_DEV_WAIT_TIMEOUT, drain and return, and the GPU stays usable."""
+    import os
+    import subprocess
+    import sys
+    import textwrap
+    from pathlib import Path
+
+    from triattention_b200 import _native, build
+    repo = Path(__file__).resolve().parent.parent
+    lib = build.build_library(short_wait=True)
+    code = textwrap.dedent("""
+        import sys, torch
+        sys.path.insert(0, %r)
+        from triattention_b200 import ops
+        bits = []
+        for n, g, D in ((1, 4, 128), (1, 16, 64), (8, 4, 128), (40, 4, 64)):
+            T, H = 900, 2
+            cache = torch.randn((2, 60, 16, H, D), device="cuda").bfloat16()
+            q = torch.randn((2 * n, H * g, D), device="cuda").bfloat16()
+            i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+            table = torch.arange(57, dtype=torch.int32, device="cuda").repeat(2, 1)
+            status, sums = i32([0]), torch.zeros((60, H, 16), device="cuda")
+            ops.attend_paged(q, cache, table, i32([T, T - 100]), i32([0, n, 2 * n]), n, weight_sums=sums, status=status)
+            torch.cuda.synchronize()
+            bits.append(int(status))
+        print("STATUS", *bits, torch.arange(10, device="cuda").sum().item())
+    """) % str(repo)
+    out = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, TRIATTN_B200_LIB=str(lib)), capture_output=True,
+                         text=True, timeout=300)
+    assert out.returncode == 0, out.stderr[-2000:]
+    line = [x for x in out.stdout.splitlines() if x.startswith("STATUS")][-1].split()
+    assert all(int(b) & _native.DEV_WAIT_TIMEOUT for b in line[1:5]) and int(line[5]) == 45, line

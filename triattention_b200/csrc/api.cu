@@ -328,7 +328,7 @@ static int compact_common(const triattn_paged_layout* layout, void* const* k_lay
                           const int32_t* block_table, const int32_t* seq_lens, const int32_t* keep,
                           int64_t keep_ls, int64_t keep_rs, int64_t keep_hs, const int32_t* keep_counts,
                           void* scratch, long long scratch_stream_bytes, int scratch_rows, bool preserve,
-                          uint32_t* device_status, void* stream, bool pdl = false) {
+                          uint32_t* device_status, void* stream, bool pdl = false, int keep_pitch = 0) {
   int rc = validate_layout(layout);
   if (rc != TRIATTN_OK) return rc;
   if (!k_layer_ptrs || !v_layer_ptrs || !block_table || !seq_lens || !keep || !keep_counts)
@@ -351,6 +351,7 @@ static int compact_common(const triattn_paged_layout* layout, void* const* k_lay
   p.keep_rs = keep_rs;
   p.keep_hs = keep_hs;
   p.keep_counts = keep_counts;
+  p.keep_pitch = keep_pitch;
   p.status = device_status;
   p.L = Y.num_layers;
   p.B = Y.num_reqs;
@@ -445,7 +446,7 @@ int triattn_evict_paged(const triattn_paged_layout* layout, void* const* k_layer
   if (rc != TRIATTN_OK) return rc;
   const int64_t hs = keep_pitch, rs = hs * Y.num_kv_heads, ls = rs * Y.num_reqs;
   return compact_common(layout, k_layer_ptrs, v_layer_ptrs, block_table, seq_lens, keep_out, ls, rs, hs, keep_counts,
-                        nullptr, 0, 0, false, device_status, stream, true);
+                        nullptr, 0, 0, false, device_status, stream, true, keep_pitch);
 }
 
 int triattn_rewrite_block_tables(int32_t* block_table, int num_reqs, int max_blocks_per_req, int block_size,

@@ -172,7 +172,7 @@ __device__ __forceinline__ bool attend_plan_run(const AttendParams& p, int runs,
     count = (int)(attend_first_tile(W, J, run + 1) - first);
     const bool here = first >= before && first < before + (long long)mine.tiles * mine.row_tiles;
     const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-    const int at = (int)__shfl_sync(0xffffffffu, first - before, from);  // inside one request's tiles: 32 bits
+    const long long at = __shfl_sync(0xffffffffu, first - before, from);
     c.b = from;
     c.r.T = __shfl_sync(0xffffffffu, mine.T, from);
     c.r.n = __shfl_sync(0xffffffffu, mine.n, from);
@@ -180,8 +180,8 @@ __device__ __forceinline__ bool attend_plan_run(const AttendParams& p, int runs,
     c.r.vlen = __shfl_sync(0xffffffffu, mine.vlen, from);
     c.r.tiles = __shfl_sync(0xffffffffu, mine.tiles, from);
     c.r.row_tiles = __shfl_sync(0xffffffffu, mine.row_tiles, from);
-    c.rt = at / c.r.tiles;
-    c.t = at - c.rt * c.r.tiles;
+    c.rt = at < (1ll << 31) ? (int)((unsigned)at / (unsigned)c.r.tiles) : (int)(at / c.r.tiles);
+    c.t = (int)(at - (long long)c.rt * c.r.tiles);
     __syncthreads();  // what the CTA has set up meanwhile
     return true;
   }

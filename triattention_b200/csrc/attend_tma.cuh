@@ -25,6 +25,11 @@ __device__ __forceinline__ void tma_load_tokens(uint32_t dst, const CUtensorMap*
       : "memory");
 }
 
+// the descriptor of a kernel parameter into the descriptor cache, ahead of the first load
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 // byte offset of 16-byte piece `piece` (0 .. D / 8 - 1) of token row `row` in a [tokens / 8][D / 64][8][128 B] swizzled tile
 template <int D>
 __device__ __forceinline__ uint32_t swz_off(int row, int piece) {
@@ -202,6 +207,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     }
     mbar_fence_init();
     ring.err = ring.gaps = 0;
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
   }
   grid_dependency_wait();
   trigger_dependents();
@@ -537,6 +544,7 @@ __global__ void __launch_bounds__(kObserveThreads<D>, 1)
     }
     mbar_fence_init();
     ring.err = ring.gaps = 0;
+    prefetch_map(&kmap);
   }
   grid_dependency_wait();
   trigger_dependents();

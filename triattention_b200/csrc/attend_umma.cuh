@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   __shared__ AttendPlanShared<THREADS> plan;
   __shared__ uint32_t s_tmem;
   __shared__ float pair_val[2][NT][2][128];  // what the two threads of a row tell each other (tiles in turn)
-  __shared__ bool pair_over[2][NT][2][4];
+  __shared__ bool pair_over[2][NT][2][4], row_over[2][NT][2][128];
   __shared__ int odd_piece;  // the last piece in which a query token's value held an infinity or NaN
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
@@ -140,6 +140,8 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     mbar_init(smem_u32(&drained), 1);
     mbar_fence_init();
     ring.err = ring.gaps = 0;
+    prefetch_map(&kmap);
+    prefetch_map(&vmap);
     odd_piece = -1;
   }
   grid_dependency_wait();
@@ -300,8 +302,12 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
           }
           edge = low_pos < 0 || top_pos + 8 > ctx;
         }
-        if (dead) {
-          if (!idle) pair_sync();
+        if (dead) {  // as many barriers as a partner that is not (yet) dead passes
+          if (!idle) {
+            if (x > 0 && lane == 0) pair_over[n & 1][g][half][wid & 3] = false;
+            pair_sync();
+            if (x > 0 && pair_over[n & 1][g][half ^ 1][wid & 3]) pair_sync();
+          }
           continue;
         }
         if (!idle) {
@@ -334,10 +340,12 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
             }
           };
           uint32_t pv[2][16];  // P, kept until it is known to be in range: the logits stay where they are until then
-          float sum;
+          float sum = 0.f;
+          bool over = true;  // this thread's half of the row asks for a new reference
           for (bool raise = x == 0;;) {
             if (raise) {
-              // the reference becomes the maximum so far (of both threads); what the row has accumulated is rescaled
+              // the reference of a row that asks for it becomes the maximum so far (of both threads), and what the row has
+              // accumulated is rescaled; the warp's other rows stay as they are
               float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
               for (int q = 0; q < 2; ++q) {
@@ -348,8 +356,9 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
               }
               float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
               pair_val[n & 1][g][half][row] = mx;
+              row_over[n & 1][g][half][row] = over;
               pair_sync();
-              mx = fmaxf(m, fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]) * p.scale_log2);
+              mx = over || row_over[n & 1][g][half ^ 1][row] ? fmaxf(m, fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]) * p.scale_log2) : m;
               const float f = mx > m ? ex2(m - mx) : 1.f;
               l *= f;
               m = mx;
@@ -388,10 +397,11 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
             la = fadd2(la, lb);
             sum = la.x + la.y;
             if (raise) break;  // nothing exceeds 1
-            const bool over = __any_sync(0xffffffffu, !(sum < kTreeSlack) || m == -INFINITY);
-            if (lane == 0) pair_over[n & 1][g][half][wid & 3] = over;
+            over = !(sum < kTreeSlack) || m == -INFINITY;
+            const bool any = __any_sync(0xffffffffu, over);
+            if (lane == 0) pair_over[n & 1][g][half][wid & 3] = any;
             pair_sync();
-            if (!over && !pair_over[n & 1][g][half ^ 1][wid & 3]) break;
+            if (!any && !pair_over[n & 1][g][half ^ 1][wid & 3]) break;
             raise = true;
           }
           l += sum;

@@ -281,6 +281,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_blocks_kernel(const __grid_
   extern __shared__ __align__(16) unsigned char pick_smem[];
   __shared__ TopkShared<kPickThreads> sh;
   grid_dependency_wait();
+  trigger_dependents();
   const int h = blockIdx.x, b = blockIdx.y;
   unsigned err = 0u;
   const BlocksReq r = blocks_req(p, b, err);

@@ -33,6 +33,7 @@ struct CompactParams {
   const int32_t* keep;
   long long keep_ls, keep_rs, keep_hs;
   const int32_t* keep_counts;
+  int keep_pitch;  // entries of a keep row where the caller states them, else 0: no more are read
   uint32_t* status;
   int L, B, Hkv, bs, num_blocks, max_blocks;
   long long block_stride, token_stride, head_stride;  // elements (multiples of 8)
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(THREADS) compact_paged_kernel(const __grid_con
   const int head = blockIdx.x >> 1;
   const int l = blockIdx.y, b = blockIdx.z;
   const int seq_len = min(p.seq_lens[b], p.max_blocks * p.bs);
-  const int k = min(p.keep_counts[b], seq_len);
+  const int k = min(min(p.keep_counts[b], seq_len), p.keep_pitch > 0 ? p.keep_pitch : seq_len);
   if (k <= 0) return;
   const int32_t* keep = p.keep + l * p.keep_ls + b * p.keep_rs + head * p.keep_hs;
   const int32_t* bt = p.block_table + (size_t)b * p.max_blocks;

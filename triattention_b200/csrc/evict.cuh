@@ -48,6 +48,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   }
   n = max(n, 0);
   const int k = max(0, min(p.keep_counts[b], min(n, p.pitch)));
+  if (p.keep_counts[b] > p.pitch && n > p.pitch) err |= TRIATTN_DEV_BAD_LENGTH;  // the row holds no more
   const int guard = p.prefill_lens != nullptr ? p.prefill_lens[b] : 0;
   const int recent = n - p.window;
   const int32_t* bt = p.block_table + (long long)b * p.max_blocks;
