@@ -296,6 +296,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_blocks_kernel(const __grid_
         const float w = __uint_as_float(bits);
         return float_to_ordered(w == w ? w + 0.f : -INFINITY);  // -0 ranks as 0, NaN last
       },
+      [&](int rank, int i) { out[rank] = i; },
       [&](const bool(&sel)[4], const int(&rank)[4], const int(&at)[4], const unsigned(&)[4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)

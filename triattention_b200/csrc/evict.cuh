@@ -14,7 +14,7 @@
 namespace triattn {
 
 constexpr int kEvictLongRow = 8192;  // rows that may be longer run 1024 threads, one CTA per SM; others 512, two per SM
-constexpr int kEvictCap = 49152;  // keys of a row kept in shared memory (192 KB)
+constexpr int kEvictCap = 49152;  // keys of a row kept in shared memory (192 KB); below 65536, see topk_row
 
 struct EvictParams {
   float* sums;  // [L, num_blocks, Hkv, bs]
@@ -78,13 +78,14 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
         if (bits == 0x7fffffffu) return 0x80000000u;  // -0 ranks as 0
         return bits > kTop ? 0u : bits;               // NaN last
       },
+      [&](int rank, int i) { out[rank] = i; },
       [&](const bool(&sel)[4], const int(&rank)[4], const int(&at)[4], const unsigned(&bits)[4]) {
-        if (!cached) __syncthreads();  // the run's sums are in registers before any of its destinations is written
+        __syncthreads();  // the run's sums are in registers before any of its destinations is written
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (!sel[j]) continue;
           out[rank[j]] = at[j];
-          if (!cached && rank[j] != at[j]) {
+          if (rank[j] != at[j]) {
             const long long to = slot(rank[j]);
             if (to >= 0) sums[to] = ordered_to_float(bits[j]);
           }

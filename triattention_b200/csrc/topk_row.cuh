@@ -40,13 +40,14 @@ __device__ __forceinline__ unsigned topk_scan(unsigned v, TopkShared<THREADS>& s
   return before + incl - v;
 }
 
-// where(i) -> the address index of element i < n, fetch(index) -> its bits, key(bits, i) -> what it is ranked by.  emit(sel, rank, i, bits) is called by all threads
-// together for runs of 4 * THREADS consecutive elements in ascending order (four to a thread): where sel holds, element i is
-// chosen with that rank (0 .. k-1, ascending with i).  With n <= cap (a multiple of 4; bits 16-byte aligned)
-// the row is read once, before the first emit.
-template <int THREADS, class Where, class Fetch, class Key, class Emit>
+// where(i) -> the address index of element i < n, fetch(index) -> its bits, key(bits, i) -> what it is ranked by.  put(rank, i) is called once for every chosen element
+// (rank 0 .. k-1, ascending with i).  Rows of n <= cap (a multiple of 4; bits 16-byte aligned) are read once; they are
+// counted and put segment by segment, a thread's segment being an odd number of consecutive elements (no bank conflicts), with a
+// single scan over the threads.  Longer rows are read again in every pass, and put in runs of 4 * THREADS elements: all threads
+// call run(sel, rank, i, bits) together, run by run in ascending order, before the puts of the next one.
+template <int THREADS, class Where, class Fetch, class Key, class Put, class Run>
 __device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, TopkShared<THREADS>& sh, Where where,
-                                         Fetch fetch, Key key, Emit emit) {
+                                         Fetch fetch, Key key, Put put, Run run) {
   constexpr int VEC = 4;
   const int tid = threadIdx.x;
   const bool cached = n <= cap;
@@ -75,20 +76,8 @@ __device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, 
       for (int j = 0; j < VEC; ++j) v[j] = i + j < n ? bits_at(i + j) : 0u;
     }
   };
-  if (k >= n) {
-    __syncthreads();
-    for (int i0 = 0; i0 < n; i0 += THREADS * VEC) {
-      bool sel[VEC];
-      int rank[VEC], at[VEC];
-      unsigned v[VEC] = {0u, 0u, 0u, 0u};
-      if (i0 + tid * VEC < n) four_at(i0 + tid * VEC, v);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        at[j] = rank[j] = i0 + tid * VEC + j;
-        sel[j] = at[j] < n;
-      }
-      emit(sel, rank, at, v);
-    }
+  if (k >= n) {  // everything stays where it is
+    for (int i = tid; i < n; i += THREADS) put(i, i);
     return;
   }
   if (tid == 0) {
@@ -135,6 +124,26 @@ __device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, 
     __syncthreads();
   }
   const unsigned kth = sh.prefix, need_eq = sh.remaining;
+  if (cached) {
+    const int len = ((n + THREADS - 1) / THREADS) | 1, i0 = min(tid * len, n), i1 = min(i0 + len, n);
+    unsigned gt = 0u, eq = 0u;
+    for (int i = i0; i < i1; ++i) {
+      const unsigned x = key(bits[i], i);
+      gt += x > kth ? 1u : 0u;
+      eq += x == kth ? 1u : 0u;
+    }
+    // both prefixes in one scan where the counts fit 16 bits each (n < 65536: cap is below that)
+    unsigned total;
+    const unsigned before = topk_scan<THREADS>(gt | eq << 16, sh, total);
+    unsigned eq_before = before >> 16, rank = (before & 0xffffu) + min(eq_before, need_eq);
+    for (int i = i0; i < i1; ++i) {
+      const unsigned x = key(bits[i], i);
+      const bool border = x == kth;
+      if (x > kth || (border && eq_before < need_eq)) put((int)rank++, i);
+      eq_before += border ? 1u : 0u;
+    }
+    return;
+  }
   unsigned base_eq = 0u, base_out = 0u;
   for (int i0 = 0; i0 < n; i0 += THREADS * VEC) {
     bool sel[VEC], eq[VEC];
@@ -158,7 +167,7 @@ __device__ __forceinline__ void topk_row(int n, int k, unsigned* bits, int cap, 
       before += (sel[j] ? 1u : 0u) + (eq[j] ? 0x10000u : 0u);
       sel[j] = sel[j] || (eq[j] && eq_before < need_eq);
     }
-    emit(sel, rank, at, v);
+    run(sel, rank, at, v);
     const unsigned eq_after = base_eq + (total >> 16);
     base_out += (total & 0xffffu) + (min(eq_after, need_eq) - min(base_eq, need_eq));
     base_eq = eq_after;
