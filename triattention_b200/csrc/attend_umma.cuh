@@ -526,4 +526,192 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   }
 }
 
+// ------------------------------------------------------------------------------------------ weight sums of many rows
+// The second pass over K (see attend.cuh for the formula) for more than 16 rows: S^T = K Q^T with 128 tokens as the rows of the
+// product (M) and up to 256 query rows as its columns (N), so that a thread has one token and adds up its row of tensor memory: no
+// exchange between threads.  K tiles come in through the ring (two loading warps), one thread issues the products into two
+// accumulators, two groups of four warps empty them in turn.  Bound by the exponentials, N per token: at 128 rows as long as the
+// keys' transfer.  More than 256 rows: one launch per 256 (row0), the first sets or adds, the others add.
+constexpr int kObserveMmaRows = 256;
+template <int D>
+constexpr int kObserveMmaStages = D == 64 ? 6 : 4;
+constexpr int kObserveMmaThreads = (8 + 1 + 2) * 32;
+template <int D>
+constexpr size_t observe_mma_smem_bytes() {
+  return 1024 + (size_t)kObserveMmaStages<D> * 128 * D * 2 + (size_t)kObserveMmaRows * D * 2;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kObserveMmaThreads, 1)
+    attend_observe_mma_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap, const int runs,
+                              const int row0) {
+  constexpr int TILE = 128, STAGES = kObserveMmaStages<D>, THREADS = kObserveMmaThreads, RMAX = kObserveMmaRows;
+  constexpr int kAll = 1 << 24;  // all rows of a (request, KV head) in one segment
+  constexpr uint32_t kTileBytes = TILE * D * 2, kGroup = D * 16;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ AttendRing<TILE, STAGES, true> ring;
+  __shared__ AttendPlanShared<THREADS> plan;
+  __shared__ uint64_t acc_full[2], acc_empty[2], q_ready, drained;
+  __shared__ __align__(16) float lse2[RMAX];
+  __shared__ unsigned long long words[RMAX];
+  __shared__ uint32_t s_tmem;
+  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&ring.full[0][s]), 1);
+      mbar_init(smem_u32(&ring.empty[0][s]), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(&acc_full[a]), 1);
+      mbar_init(smem_u32(&acc_empty[a]), 4);
+    }
+    mbar_init(smem_u32(&q_ready), 8);
+    mbar_init(smem_u32(&drained), 1);
+    mbar_fence_init();
+    ring.err = ring.gaps = 0;
+    prefetch_map(&kmap);
+  }
+  grid_dependency_wait();
+  trigger_dependents();
+  const int run = (int)blockIdx.x / p.Hkv;
+  AttendCursor c;
+  int count;
+  if (!attend_plan_run<THREADS>(p, runs, 2, run, TILE, kAll, plan, c, count)) return;  // nothing allocated yet
+  c.h = (int)blockIdx.x - run * p.Hkv;
+  if (wid == 8) {
+    tmem_alloc(smem_u32(&s_tmem), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, q_base = base + STAGES * kTileBytes;
+  unsigned char* const q_smem = smem_raw + (q_base - smem_u32(smem_raw));
+  // columns of the product for a request's rows of this pass: a multiple of 32 (what the threads read at a time)
+  auto columns = [&](const AttendReq& r) { return (min(max(r.n * p.g - row0, 1), RMAX) + 31) & ~31; };
+
+  if (wid > 8) {
+    attend_produce<D, TILE, STAGES>(p, &kmap, 0, c, count, kAll, base, kTileBytes, ring.full[0], ring.empty[0], ring, wid - 9, 2);
+  } else if (wid == 8) {
+    if (elect_one()) {
+      bool ok = true;
+      int piece_no = 0;
+      for (int it = 0; it < count && ok; ++piece_no) {
+        const int piece = min(c.r.tiles - c.t, count - it);
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(columns(c.r) >> 3) << 17) | ((128u >> 4) << 24);
+        ok = thread_wait(q_ready, (uint32_t)piece_no & 1u, &ring.err, p.status);
+        for (int x = 0; x < piece && ok; ++x) {
+          const int n = it + x, s = n % STAGES, a = n & 1;
+          ok = thread_wait(ring.full[0][s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status) &&
+               (n < 2 || thread_wait(acc_empty[a], (uint32_t)((n >> 1) - 1) & 1u, &ring.err, p.status));
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t dk = umma_desc(base + (uint32_t)s * kTileBytes, 16u, kGroup), dq = umma_desc(q_base, 16u, 1024u);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16(tmem + (uint32_t)a * 256u, dk + (uint64_t)((k & 3) * 2 + (k >> 2) * (1024 >> 4)),
+                      dq + (uint64_t)((k & 3) * 2 + (k >> 2) * ((RMAX * 128) >> 4)), idesc, k ? 1u : 0u);
+          umma_commit(smem_u32(&acc_full[a]));
+          umma_commit(smem_u32(&ring.empty[0][s]));
+        }
+        it += piece;
+        c.t += piece - 1;
+        if (it < count) attend_advance(p, c, TILE, kAll);
+      }
+      if (!ok) {  // a wait ran out: the operands must outlive what has been issued
+        umma_commit(smem_u32(&drained));
+        mbar_wait_bounded(smem_u32(&drained), 0u);
+      }
+    }
+    __syncwarp();
+  } else {
+    const int group = wid >> 2, token = (wid & 3) * 32 + lane;
+    const uint32_t t_acc = tmem + ((uint32_t)((wid & 3) * 32) << 16) + (uint32_t)group * 256u;
+    auto meet = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+    bool dead = false;
+    for (int it = 0; it < count;) {
+      const int piece = min(c.r.tiles - c.t, count - it);
+      const int R = c.r.n * p.g, ctx = c.r.T - c.r.n, cols = columns(c.r);
+      meet();  // the tiles of the piece before have been emptied: its rows are not needed any more
+      for (int x = tid; x < cols * (D / 8); x += 256) {
+        const int row = x / (D / 8), pc = x % (D / 8), r = row0 + row;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (r < R) {
+          const int i = r / p.g, j = r - i * p.g;
+          w = *reinterpret_cast<const uint4*>(p.q + (long long)(c.r.q0 + i) * p.q_ts + (long long)(c.h * p.g + j) * p.q_hs + pc * 8);
+        }
+        *reinterpret_cast<uint4*>(q_smem + (pc >> 3) * (RMAX * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4)) = w;
+      }
+      if (tid < cols) {
+        const int r = row0 + tid;
+        float z = INFINITY;  // rows that do not exist, or see nothing, add exp2(-inf) = 0
+        unsigned long long w = 0ull;
+        if (r < R) {
+          const int i = r / p.g, j = r - i * p.g;
+          const float e = p.lse[(long long)(c.r.q0 + i) * (p.Hkv * p.g) + c.h * p.g + j];
+          if (e != -INFINITY) z = e * kLog2e;
+          w = attend_word(p, c.r, i);
+        }
+        lse2[tid] = z;
+        words[tid] = w;
+      }
+      fence_proxy_async();
+      meet();
+      if (lane == 0) mbar_arrive(smem_u32(&q_ready));
+      for (int x = (group + it) & 1; x < piece; x += 2) {  // tiles whose accumulator is this group's
+        const int n = it + x;
+        dead = dead || !ring_wait(acc_full[group], (uint32_t)(n >> 1) & 1u, &ring.err, p.status);
+        if (dead) break;
+        tc_fence_after();
+        const int q8 = ring.pos[n % kPosRing<TILE>][token >> 3], pos = q8 + (token & 7);
+        float* at = nullptr;
+        float old = 0.f;
+        if (q8 >= 0 && pos < c.r.T) {
+          at = p.sums + ((long long)ring.blk[n % kPosRing<TILE>][token >> 3] * p.Hkv + c.h) * p.bs + pos % p.bs;
+          // a query's own token, or sums that start anew: whatever the slot holds is nobody's
+          if (row0 > 0 || (p.reset_sums == 0 && pos < ctx)) old = *at;
+        }
+        const bool own = __any_sync(0xffffffffu, at != nullptr && pos >= ctx);
+        float2 wa = make_float2(0.f, 0.f), wb = make_float2(0.f, 0.f);
+        const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+#pragma unroll 1
+        for (int c0 = 0; c0 < cols; c0 += 32) {
+          uint32_t sv[32];
+          tmem_ld32(t_acc + (uint32_t)c0, sv);
+          tmem_ld_wait32(sv);
+          if (own && pos >= ctx) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (!((words[c0 + j] >> ((pos - ctx) & 63)) & 1ull)) sv[j] = 0xff800000u;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 z = *reinterpret_cast<const float4*>(lse2 + c0 + j);
+            float2 e = ffma2(make_float2(__uint_as_float(sv[j]), __uint_as_float(sv[j + 1])), sc2, make_float2(-z.x, -z.y));
+            float2 f = ffma2(make_float2(__uint_as_float(sv[j + 2]), __uint_as_float(sv[j + 3])), sc2, make_float2(-z.z, -z.w));
+            wa = fadd2(wa, make_float2(ex2(e.x), ex2(e.y)));
+            wb = fadd2(wb, make_float2(ex2(f.x), ex2(f.y)));
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&acc_empty[group]));
+        wa = fadd2(wa, wb);
+        if (at != nullptr) *at = old + (wa.x + wa.y);
+      }
+      it += piece;
+      c.t += piece - 1;
+      if (it < count) attend_advance(p, c, TILE, kAll);
+    }
+  }
+  // all roles are done (or gave up): free the tensor memory
+  tc_fence_before();
+  __syncthreads();
+  if (wid == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 }  // namespace triattn
