@@ -160,29 +160,13 @@ int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensor
   rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)(max_row_tiles * ((a.rows + 7) / 8)), (unsigned)p.Hkv, (unsigned)p.B),
                      dim3(kCombineThreads), 0, st, true, p, a.runs, a.tile, a.rows);
   if (rc != TRIATTN_OK || p.sums == nullptr) return rc;
-  if constexpr (D <= 128) {
-    // more than 16 rows to a KV head: the tensor cores' tokens-by-rows product (prompt end of 2 x 14300 tokens, 128 rows: see the
-    // kernel); at most 16 rows leave nothing for it to gain on mma.sync
-    if (observe_map != nullptr && p.max_q * p.g > 16) {
-      constexpr size_t smem = observe_mma_smem_bytes<D>();
-      if (!ensure_dynamic_smem<attend_observe_mma_kernel<D>>(smem)) return TRIATTN_ERR_CUDA;
-      for (int row0 = 0; row0 < p.max_q * p.g; row0 += kObserveMmaRows) {
-        AttendParams o = p;
-        o.box = observe_box;
-        rc = launch_kernel(attend_observe_mma_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kObserveMmaThreads), smem, st,
-                           true, o, *observe_map, observe_runs, row0);
-        if (rc != TRIATTN_OK) return rc;
-      }
-      return TRIATTN_OK;
-    }
-  }
   if (observe_map != nullptr) {
-    constexpr size_t smem = observe_tiled_smem_bytes<D>();
-    if (!ensure_dynamic_smem<attend_observe_tiled_kernel<D>>(smem)) return TRIATTN_ERR_CUDA;
-    for (int row0 = 0; row0 < p.max_q * p.g; row0 += kObserveTileRows<D>) {
+    constexpr size_t smem = observe_mma_smem_bytes<D>();
+    if (!ensure_dynamic_smem<attend_observe_mma_kernel<D>>(smem)) return TRIATTN_ERR_CUDA;
+    for (int row0 = 0; row0 < p.max_q * p.g; row0 += kObserveRowsMax<D>) {
       AttendParams o = p;
       o.box = observe_box;
-      rc = launch_kernel(attend_observe_tiled_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kObserveThreads<D>), smem, st,
+      rc = launch_kernel(attend_observe_mma_kernel<D>, dim3((unsigned)(observe_runs * p.Hkv)), dim3(kObserveMmaThreads), smem, st,
                          true, o, *observe_map, observe_runs, row0);
       if (rc != TRIATTN_OK) return rc;
     }
@@ -275,10 +259,8 @@ int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache
     return TRIATTN_ERR_CUDA;
   int observe_runs = 0, observe_box = 128;
   if (weight_sums != nullptr) {
-    const bool many = Y.head_dim <= 128 && max_query_len * Y.group_size > 16;
     observe_runs = (int)std::min<long long>(attend_max_runs(tiled || Y.head_dim > 128 ? kSMs : 2 * kSMs, Y.num_kv_heads),
-                                            attend_max_tiles(Y, 1, num_listed, tiled ? 32 : kAttendTile, 64));
-    observe_box = many ? 128 : Y.head_dim == 64 ? kObserveTile<64> : kObserveTile<128>;
+                                            attend_max_tiles(Y, 1, num_listed, tiled ? 128 : kAttendTile, 64));
     for (; Y.block_size % observe_box && observe_box > 8; observe_box /= 2) {
     }
     if (tiled && !encode_cache_map(&om, k_cache, Y, observe_box)) return TRIATTN_ERR_CUDA;

@@ -12,8 +12,6 @@
 
 #include <cuda.h>  // CUtensorMap
 
-#include <type_traits>
-
 #include "attend.cuh"
 
 namespace triattn {
@@ -496,185 +494,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     it += piece;
     c.t += piece - 1;
     if (it < count) attend_advance(p, c, TILE, ROWS);
-  }
-}
-
-// ------------------------------------------------------------------------------------------ weight sums
-// The second pass of attend_observe_kernel (see attend.cuh for the formula), K tiles from the ring.  S^T = K Q^T: 32 tokens of a
-// warp's tile are the A operand (two 16-row fragments, held in registers), the query rows are the columns, eight at a
-// time from shared memory; a token's sum over the rows stays inside four lanes.  The old sums are requested when the
-// tokens are taken up.  Two warps load, tile by tile in turn: a warp issues a load every 80 cycles or so, and a box is only
-// 16 D bytes per 8 tokens.
-// Calls with more than kObserveRows<D> rows run the kernel once per that many (row0): the first pass sets or adds, the
-// others add.
-template <int D>
-constexpr int kObserveWarps = D == 256 ? 6 : 8;
-template <int D>
-constexpr int kObserveThreads = (kObserveWarps<D> + 2) * 32;
-template <int D>
-constexpr int kObserveTile = D == 64 ? 64 : 32;  // tokens: 8 KB (D = 256: 16 KB)
-template <int D>
-constexpr int kObserveStages = D == 256 ? 6 : 16;
-template <int D>
-constexpr int kObserveTileRows = D == 256 ? 128 : 256;
-template <int D>
-constexpr size_t observe_tiled_smem_bytes() {
-  return 1024 + (size_t)kObserveStages<D> * kObserveTile<D> * D * 2 + (size_t)kObserveTileRows<D> * D * 2;
-}
-
-template <int D>
-__global__ void __launch_bounds__(kObserveThreads<D>, 1)
-    attend_observe_tiled_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap, const int runs,
-                                const int row0) {
-  constexpr int TILE = kObserveTile<D>, STAGES = kObserveStages<D>, WARPS = kObserveWarps<D>, THREADS = kObserveThreads<D>;
-  constexpr int RMAX = kObserveTileRows<D>;
-  constexpr int kAll = 1 << 24;  // all rows of a (request, KV head) in one segment
-  static_assert(STAGES % WARPS == 0, "a stage belongs to one warp");
-  constexpr uint32_t kTileBytes = TILE * D * 2;
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ AttendRing<TILE, STAGES, true> ring;
-  __shared__ AttendPlanShared<THREADS> plan;
-  __shared__ float lse2[RMAX];
-  __shared__ unsigned long long words[RMAX];
-  const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
-  if (tid == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&ring.full[0][s]), 1);
-      mbar_init(smem_u32(&ring.empty[0][s]), 1);
-    }
-    mbar_fence_init();
-    ring.err = ring.gaps = 0;
-    prefetch_map(&kmap);
-  }
-  grid_dependency_wait();
-  trigger_dependents();
-  const int run = (int)blockIdx.x / p.Hkv;
-  AttendCursor c;
-  int count;
-  if (!attend_plan_run<THREADS>(p, runs, WARPS, run, TILE, kAll, plan, c, count)) return;
-  c.h = (int)blockIdx.x - run * p.Hkv;
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  unsigned char* const q_smem = smem_raw + (base - smem_u32(smem_raw)) + STAGES * kTileBytes;
-  const uint32_t q_base = base + STAGES * kTileBytes;
-  if (wid >= WARPS) {
-    attend_produce<D, TILE, STAGES>(p, &kmap, 0, c, count, kAll, base, kTileBytes, ring.full[0], ring.empty[0], ring, wid - WARPS, 2);
-    return;
-  }
-  auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
-  bool dead = false;
-  for (int it = 0; it < count;) {
-    const int piece = min(c.r.tiles - c.t, count - it);
-    const int R = c.r.n * p.g, ctx = c.r.T - c.r.n;
-    const int live = min(R - row0, RMAX), nt = (max(live, 0) + 7) >> 3;  // 8-row groups of this pass
-    meet();
-    for (int x = tid; x < nt * 8 * (D / 8); x += WARPS * 32) {
-      const int row = x / (D / 8), pc = x % (D / 8), r = row0 + row;
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (r < R) {
-        const int i = r / p.g, j = r - i * p.g;
-        w = *reinterpret_cast<const uint4*>(p.q + (long long)(c.r.q0 + i) * p.q_ts + (long long)(c.h * p.g + j) * p.q_hs + pc * 8);
-      }
-      *reinterpret_cast<uint4*>(q_smem + tile_off<D>(row, pc)) = w;
-    }
-    for (int row = tid; row < nt * 8; row += WARPS * 32) {
-      const int r = row0 + row;
-      float z = INFINITY;  // rows that do not exist, or see nothing, add exp2(-inf) = 0
-      unsigned long long w = 0ull;
-      if (r < R) {
-        const int i = r / p.g, j = r - i * p.g;
-        const float e = p.lse[(long long)(c.r.q0 + i) * (p.Hkv * p.g) + c.h * p.g + j];
-        if (e != -INFINITY) z = e * kLog2e;
-        w = attend_word(p, c.r, i);
-      }
-      lse2[row] = z;
-      words[row] = w;
-    }
-    meet();
-    for (int x0 = (wid + WARPS - it % WARPS) % WARPS; x0 < piece; x0 += WARPS) {
-      const int n = it + x0, s = n % STAGES;
-      if (dead || !ring_wait(ring.full[0][s], (uint32_t)(n / STAGES) & 1u, &ring.err, p.status)) {
-        dead = true;
-        break;
-      }
-      const uint32_t kb = base + (uint32_t)s * kTileBytes;
-      // In the products a lane has tokens lane / 4 + 8 i of 32; of the sums it keeps one token's, i = lane % 4.
-      int pos[TILE / 8];
-      float old[TILE / 32];
-      float* at[TILE / 32];
-#pragma unroll
-      for (int i = 0; i < TILE / 8; ++i) {
-        const int q8 = ring.pos[n % kPosRing<TILE>][i];
-        pos[i] = q8 < 0 || q8 + (lane >> 2) >= c.r.T ? -1 : q8 + (lane >> 2);
-      }
-#pragma unroll
-      for (int y = 0; y < TILE / 32; ++y) {
-        const int run8 = y * 4 + (lane & 3), q8 = ring.pos[n % kPosRing<TILE>][run8], t = q8 + (lane >> 2);
-        old[y] = 0.f;
-        at[y] = nullptr;
-        if (q8 >= 0 && t < c.r.T) {
-          at[y] = p.sums + ((long long)ring.blk[n % kPosRing<TILE>][run8] * p.Hkv + c.h) * p.bs + t % p.bs;
-          // a query's own token, or sums that start anew: whatever the slot holds is nobody's
-          if (row0 > 0 || (p.reset_sums == 0 && t < ctx)) old[y] = *at[y];
-        }
-      }
-#pragma unroll
-      for (int sub = 0; sub < TILE; sub += 32) {
-        uint32_t kf[2][D / 16][4];
-  #pragma unroll
-        for (int a = 0; a < 2; ++a)
-  #pragma unroll
-          for (int k = 0; k < D / 16; ++k) ldsm_x4(kf[a][k], kb + swz_off<D>(sub + a * 16 + (lane & 15), k * 2 + (lane >> 4)));
-        const int* ps = pos + (sub >> 3);
-        const bool own = max(max(ps[0], ps[1]), max(ps[2], ps[3])) >= ctx;
-        float w[4] = {0.f, 0.f, 0.f, 0.f};
-        auto rows8 = [&](int j, auto pair) {  // 8 query rows, or 16: the products of two groups overlap
-          constexpr int G = decltype(pair)::value;
-          float e[G][2][4] = {};
-#pragma unroll
-          for (int k = 0; k < D / 32; ++k) {
-#pragma unroll
-            for (int y = 0; y < G; ++y) {
-              uint32_t qf[4];
-              ldsm_x4(qf, q_base + tile_off<D>((j + y) * 8 + (lane & 7), k * 4 + (lane >> 3)));
-#pragma unroll
-              for (int a = 0; a < 2; ++a) {
-                mma_bf16(e[y][a], kf[a][2 * k], qf[0], qf[1]);
-                mma_bf16(e[y][a], kf[a][2 * k + 1], qf[2], qf[3]);
-              }
-            }
-          }
-#pragma unroll
-          for (int y = 0; y < G; ++y) {
-            const int row = (j + y) * 8 + (lane & 3) * 2;
-            const float z0 = lse2[row], z1 = lse2[row + 1];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float p0 = ex2(fmaf(e[y][i >> 1][(i & 1) * 2], p.scale_log2, -z0)), p1 = ex2(fmaf(e[y][i >> 1][(i & 1) * 2 + 1], p.scale_log2, -z1));
-              if (own && ps[i] >= ctx) {
-                p0 = (words[row] >> (ps[i] - ctx)) & 1ull ? p0 : 0.f;
-                p1 = (words[row + 1] >> (ps[i] - ctx)) & 1ull ? p1 : 0.f;
-              }
-              w[i] += p0 + p1;
-            }
-          }
-        };
-        int j = 0;
-        for (; j + 1 < nt; j += 2) rows8(j, std::integral_constant<int, 2>{});
-        if (j < nt) rows8(j, std::integral_constant<int, 1>{});
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] += __shfl_xor_sync(0xffffffffu, w[i], 1);
-          w[i] += __shfl_xor_sync(0xffffffffu, w[i], 2);
-        }
-        const float w01 = lane & 1 ? w[1] : w[0], w23 = lane & 1 ? w[3] : w[2];
-        if (at[sub / 32] != nullptr) *at[sub / 32] = old[sub / 32] + (lane & 2 ? w23 : w01);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ring.empty[0][s]));
-    }
-    it += piece;
-    c.t += piece - 1;
-    if (it < count) attend_advance(p, c, TILE, kAll);
   }
 }
 

@@ -526,26 +526,29 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   }
 }
 
-// ------------------------------------------------------------------------------------------ weight sums of many rows
-// The second pass over K (see attend.cuh for the formula) for more than 16 rows: S^T = K Q^T with 128 tokens as the rows of the
-// product (M) and up to 256 query rows as its columns (N), so that a thread has one token and adds up its row of tensor memory: no
-// exchange between threads.  K tiles come in through the ring (two loading warps), one thread issues the products into two
-// accumulators, two groups of four warps empty them in turn.  Bound by the exponentials, N per token: at 128 rows as long as the
-// keys' transfer.  More than 256 rows: one launch per 256 (row0), the first sets or adds, the others add.
-constexpr int kObserveMmaRows = 256;
+// ------------------------------------------------------------------------------------------ weight sums
+// The second pass over K (see attend.cuh for the formula): S^T = K Q^T with 128 tokens as the rows of the product (M) and up to
+// 256 query rows as its columns (N), so that a thread has one token and adds up its row of tensor memory: no exchange between
+// threads.  K tiles come in through the ring (two loading warps: a warp issues a load every 80 cycles or so), one thread issues
+// the products into two accumulators, two groups of four warps empty them in turn.  Bound by the keys' bytes and, from about 128 rows,
+// by the exponentials, N per token.  (With the products on mma.sync and a token's sum spread over four lanes, 128 rows took 43
+// instead of 27 us for 2 x 14300 tokens and 8 heads, and a decode step of 16 x 4600 tokens 6 us longer.)  More rows than N: one launch per N
+// (row0), the first sets or adds, the others add.
 template <int D>
-constexpr int kObserveMmaStages = D == 64 ? 6 : 4;
+constexpr int kObserveRowsMax = D == 256 ? 128 : 256;
+template <int D>
+constexpr int kObserveMmaStages = D == 64 ? 6 : D == 128 ? 4 : 2;
 constexpr int kObserveMmaThreads = (8 + 1 + 2) * 32;
 template <int D>
 constexpr size_t observe_mma_smem_bytes() {
-  return 1024 + (size_t)kObserveMmaStages<D> * 128 * D * 2 + (size_t)kObserveMmaRows * D * 2;
+  return 1024 + (size_t)kObserveMmaStages<D> * 128 * D * 2 + (size_t)kObserveRowsMax<D> * D * 2;
 }
 
 template <int D>
 __global__ void __launch_bounds__(kObserveMmaThreads, 1)
     attend_observe_mma_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap, const int runs,
                               const int row0) {
-  constexpr int TILE = 128, STAGES = kObserveMmaStages<D>, THREADS = kObserveMmaThreads, RMAX = kObserveMmaRows;
+  constexpr int TILE = 128, STAGES = kObserveMmaStages<D>, THREADS = kObserveMmaThreads, RMAX = kObserveRowsMax<D>;
   constexpr int kAll = 1 << 24;  // all rows of a (request, KV head) in one segment
   constexpr uint32_t kTileBytes = TILE * D * 2, kGroup = D * 16;
   extern __shared__ unsigned char smem_raw[];
