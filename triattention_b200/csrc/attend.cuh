@@ -365,6 +365,9 @@ __device__ __forceinline__ unsigned long long attend_word(const AttendParams& p,
   return i >= 63 ? ~0ull : ((2ull << i) - 1ull);
 }
 
+// The general kernel, for caches the TMA kernels do not take (block sizes that are no multiple of 8, odd strides, more than 16 rows at
+// head dimension 256): cp.async, token by token, 16 bytes a piece.  Bound by the address arithmetic and the waits of its
+// loads: 2.8 TB/s on the case the TMA kernel streams at 5.7.
 // MT x 16 query rows per CTA: MT warps side by side over the rows, 4 / MT over the tokens of a tile.
 // SPLIT_P (at most 8 rows): the probabilities are carried as bf16 + bf16 remainder; the remainders ride in the
 // eight rows of the operand that would otherwise be padding, so their products cost nothing.
@@ -832,7 +835,8 @@ __global__ void __launch_bounds__(kCombineThreads) attend_combine_kernel(const _
 // complete only after the last tile, so the weights are formed in a second pass over K (not V): S^T = K Q^T with the
 // tokens as the rows of the product, so that a token's sum over query rows stays inside four lanes.  Every (token, KV head)
 // belongs to one CTA: no atomics, results repeat bit for bit.  A token of the query itself starts at 0 (its slot
-// may hold an earlier owner's sum), an older one keeps its sum unless the call starts the sums anew.
+// may hold an earlier owner's sum), an older one keeps its sum unless the call starts the sums anew.  This kernel serves the
+// caches that no tensor map describes; the others take attend_observe_mma_kernel.
 constexpr int kObserveRows = 128;  // query rows in shared memory at a time
 template <int D>
 constexpr size_t observe_smem_bytes() { return (size_t)kAttendStages<D> * kAttendStageBytes<D> + (size_t)kObserveRows * D * 2; }

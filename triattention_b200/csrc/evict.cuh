@@ -6,6 +6,9 @@
 // the radix passes and the output pass run from there, and the surviving sums go from there to their new slots.  Rows of more than
 // kEvictCap tokens are read from the cache in every pass; their sums move in the output pass, run by run: rank r <= index
 // i, and a run's values are in registers before any slot of it is written.
+// Bound by the row's dependent look-ups and the latency of the passes, not by bytes: 128 rows of 31000 tokens 40 us (one CTA of 1024
+// threads per SM), 256 rows of 2176 tokens 14 us (two CTAs of 512 per SM: with 1024 threads the second half of the rows had to
+// wait, 20 us).  The compaction behind it moves its bytes at 5.7 TB/s.
 #pragma once
 
 #include "common.cuh"
