@@ -350,10 +350,11 @@ int triattn_compress_paged(const triattn_paged_layout* layout /* host */, void* 
  * any order, negative entries are unused); the first min(num_listed, blocks of the request) entries count.
  * weight_sums (may be NULL) [num_blocks, num_kv_heads, block_size] fp32: every token read receives the sum over the
  * query rows of its KV head of exp(s - lse); older tokens add it to what is there (or start anew with
- * reset_weight_sums), the query's own tokens always start anew.
+ * reset_weight_sums), the query's own tokens always start anew.  With weight_sums the requests of a call share no cache blocks
+ * (a shared block's sums would be updated by several of them at once); without, they may.
  * layout: num_reqs, group_size (query heads per KV head), the cache geometry; head_dim 64, 128 or 256; any block size and
  * strides that are multiples of 8 elements.  k_cache / v_cache: the layer's base pointers (device memory, 16-byte
- * aligned).  q [num_query_tokens, num_kv_heads * group_size, head_dim] bf16 with the given strides, out likewise, lse contiguous.
+ * aligned).  out overlaps no input.  q [num_query_tokens, num_kv_heads * group_size, head_dim] bf16 with the given strides, out likewise, lse contiguous.
  * No two calls that may overlap share a workspace.  Results do not depend on scheduling: equal calls give equal bits.
  * Requests with more query tokens than max_query_len or than cached tokens, or more tokens than their block-table row holds, are skipped
  * (TRIATTN_DEV_BAD_LENGTH); tokens of blocks outside the cache are not read (TRIATTN_DEV_BAD_BLOCK_ID), nor listed

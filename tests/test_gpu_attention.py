@@ -682,3 +682,64 @@ def test_wait_timeout_in_the_attention_kernels_reports_status_and_returns():
     assert out.returncode == 0, out.stderr[-2000:]
     line = [x for x in out.stdout.splitlines() if x.startswith("STATUS")][-1].split()
     assert all(int(b) & _native.DEV_WAIT_TIMEOUT for b in line[1:5]) and int(line[5]) == 45, line
+
+
+def test_strides_of_axes_with_one_entry_do_not_matter():
+    """One KV head or one block: whatever the stride of that axis says, the same result."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1400)
+    bt = Batch([130], [1], 1, 4, 64, 16, gen).dev()
+    want, wl = ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, 1, kv_axis=0)
+    check_rows(bt, want, wl, 1, 1 / 8)
+    st = list(bt.d_cache[0].stride())
+    for s in (8, 72, 1 << 20):
+        odd = bt.d_cache[0].as_strided(bt.d_cache[0].shape, st[:3] + [s] + st[4:])
+        out, lse = ops.attend_paged(bt.d_q, odd, bt.d_table, bt.d_lens, bt.d_start, 1, kv_axis=0)
+        assert torch.equal(out, want) and torch.equal(lse, wl)
+    one = torch.randn((2, 1, 16, 2, 64), generator=gen).to(torch.bfloat16).to(DEV)
+    q = torch.randn((1, 8, 64), generator=gen).to(torch.bfloat16).to(DEV)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    outs = []
+    for s in (16 * 128, 8, 24, 1 << 21):
+        c = one.as_strided(one.shape, (one.stride(0), s, *one.stride()[2:]))
+        outs.append(ops.attend_paged(q, c, i32([[0]]), i32([11]), i32([0, 1]), 1, kv_axis=0)[0])
+    assert all(torch.equal(o, outs[0]) for o in outs[1:])
+
+
+def test_choice_among_more_blocks_than_shared_memory_holds():
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1500)
+    T, n = 40000, 2
+    bt = Batch([T, 33000], [n, 1], 1, 2, 64, 1, gen).dev()            # a block is a token
+    bounds = torch.zeros((bt.nb, 1, 2, 64), dtype=torch.bfloat16, device=DEV)
+    view = ops.PagedCacheView.from_layers([bt.d_cache[0]], kv_axis=0)
+    zero = torch.zeros(2, dtype=torch.int32, device=DEV)
+    ops.update_block_bounds(view, view.layout(2, 2, bt.width), bounds[None], bt.d_table, zero, bt.d_lens)
+    got = ops.select_blocks(bt.d_q, bounds, bt.d_lens, bt.d_start, bt.d_table, n, 1, 700, sink_blocks=3, recent_blocks=20).cpu()
+    for b in range(2):
+        k, _ = bt.tokens(b)
+        lo, hi = oa.block_bounds(k, 1)
+        want = oa.select_blocks(oa.block_scores(bt.q[bt.rows(b)], lo, hi), bt.lens[b], bt.counts[b], 1, 700, 3, 20)
+        assert torch.equal(got[b], want)
+
+
+def test_eviction_refused_before_anything_moves():
+    """A pool too large for the compaction is refused by the entry point before the selection has moved the sums."""
+    import ctypes
+
+    from triattention_b200 import _native
+    lib = _native.load()
+    lay = _native.PagedLayout(1, 1, 8, 1, 128, 16, 3_000_000, 8, 16 * 8 * 128, 8 * 128, 128, 0, 0)
+    sums = torch.ones(64, device=DEV)
+    p = sums.data_ptr()
+    assert lib.triattn_evict_paged(ctypes.byref(lay), p, p, p, p, p, p, None, 1, p, 4, None, None) == 2
+    torch.cuda.synchronize()
+    assert (sums == 1).all()
+
+
+def test_output_on_top_of_the_queries_is_refused():
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1600)
+    bt = Batch([20], [1], 1, 2, 64, 16, gen).dev()
+    with pytest.raises(ValueError):
+        ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, 1, kv_axis=0, out=bt.d_q)

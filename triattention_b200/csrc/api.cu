@@ -324,6 +324,16 @@ int triattn_select_topk(const float* scores, int num_rows, int64_t row_stride, c
                           keep_pitch, device_status, static_cast<cudaStream_t>(stream), false);
 }
 
+static int compact_supported(const triattn_paged_layout& Y) {
+  const int row_bytes = Y.head_dim * 2;
+  if (row_bytes % 16 != 0) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  const int ppr = row_bytes / 16, nsub = (ppr + 31) / 32;
+  if (ppr % nsub != 0) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  // row offsets inside a layer's pool are kept as 32-bit counts of 16 bytes: pools up to 64 GB per layer
+  if (((long long)Y.num_blocks * Y.block_stride >> 3) >= (1ll << 32) - (1ll << 20)) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  return TRIATTN_OK;
+}
+
 static int compact_common(const triattn_paged_layout* layout, void* const* k_layer_ptrs, void* const* v_layer_ptrs,
                           const int32_t* block_table, const int32_t* seq_lens, const int32_t* keep,
                           int64_t keep_ls, int64_t keep_rs, int64_t keep_hs, const int32_t* keep_counts,
@@ -335,11 +345,9 @@ static int compact_common(const triattn_paged_layout* layout, void* const* k_lay
     return TRIATTN_ERR_INVALID_ARGUMENT;
   const triattn_paged_layout& Y = *layout;
   const int row_bytes = Y.head_dim * 2;
-  if (row_bytes % 16 != 0) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
-  const int ppr = row_bytes / 16, nsub = (ppr + 31) / 32;
-  if (ppr % nsub != 0) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
-  // row offsets inside a layer's pool are kept as 32-bit counts of 16 bytes: pools up to 64 GB per layer
-  if (((long long)Y.num_blocks * Y.block_stride >> 3) >= (1ll << 32) - (1ll << 20)) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  rc = compact_supported(Y);
+  if (rc != TRIATTN_OK) return rc;
+  const int nsub = (row_bytes / 16 + 31) / 32;
   CompactParams p{};
   p.nsub = nsub;
   p.k_ptrs = k_layer_ptrs;
@@ -418,6 +426,8 @@ int triattn_evict_paged(const triattn_paged_layout* layout, void* const* k_layer
   if (window < 0 || keep_pitch <= 0) return TRIATTN_ERR_INVALID_ARGUMENT;
   const triattn_paged_layout& Y = *layout;
   if ((long long)Y.max_blocks_per_req * Y.block_size > (1ll << 30)) return TRIATTN_ERR_UNSUPPORTED_SHAPE;
+  rc = compact_supported(Y);  // before the sums have moved
+  if (rc != TRIATTN_OK) return rc;
   EvictParams p{};
   p.sums = weight_sums;
   p.block_table = block_table;

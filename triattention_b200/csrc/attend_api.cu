@@ -49,6 +49,15 @@ int attend_max_runs(int slots, int heads) {
   return runs;
 }
 
+// The stride of an axis with one entry says nothing: give it the value the tensor maps want.
+triattn_paged_layout with_plain_strides(const triattn_paged_layout& L) {
+  triattn_paged_layout Y = L;
+  if (Y.num_blocks == 1) Y.block_stride = std::max(Y.block_size * Y.token_stride, Y.num_kv_heads * Y.head_stride);
+  if (Y.num_kv_heads == 1) Y.head_stride = Y.block_stride;
+  else if (Y.num_blocks == 1) Y.block_stride = (Y.block_stride + Y.head_stride - 1) / std::max<int64_t>(Y.head_stride, 1) * Y.head_stride;
+  return Y;
+}
+
 // Can the layer's K and V be described by the tensor maps of attend_tma.cuh?
 bool tileable(const triattn_paged_layout& Y) {
   const int64_t strides[3] = {Y.block_stride, Y.token_stride, Y.head_stride};
@@ -189,7 +198,7 @@ extern "C" {
 
 size_t triattn_attend_workspace_bytes(const triattn_paged_layout* layout, int max_query_len, int num_listed) {
   if (validate_attend(layout, max_query_len, num_listed) != TRIATTN_OK) return 0;
-  return attend_plan(*layout, max_query_len, num_listed).bytes;
+  return attend_plan(with_plain_strides(*layout), max_query_len, num_listed).bytes;
 }
 
 int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache, const void* v_cache,
@@ -211,7 +220,7 @@ int triattn_attend_paged(const triattn_paged_layout* layout, const void* k_cache
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q) || !aligned16(out) || !aligned16(workspace) ||
       q_token_stride % 8 || q_head_stride % 8 || out_token_stride % 8 || out_head_stride % 8)
     return TRIATTN_ERR_MISALIGNED;
-  const triattn_paged_layout& Y = *layout;
+  const triattn_paged_layout Y = with_plain_strides(*layout);
   const AttendPlan a = attend_plan(Y, max_query_len, num_listed);
   if (workspace_bytes < a.bytes) return TRIATTN_ERR_WORKSPACE_TOO_SMALL;
   AttendParams p{};

@@ -497,7 +497,8 @@ def attend_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
     ``block_list`` ``[B, Hkv, S]`` int32 (:func:`select_blocks`) restricts each KV head to the listed blocks.
     ``weight_sums`` ``[num_blocks, Hkv, block_size]`` fp32 receives, per cached token and KV head, the attention weight the
     token got from this call's rows: added to what older tokens have (``reset_weight_sums``: starting anew), while the
-    request's own tokens always start anew, whatever their slots held.  ``out`` ``[N, Hq, D]`` bf16, ``lse`` ``[N, Hq]`` fp32
+    request's own tokens always start anew, whatever their slots held (the requests of such a call share no cache
+    blocks).  ``out`` ``[N, Hq, D]`` bf16, ``lse`` ``[N, Hq]`` fp32
     (natural log); rows that no request owns are left as they are.  ``workspace``: at least
     :func:`attend_workspace_bytes` bytes that no overlapping call uses.
     """
@@ -530,6 +531,8 @@ def attend_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
             out = q.new_empty(q.shape)
         elif out.dtype is not torch.bfloat16 or out.get_device() != index or out.shape != q.shape or out.stride(2) != 1:
             raise ValueError("out must be a bf16 tensor of q's shape on q's device with a contiguous last axis")
+        elif out.data_ptr() == q.data_ptr() and N > 0:
+            raise ValueError("out must not be q")
         if lse is None:
             lse = q.new_empty((N, H * g), dtype=torch.float32)
             p_lse = lse.data_ptr()
