@@ -39,7 +39,7 @@ struct AttendParams {
   int B, Hkv, g, bs, num_blocks, max_blocks;
   long long block_stride, token_stride, head_stride;  // elements
   int N, max_q;
-  int box;        // tokens per TMA box: the largest of 32, 16, 8 that divides the block size (tiled kernels)
+  int box;        // tokens per TMA box: the tile's tokens, halved until they divide the block size (tiled kernels)
   int slots_per_block;  // head slots per block: block_stride / head_stride (tiled kernels)
   int min_tiles;  // tiles a CTA should have before another one is started
   float scale_log2;

@@ -166,7 +166,8 @@ int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensor
                       int max_row_tiles, const CUtensorMap* observe_map, int observe_box, int observe_runs, cudaStream_t st) {
   int rc = launch_attend<D>(p, a, km, vm, st);
   if (rc != TRIATTN_OK) return rc;
-  rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)(max_row_tiles * ((a.rows + 7) / 8)), (unsigned)p.Hkv, (unsigned)p.B),
+  const int chunks = (a.rows + 7) / 8, live = (p.max_q * p.g + 7) / 8;  // CTAs per row tile; of them with rows, where there is one tile
+  rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)(max_row_tiles > 1 ? max_row_tiles * chunks : std::min(chunks, live)), (unsigned)p.Hkv, (unsigned)p.B),
                      dim3(kCombineThreads), 0, st, true, p, a.runs, a.tile, a.rows);
   if (rc != TRIATTN_OK || p.sums == nullptr) return rc;
   if (observe_map != nullptr) {
