@@ -213,14 +213,19 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       }
       return true;
     };
-    for (int i = 0; i < count && ok; ++i) {
+    // (one place in the code for each of the two: the kernel's loops share the instruction cache)
+#pragma unroll 1
+    for (int i = 0; i <= count && ok; ++i) {
       // a new segment's query rows are written after the last P V of the one before; with one S buffer P V comes first anyway
-      const bool pv_first = i > 0 && (SB == 1 || t_in_piece == 0);
-#pragma unroll
-      for (int g = 0; g < NT; ++g) {
-        if (ok && pv_first) ok = issue_pv(i - 1, g, prev_in_piece);
-        if (ok) ok = issue_s(i, g);
-        if (ok && i > 0 && !pv_first) ok = issue_pv(i - 1, g, prev_in_piece);
+      const bool pv_first = SB == 1 || t_in_piece == 0 || i == count;
+#pragma unroll 1
+      for (int step = 0; step < 2 * NT && ok; ++step) {
+        const int g = step >> 1;
+        if (((step & 1) == 0) == pv_first) {
+          if (i > 0) ok = issue_pv(i - 1, g, prev_in_piece);
+        } else if (i < count) {
+          ok = issue_s(i, g);
+        }
       }
       prev_in_piece = t_in_piece++;
       if (--left == 0 && i + 1 < count) {
@@ -231,9 +236,6 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         left = min(c.r.tiles, count - i - 1);
       }
     }
-#pragma unroll
-    for (int g = 0; g < NT; ++g)
-      if (ok) ok = issue_pv(count - 1, g, prev_in_piece);
     if (!ok) {  // a wait ran out: the operands must outlive what has been issued
       umma_commit(smem_u32(&drained));
       mbar_wait_bounded(smem_u32(&drained), 0u);
