@@ -67,6 +67,10 @@ bool tileable(const triattn_paged_layout& Y) {
          Y.num_blocks * (Y.block_stride / Y.head_stride) < (1ll << 31);
 }
 
+// Tiles per warp up to which one CTA takes all of a KV head's tiles.  One request, 8 heads, on the device: 150 tokens 8.5 us whole and 9.2
+// in parts with the launch that joins them, 300 tokens 9.6 and 10.8, 517 (three tiles per warp) 11.8 and 11.1, 1100 16.7 and 11.9.
+constexpr int kDecodeWholeTiles = 2;
+
 AttendPlan attend_plan(const triattn_paged_layout& Y, int max_q, int num_listed) {
   AttendPlan a{};
   const long long R = (long long)max_q * Y.group_size;
@@ -92,7 +96,10 @@ AttendPlan attend_plan(const triattn_paged_layout& Y, int max_q, int num_listed)
   }
   for (a.box = a.tile; a.box > 8 && Y.block_size % a.box; a.box /= 2) {
   }
-  a.runs = (int)std::min<long long>(attend_max_runs(ctas, Y.num_kv_heads), attend_max_tiles(Y, max_q, num_listed, a.tile, a.rows));
+  const long long most = attend_max_tiles(Y, max_q, num_listed, a.tile, a.rows);
+  a.runs = (int)std::min<long long>(attend_max_runs(ctas, Y.num_kv_heads), most);
+  // a few tiles per warp and head: one CTA per head does them all, and nothing is left to join
+  if (a.kind == AttendKind::kDecode && most <= kDecodeWholeTiles * kDecodeWarps) a.runs = 1;
   a.part_o = (size_t)2 * a.runs * Y.num_kv_heads * a.rows * Y.head_dim * sizeof(float);
   a.part_ml = (size_t)2 * a.runs * Y.num_kv_heads * a.rows * 2 * sizeof(float);
   a.bytes = round_up(a.part_o, 256) + round_up(a.part_ml, 256);
@@ -166,9 +173,11 @@ int launch_attend_all(const AttendParams& p, const AttendPlan& a, const CUtensor
                       int max_row_tiles, const CUtensorMap* observe_map, int observe_box, int observe_runs, cudaStream_t st) {
   int rc = launch_attend<D>(p, a, km, vm, st);
   if (rc != TRIATTN_OK) return rc;
-  const int chunks = (a.rows + 7) / 8, live = (p.max_q * p.g + 7) / 8;  // CTAs per row tile; of them with rows, where there is one tile
-  rc = launch_kernel(attend_combine_kernel<D>, dim3((unsigned)(max_row_tiles > 1 ? max_row_tiles * chunks : std::min(chunks, live)), (unsigned)p.Hkv, (unsigned)p.B),
-                     dim3(kCombineThreads), 0, st, true, p, a.runs, a.tile, a.rows);
+  if (a.runs > 1) {  // (with one run per head every segment is whole)
+    const int chunks = (a.rows + 7) / 8, live = (p.max_q * p.g + 7) / 8;  // CTAs per row tile; of them with rows, where there is one tile
+    const dim3 grid((unsigned)(max_row_tiles > 1 ? max_row_tiles * chunks : std::min(chunks, live)), (unsigned)p.Hkv, (unsigned)p.B);
+    rc = launch_kernel(attend_combine_kernel<D>, grid, dim3(kCombineThreads), 0, st, true, p, a.runs, a.tile, a.rows);
+  }
   if (rc != TRIATTN_OK || p.sums == nullptr) return rc;
   if (observe_map != nullptr) {
     constexpr size_t smem = observe_mma_smem_bytes<D>();
