@@ -743,3 +743,30 @@ def test_output_on_top_of_the_queries_is_refused():
     bt = Batch([20], [1], 1, 2, 64, 16, gen).dev()
     with pytest.raises(ValueError):
         ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, 1, kv_axis=0, out=bt.d_q)
+
+
+@pytest.mark.parametrize("g,n,D,bs", [(3, 1, 128, 16), (4, 1, 64, 16), (5, 7, 128, 16), (4, 40, 64, 16), (3, 2, 128, 5), (5, 3, 256, 16)])
+def test_keys_of_minus_infinite_logit_weigh_nothing(g, n, D, bs):
+    """An infinite key channel against queries that are all negative there: the logit is -inf, the token weighs 0 and no
+    other token is disturbed, in the output or in the sums."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1700 + n)
+    bt = Batch([150], [n], 2, g, D, bs, gen, tree=n > 1)
+    bt.q[:, :, 0] = -bt.q[:, :, 0].abs() - 0.5
+    blk, off = oa.token_slots(bt.table[0].tolist(), bs, 150)
+    k, _ = split(bt.cache[0], 0)
+    k[blk[37], off[37], :, 0] = float("inf")
+    bt.dev()
+    sums = torch.zeros((bt.nb, 2, bs), device=DEV)
+    out, lse = ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, n, tree_mask=bt.d_words, kv_axis=0, weight_sums=sums)
+    finite = bt.cache.clone()
+    kk, vv = split(finite[0], 0)
+    tk, tv = kk[blk, off].clone(), vv[blk, off]
+    tk[37, :, 0] = 0
+    see = oa.visible(150, n, bt.words)
+    see[:, 37] = False
+    e = oa.attend_request(bt.q, tk, tv, see, 1 / math.sqrt(D))
+    assert torch.allclose(lse.cpu().double(), e["lse"], atol=1e-4)
+    assert ((out.cpu().double() - e["out"]).abs() <= 2.0 ** -8 * e["out"].abs() + 2.0 ** -7.9 * e["spread"]).all()
+    got = sums.cpu()[blk, :, off].T.double()
+    assert (got[:, 37] == 0).all() and torch.allclose(got, e["weight"], rtol=1e-3, atol=1e-7)

@@ -892,13 +892,11 @@ __global__ void __launch_bounds__(kAttendThreads) attend_observe_kernel(const __
   auto load_rows = [&](int r0) {
     const int R = c.r.n * p.g;
     for (int x = tid; x < kObserveRows * PPR; x += kAttendThreads) {
-      const int row = x / PPR, piece = x % PPR, r = r0 + row;
+      // (rows up to a multiple of 8 repeat the last one: a zero row times an infinite key would be NaN, and stay it)
+      const int row = x / PPR, piece = x % PPR, r = min(r0 + row, R - 1);
       if (row >= ((min(R - r0, kObserveRows) + 7) & ~7)) break;
-      uint4 w = make_uint4(0u, 0u, 0u, 0u);
-      if (r < R) {
-        const int i = r / p.g, j = r - i * p.g;
-        w = *reinterpret_cast<const uint4*>(p.q + (long long)(c.r.q0 + i) * p.q_ts + (long long)(c.h * p.g + j) * p.q_hs + piece * 8);
-      }
+      const int i = r / p.g, j = r - i * p.g;
+      const uint4 w = *reinterpret_cast<const uint4*>(p.q + (long long)(c.r.q0 + i) * p.q_ts + (long long)(c.h * p.g + j) * p.q_hs + piece * 8);
       *reinterpret_cast<uint4*>(q_smem + tile_off<D>(row, piece)) = w;
     }
     for (int row = tid; row < kObserveRows; row += kAttendThreads) {

@@ -643,12 +643,10 @@ __global__ void __launch_bounds__(kObserveMmaThreads, 1)
       const int R = c.r.n * p.g, ctx = c.r.T - c.r.n, cols = columns(c.r);
       meet();  // the tiles of the piece before have been emptied: its rows are not needed any more
       for (int x = tid; x < cols * (D / 8); x += 256) {
-        const int row = x / (D / 8), pc = x % (D / 8), r = row0 + row;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (r < R) {
-          const int i = r / p.g, j = r - i * p.g;
-          w = *reinterpret_cast<const uint4*>(p.q + (long long)(c.r.q0 + i) * p.q_ts + (long long)(c.h * p.g + j) * p.q_hs + pc * 8);
-        }
+        // (columns without a row repeat the last one: a zero row times an infinite key would be NaN, and stay it)
+        const int row = x / (D / 8), pc = x % (D / 8), r = min(row0 + row, R - 1);
+        const int i = r / p.g, j = r - i * p.g;
+        const uint4 w = *reinterpret_cast<const uint4*>(p.q + (long long)(c.r.q0 + i) * p.q_ts + (long long)(c.h * p.g + j) * p.q_hs + pc * 8);
         *reinterpret_cast<uint4*>(q_smem + (pc >> 3) * (RMAX * 128) + row * 128 + (((pc & 7) ^ (row & 7)) << 4)) = w;
       }
       if (tid < cols) {
