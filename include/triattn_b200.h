@@ -401,7 +401,8 @@ int triattn_update_block_bounds(const triattn_paged_layout* layout /* host */, c
  * The blocks a step reads: per request and KV head the num_selected blocks with the largest upper bound of the
  * attention logits, summed over the request's query tokens and the heads of the group (ties: lowest index), ascending, tail filled
  * with -1.  The first sink_blocks, the last recent_blocks and the blocks of the query's own tokens are always taken;
- * num_selected must hold them.  bounds: ONE layer's [num_blocks, num_kv_heads, 2, head_dim].
+ * num_selected must hold them; infinite bounds count as 2^128, and where a block with NaN among its bounds ranks is not
+ * defined.  bounds: ONE layer's [num_blocks, num_kv_heads, 2, head_dim].
  *   block_list [num_reqs, num_kv_heads, num_selected] int32: the argument of triattn_attend_paged.
  */
 int triattn_select_blocks(const triattn_paged_layout* layout /* host */, const void* q, int64_t q_token_stride,

@@ -180,3 +180,16 @@ def test_oracle_against_a_dense_softmax():
     best = torch.einsum("nhd,thd->nht", q, k.repeat_interleave(g, 1)).view(n, H, g, T)
     for b in range(3):  # an upper bound of every logit, summed over the rows
         assert (sc[:, b] + 1e-4 >= best[..., 4 * b : 4 * b + 4].amax(-1).sum((0, 2))).all()
+
+
+@pytest.mark.parametrize("name", ["num_layers", "num_blocks", "block_size", "num_kv_heads", "head_dim", "block_stride", "token_stride", "head_stride"])
+def test_a_layout_that_is_not_the_views_is_refused(on_cpu, monkeypatch, name):
+    monkeypatch.setattr(ops, "_on_device", lambda index: ops._NO_GUARD)
+    x = inputs()
+    view = ops.PagedCacheView._build([x["kv_cache"], x["kv_cache"].clone()], 0)
+    lay, one = view.layout(2, 1, 4), torch.zeros(2, dtype=torch.int32)
+    setattr(lay, name, getattr(lay, name) * 2)
+    with pytest.raises(ValueError, match=name):
+        ops.evict_paged(view, lay, torch.zeros((2, 9, 2, 16)), x["block_table"], one, one, 4, 2)
+    with pytest.raises(ValueError, match=name):
+        ops.update_block_bounds(view, lay, torch.zeros((2, 9, 2, 2, 64), dtype=torch.bfloat16), x["block_table"], one, one)

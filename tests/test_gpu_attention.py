@@ -770,3 +770,21 @@ def test_keys_of_minus_infinite_logit_weigh_nothing(g, n, D, bs):
     assert ((out.cpu().double() - e["out"]).abs() <= 2.0 ** -8 * e["out"].abs() + 2.0 ** -7.9 * e["spread"]).all()
     got = sums.cpu()[blk, :, off].T.double()
     assert (got[:, 37] == 0).all() and torch.allclose(got, e["weight"], rtol=1e-3, atol=1e-7)
+
+
+def test_what_is_always_kept_ranks_above_infinities():
+    """More infinite sums, or bounds, in front than there are places: the window's tokens and the recent blocks stay."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1800)
+    bt = Batch([640], [1], 1, 2, 64, 16, gen).dev()
+    bounds = torch.full((bt.nb, 1, 2, 64), float("inf"), dtype=torch.bfloat16, device=DEV)
+    got = ops.select_blocks(bt.d_q.abs(), bounds, bt.d_lens, bt.d_start, bt.d_table, 1, 16, 6, sink_blocks=1, recent_blocks=2)
+    assert got[0, 0].tolist() == [0, 1, 2, 3, 38, 39]
+    bounds.fill_(2.0 ** 127)                         # finite bounds whose sum is beyond 32 bits
+    got = ops.select_blocks(bt.d_q.abs(), bounds, bt.d_lens, bt.d_start, bt.d_table, 1, 16, 6, sink_blocks=1, recent_blocks=2)
+    assert got[0, 0].tolist() == [0, 1, 2, 3, 38, 39]
+    view = ops.PagedCacheView.from_layers(list(bt.d_cache.unbind(0)), kv_axis=0)
+    sums = torch.full((1, bt.nb, 1, 16), float("inf"), device=DEV)
+    one = lambda v: torch.tensor([v], dtype=torch.int32, device=DEV)  # noqa: E731
+    keep = ops.evict_paged(view, view.layout(1, 1, bt.width), sums, bt.d_table, bt.d_lens, one(20), 20, 8, one(3))
+    assert keep[0, 0, 0].tolist() == list(range(12)) + list(range(632, 640))

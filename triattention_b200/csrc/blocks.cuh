@@ -6,6 +6,8 @@
 // of 2 D terms per block.  The blocks with the largest sums are read.
 #pragma once
 
+#include <cfloat>
+
 #include "common.cuh"
 #include "attend.cuh"
 #include "topk_row.cuh"
@@ -104,7 +106,8 @@ __global__ void __launch_bounds__(kBoundsThreads) block_bounds_kernel(const __gr
 // ------------------------------------------------------------------------------------------ block scores
 // The order of the scores decides which blocks are read, so they are formed in 64 bits and rounded to 32 once: equal scores
 // stay equal whatever the order of the sum.  A bf16 word shifted into the high half of a double is the value times
-// 2^-896, exactly (subnormal bf16 values land on subnormal doubles): no conversion instructions.
+// 2^-896, exactly: no conversion instructions.  Infinite bounds count as 2^128, so that 0 times them is 0; a block whose bounds
+// hold NaN (a NaN among its keys) gets some score of that size.
 constexpr int kScoreThreads = 256;
 
 struct SelectBlocksParams {
@@ -273,7 +276,11 @@ __global__ void __launch_bounds__(kScoreThreads) block_scores_kernel(const __gri
     for (int k = 4; k; k >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], k);
     const int j = j0 + (upper ? 2 : 0) + (odd ? 1 : 0);
     const int blk = __shfl_sync(0xffffffffu, my_blk, j & 31);
-    if ((lane & 7) == 0 && j < count) out[lb0 + j] = blk >= 0 ? (float)(s[0] * unscale) : blk == -1 ? INFINITY : -INFINITY;
+    if ((lane & 7) == 0 && j < count) {
+      float v = (float)(s[0] * unscale);
+      if (v == INFINITY) v = FLT_MAX;  // only the blocks that are always read are above every number
+      out[lb0 + j] = blk >= 0 ? v : blk == -1 ? INFINITY : -INFINITY;
+    }
   }
   if (err) flag_status(p.status, err);
 }

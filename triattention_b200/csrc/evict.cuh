@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
   };
   for (int i = k + threadIdx.x; i < p.pitch; i += THREADS) out[i] = -1;
   const bool cached = n <= p.cap;
-  constexpr unsigned kTop = 0xff800000u;  // float_to_ordered(+inf)
+  constexpr unsigned kInf = 0xff800000u;  // float_to_ordered(+inf); guarded tokens rank above it
   topk_row<THREADS>(
       n, k, reinterpret_cast<unsigned*>(evict_smem), p.cap, sh,
       slot,
@@ -77,9 +77,9 @@ __global__ void __launch_bounds__(THREADS) evict_select_kernel(const __grid_cons
         return float_to_ordered(at < 0 ? -INFINITY : w);
       },
       [&](unsigned bits, int i) -> unsigned {
-        if (i >= recent || i < guard) return kTop;
+        if (i >= recent || i < guard) return kInf + 1u;
         if (bits == 0x7fffffffu) return 0x80000000u;  // -0 ranks as 0
-        return bits > kTop ? 0u : bits;               // NaN last
+        return bits > kInf ? 0u : bits;               // NaN last
       },
       [&](int rank, int i) { out[rank] = i; },
       [&](const bool(&sel)[4], const int(&rank)[4], const int(&at)[4], const unsigned(&bits)[4]) {

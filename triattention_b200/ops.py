@@ -554,6 +554,13 @@ def attend_workspace_bytes(layout: PagedLayout, max_query_len: int, num_listed: 
     return int(_native.load().triattn_attend_workspace_bytes(ctypes.byref(layout), int(max_query_len), int(num_listed)))
 
 
+def _check_view(view: PagedCacheView, layout: PagedLayout) -> None:
+    """The layout handed to the library has to be the view's own: its counts and strides address the cache."""
+    for name in ("num_layers", "num_blocks", "block_size", "num_kv_heads", "head_dim", "block_stride", "token_stride", "head_stride"):
+        if getattr(layout, name) != getattr(view, name):
+            raise ValueError(f"layout has {name} {getattr(layout, name)}, the cache view {getattr(view, name)}")
+
+
 def evict_paged(view: PagedCacheView, layout: PagedLayout, weight_sums: torch.Tensor, block_table: torch.Tensor,
                 seq_lens: torch.Tensor, keep_counts: torch.Tensor, keep_pitch: int, window: int,
                 prefill_lens: Optional[torch.Tensor] = None, keep_out: Optional[torch.Tensor] = None,
@@ -567,6 +574,7 @@ def evict_paged(view: PagedCacheView, layout: PagedLayout, weight_sums: torch.Te
     lib = _native.load()
     _require_cuda(weight_sums, "weight_sums")
     index = weight_sums.get_device()
+    _check_view(view, layout)
     L, B, H = view.num_layers, layout.num_reqs, view.num_kv_heads
     if view.k_ptrs.get_device() != index:
         raise ValueError(f"weight_sums is on {weight_sums.device}, the cache on {view.device}")
@@ -593,6 +601,7 @@ def update_block_bounds(view: PagedCacheView, layout: PagedLayout, bounds: torch
     lib = _native.load()
     _require_cuda(bounds, "bounds")
     index, B = bounds.get_device(), layout.num_reqs
+    _check_view(view, layout)
     if view.k_ptrs.get_device() != index:
         raise ValueError(f"bounds is on {bounds.device}, the cache on {view.device}")
     p_bounds = _expect(bounds, "bounds", torch.bfloat16, index,
