@@ -788,3 +788,22 @@ def test_what_is_always_kept_ranks_above_infinities():
     one = lambda v: torch.tensor([v], dtype=torch.int32, device=DEV)  # noqa: E731
     keep = ops.evict_paged(view, view.layout(1, 1, bt.width), sums, bt.d_table, bt.d_lens, one(20), 20, 8, one(3))
     assert keep[0, 0, 0].tolist() == list(range(12)) + list(range(632, 640))
+
+
+@pytest.mark.parametrize("D,bs,g,n", VARIANTS)
+def test_infinite_values_everyone_sees(D, bs, g, n):
+    """An infinite value of an older token: its channel is infinite for every row, the others are as without it."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(1900 + D + n)
+    bt = Batch([170], [n], 2, g, D, bs, gen, tree=n > 1).dev()
+    run = lambda: ops.attend_paged(bt.d_q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, n, tree_mask=bt.d_words, kv_axis=0)  # noqa: E731
+    want, wlse = run()
+    k, v = split(bt.cache[0], 0)
+    blk, off = oa.token_slots(bt.table[0].tolist(), bs, 170)
+    v[blk[33], off[33], :, 3] = float("inf")
+    v[blk[90], off[90], :, D - 7] = float("-inf")
+    bt.dev()
+    out, lse = run()
+    assert (out[:, :, 3] == float("inf")).all() and (out[:, :, D - 7] == float("-inf")).all()
+    others = [d for d in range(D) if d not in (3, D - 7)]
+    assert torch.equal(out[:, :, others], want[:, :, others]) and torch.equal(lse, wlse)

@@ -365,6 +365,10 @@ __device__ __forceinline__ unsigned long long attend_word(const AttendParams& p,
   return i >= 63 ? ~0ull : ((2ull << i) - 1ull);
 }
 
+// P V of the rounded probabilities and of their remainders.  Where an infinite value makes the first infinite the second says nothing:
+// remainders have either sign, or are 0, and would turn it into NaN.
+__device__ __forceinline__ float add_remainder(float o, float rest) { return isfinite(o) ? o + rest : o; }
+
 // The general kernel, for caches the TMA kernels do not take (block sizes that are no multiple of 8, odd strides, more than 16 rows at
 // head dimension 256): cp.async, token by token, 16 bytes a piece.  Bound by the address arithmetic and the waits of its
 // loads: 2.8 TB/s on the case the TMA kernel streams at 5.7.
@@ -623,8 +627,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
       if constexpr (SPLIT_P) {
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) {
-          o[j][0] += o[j][2];
-          o[j][1] += o[j][3];
+          o[j][0] = add_remainder(o[j][0], o[j][2]);
+          o[j][1] = add_remainder(o[j][1], o[j][3]);
         }
       }
 #pragma unroll

@@ -410,8 +410,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     if constexpr (SPLIT_P) {
 #pragma unroll
       for (int j = 0; j < D / 8; ++j) {
-        o[j][0] += o[j][2];
-        o[j][1] += o[j][3];
+        o[j][0] = add_remainder(o[j][0], o[j][2]);
+        o[j][1] = add_remainder(o[j][1], o[j][3]);
       }
     }
 #pragma unroll
