@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   if (wid > MMA_WARP) {
     const int w = wid - MMA_WARP - 1;
     attend_produce<D, TILE, STAGES>(p, w == 0 ? &kmap : &vmap, w, c, count, ROWS, w == 0 ? base : v_base, kTileBytes,
-                                    ring.full[w], ring.empty[w], ring);
+                                    ring.full[w], ring.empty[w], ring, (w == 0 && p.sums != nullptr) || p.max_q * p.g > ROWS);
   } else if (wid == MMA_WARP) {
     // ------------------------------------------------------------------------------------------ MMA issue: one thread
     if (elect_one()) {
@@ -600,7 +600,8 @@ __global__ void __launch_bounds__(kObserveMmaThreads, 1)
   auto columns = [&](const AttendReq& r) { return (min(max(r.n * p.g - row0, 1), RMAX) + 31) & ~31; };
 
   if (wid > 8) {
-    attend_produce<D, TILE, STAGES>(p, &kmap, 0, c, count, kAll, base, kTileBytes, ring.full[0], ring.empty[0], ring, wid - 9, 2);
+    attend_produce<D, TILE, STAGES>(p, &kmap, 0, c, count, kAll, base, kTileBytes, ring.full[0], ring.empty[0], ring,
+                                p.max_q * p.g > row0 + RMAX, wid - 9, 2);
   } else if (wid == 8) {
     if (elect_one()) {
       bool ok = true;
