@@ -194,7 +194,7 @@ constexpr size_t decode_smem_bytes() {
 // Rows are padded to the 16 of mma.sync; a tile is one warp's business from arrival to release, so tiles of different
 // warps overlap without any barrier, and the warps meet only where a segment (or the CTA's run) ends.  mma.sync, not
 // tcgen05: with at most 16 live rows a tile's products take a fifth of the time its bytes need.  Bound by HBM: 64 requests of 2112
-// tokens, 8 KV heads, head dimension 128, in 97 us, 5.7 TB/s (87 % of the measured copy).
+// tokens, 8 KV heads, head dimension 128, in 96 us, 5.8 TB/s (88 % of the measured copy).
 template <int D, bool SPLIT_P>
 __global__ void __launch_bounds__(kDecodeThreads, 1)
     attend_decode_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,

@@ -13,7 +13,7 @@
 // P V and the next S of one group running while the other group is at its exponentials.  (One thread per row: a group took 2500
 // cycles for a tile's softmax, two and a half times what its exponentials cost, and the turns did not overlap.)  NT = 1: S has two buffers, and S of tile i
 // is issued before P V of tile i - 1.
-// Measured: 256 rows over 8 x 32768 tokens, 8 KV heads, in 285 us (850 TFLOP/s at a burst, 680 under the power cap), where the bytes take 165;
+// Measured: 256 rows over 8 x 32768 tokens, 8 KV heads, in 294 us (825 TFLOP/s in bursts, 680 under the power cap), where the bytes take 165;
 // what bounds it is the alternation of the two groups: per tile and group 1500 cycles for its products and 2000 for its softmax, the
 // tensor cores' own time for both groups being 2050.
 // A row's exponentials are taken against the maximum of the first tile it saw, which is raised only when the exponentials of
