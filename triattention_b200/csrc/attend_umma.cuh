@@ -123,7 +123,11 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   __shared__ uint32_t s_tmem;
   __shared__ float pair_val[2][NT][2][128];  // what the two threads of a row tell each other (tiles in turn)
   __shared__ bool pair_over[2][NT][2][4], row_over[2][NT][2][128];
-  __shared__ int odd_piece;  // the last piece in which a query token's value held an infinity or NaN
+  // The last even and the last odd piece in which a query token's value held an infinity or NaN.  Group 0 writes, both groups read
+  // when they write their piece out.  Two words, because group 0 may be a piece ahead: S of the next piece's first tile goes
+  // to it before P V of this piece's last tile to group 1.  It is never two ahead: S of that next tile for group 1, which the same
+  // thread issues before anything of the piece after, waits for queries that group 1 loads after it has read its word.
+  __shared__ int odd_piece[2];
   const int tid = threadIdx.x, lane = tid & 31, wid = tid >> 5;
 
   if (tid == 0) {
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
     ring.err = ring.gaps = 0;
     prefetch_map(&kmap);
     prefetch_map(&vmap);
-    odd_piece = -1;
+    odd_piece[0] = odd_piece[1] = -1;
   }
   grid_dependency_wait();
   trigger_dependents();
@@ -428,7 +432,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
               } else {
                 const uint4 w = *v;
                 if (has_nonfinite(w)) {
-                  *(volatile int*)&odd_piece = piece_no;
+                  *(volatile int*)&odd_piece[piece_no & 1] = piece_no;
                   *v = zero_nonfinite(w);
                 }
               }
@@ -453,7 +457,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
         pair_sync();  // read before the next one
         const int slot = 2 * (int)blockIdx.x + (t_begin > 0 ? 0 : 1);
         const float inv = !whole ? 1.f : l > 0.f ? 1.f / l : l;  // a NaN sum stays one
-        const bool odd = *(volatile int*)&odd_piece == piece_no;
+        const bool odd = *(volatile int*)&odd_piece[piece_no & 1] == piece_no;
         // the four rows this lane writes pieces of: where they go (null: they do not exist)
         unsigned char* to[4];
 #pragma unroll
