@@ -5,7 +5,11 @@
 //
 // over the tokens a row sees: every token before the request's query tokens, and of these (their keys are the last
 // slots of the sequence) the ones whose bit is set in the row's 64-bit word.  The softmax runs in one pass with a
-// running maximum and sum in fp32, in the base-2 domain.
+// running maximum and sum in fp32, in the base-2 domain.  Exponentials are taken against a reference kHeadroom above the maximum:
+// a row's exponentials then add up to at most 1 over the 2^30 tokens a call may have, and the unnormalised o is finite for
+// all finite values (against the maximum itself, 700 values of 2^126 and equal weights gave infinities).  What that costs lies at the
+// other end: weights below 2^-96 of the largest vanish, and outputs below 2^-96 lose bits of fp32.  The larger exponents
+// round to 2^-20, an eighth of the two bf16 parts' step and less.
 //
 // Bound: K and V are read once, 4 D bytes per (KV head, token), for 4 D R operations with R rows; up to about 32 rows the cache
 // stream is the limit, so what counts is that all SMs stream all the time.  The work of a KV head - the sequence of
@@ -24,6 +28,7 @@ namespace triattn {
 constexpr int kAttendMaxQuery = 64;  // query tokens per request: bits of a mask word
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kHeadroom = 30.f;  // base 2; 2^30: the tokens a call may have at most (validate_attend)
 
 struct AttendParams {
   const uint16_t* q;  // [N, Hq, D] bf16
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
     for (int x = 0; x < 2; ++x) {
       mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
       mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-      const float mn = fmaxf(m[x], mx[x] * p.scale_log2);
+      const float mn = fmaxf(m[x], fmaf(mx[x], p.scale_log2, kHeadroom));
       grew = grew || mn > m[x];
       base[x] = mn == -INFINITY ? 0.f : mn;
       mx[x] = mn;

@@ -16,9 +16,11 @@
 // Measured: 256 rows over 8 x 32768 tokens, 8 KV heads, in 294 us (825 TFLOP/s in bursts, 680 under the power cap), where the bytes take 165;
 // what bounds it is the alternation of the two groups: per tile and group 1500 cycles for its products and 2000 for its softmax, the
 // tensor cores' own time for both groups being 2050.
-// A row's exponentials are taken against the maximum of the first tile it saw, which is raised only when the exponentials of
-// a later tile add up to more than 2^64: P, the sums and O stay inside the range of bf16 and fp32 (2^127), and their
-// precision is relative, so a stale reference costs no accuracy - and no tile's maximum is needed.  P goes to tensor memory, over
+// A row's exponentials are taken against a reference 2^40 above the maximum of the first tile it saw, which is raised only when the
+// 64 exponentials of a later tile's thread add up to 2^-24, 2^16 times that maximum: over the 2^30 tokens a call may have, a row's
+// exponentials add up to 1 at most, so that O is finite for all finite values (see attend.cuh; with the reference at the maximum and
+// a slack of 2^64, values of 2^70 gave infinities).  Precision is relative: a stale reference costs no accuracy, and no tile's
+// maximum is needed; weights below 2^-86 of the reference's maximum vanish.  P goes to tensor memory, over
 // the logits, only when it is known to be in range; the rare raise starts from the logits again and rescales what the row has
 // accumulated, in its own threads.
 #pragma once
@@ -31,7 +33,8 @@ namespace triattn {
 constexpr int kTreeTile = 128;
 template <int D, int NT>
 constexpr int kTreeStages = 2 * (128 / D);  // of K and of V: 64 KB each
-constexpr float kTreeSlack = 18446744073709551616.f;  // 2^64: what a thread's exponentials of a tile may add up to
+constexpr float kTreeHeadroom = 40.f;             // base 2: the reference above a row's maximum
+constexpr float kTreeSlack = 1.f / (1 << 24);     // what a thread's 64 exponentials of a tile may add up to
 
 template <int NT>
 constexpr int kTreeThreads = NT * 256 + 96;  // softmax groups, MMA warp, K and V producers
@@ -367,7 +370,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
               pair_val[n & 1][g][half][row] = mx;
               row_over[n & 1][g][half][row] = over;
               pair_sync();
-              mx = over || row_over[n & 1][g][half ^ 1][row] ? fmaxf(m, fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]) * p.scale_log2) : m;
+              mx = over || row_over[n & 1][g][half ^ 1][row] ? fmaxf(m, fmaf(fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]), p.scale_log2, kTreeHeadroom)) : m;
               const float f = mx > m ? ex2(m - mx) : 1.f;
               l *= f;
               m = mx;
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
             }
             la = fadd2(la, lb);
             sum = la.x + la.y;
-            if (raise) break;  // nothing exceeds 1
+            if (raise) break;  // nothing exceeds 2^-40
             over = !(sum < kTreeSlack) || m == -INFINITY;
             const bool any = __any_sync(0xffffffffu, over);
             if (lane == 0) pair_over[n & 1][g][half][wid & 3] = any;
