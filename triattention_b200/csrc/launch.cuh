@@ -5,6 +5,7 @@
 
 #include <atomic>
 #include <cstdint>
+#include <mutex>
 #include <utility>
 
 #include "../../include/triattn_b200.h"
@@ -35,16 +36,21 @@ int launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cu
 }
 
 // Opt a kernel in to `smem` bytes of dynamic shared memory; the attribute call is made only when a device has
-// not yet been raised to that size for this kernel.
+// not yet been raised to that size for this kernel.  Some kernels are sized by the call (the width of a block table), so two threads may ask
+// for different sizes at once: calls that raise are made one at a time, and the attribute is never lowered.
 constexpr int kMaxDevicesSmem = 64;
 template <auto Kern>
 bool ensure_dynamic_smem(size_t smem) {
   static std::atomic<size_t> raised[kMaxDevicesSmem];
+  static std::mutex raising;
   int dev = -1;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevicesSmem) return false;
+  if (raised[dev].load(std::memory_order_acquire) >= smem) return true;
+  std::lock_guard<std::mutex> lock(raising);
   if (raised[dev].load(std::memory_order_relaxed) >= smem) return true;
-  if (cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return false;
-  raised[dev].store(smem, std::memory_order_relaxed);
+  if (cudaFuncSetAttribute(reinterpret_cast<const void*>(Kern), cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return false;
+  raised[dev].store(smem, std::memory_order_release);
   return true;
 }
 
