@@ -49,3 +49,48 @@ def test_infinite_drafts_in_consecutive_segments(D, g, big, small):
         assert torch.isnan(out[last][:, :, D // 2].float()).all()
         rest = [d for d in range(D) if d not in (3, D // 2, D - 2)]
         assert torch.equal(out[last][:, :, rest], want[last][:, :, rest])
+
+
+@pytest.mark.parametrize("B,H,g,n,D", [(40, 3, 2, 1, 64), (700, 1, 2, 1, 64), (400, 1, 2, 5, 64), (3, 40, 2, 1, 128), (2, 160, 2, 2, 64),
+                                       (33, 2, 2, 9, 128), (45, 2, 4, 20, 64), (600, 1, 4, 40, 64), (300, 1, 2, 12, 256), (2, 150, 4, 6, 128)])
+def test_every_row_of_large_batches(B, H, g, n, D):
+    """Batches that are planned in one pass or several, head counts around and above the number of SMs: every row that a request
+    owns is written and right, request by request, and the rows of nobody keep what they held.  out and lse start as NaN,
+    so that a row that is not written, or joined from parts that are not there, cannot pass."""
+    from triattention_b200 import ops
+    gen = torch.Generator().manual_seed(2200 + B + H)
+    lens = torch.randint(n, 60, (B,), generator=gen).tolist() if n < 60 else [n] * B
+    lens[B // 2] = 500
+    counts = [0 if b % 7 == 3 else int(torch.randint(1, n + 1, (1,), generator=gen)) for b in range(B)]
+    bt = Batch(lens, counts, H, g, D, 16, gen, tree=n > 1).dev()
+    N, extra = bt.start[-1], 5
+    q = torch.cat([bt.d_q, torch.full((extra, H * g, D), float("nan"), dtype=torch.bfloat16, device=DEV)])
+    words = None if bt.d_words is None else torch.cat([bt.d_words, torch.full((extra,), -1, dtype=torch.int64, device=DEV)])
+    out = torch.full((N + extra, H * g, D), float("nan"), dtype=torch.bfloat16, device=DEV)
+    lse = torch.full((N + extra, H * g), float("nan"), device=DEV)
+    status = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.attend_paged(q, bt.d_cache[0], bt.d_table, bt.d_lens, bt.d_start, n, tree_mask=words, kv_axis=0, out=out, lse=lse, status=status)
+    assert int(status) == 0
+    out, lse = out.cpu(), lse.cpu()
+    assert torch.isnan(out[N:].float()).all() and torch.isnan(lse[N:]).all()
+    assert torch.isfinite(out[:N].float()).all() and torch.isfinite(lse[:N]).all()
+    split_p = n * g <= 8
+    for b in range(B):
+        c, T = counts[b], lens[b]
+        if c == 0:
+            continue
+        k, v = (x.double() for x in bt.tokens(b))
+        see = oa.visible(T, c, None if bt.words is None else bt.words[bt.rows(b)])
+        r = bt.q[bt.rows(b)].double().view(c, H, g, D)
+        s = torch.einsum("nhgd,thd->nhgt", r, k) / D ** 0.5
+        L = (torch.einsum("nhgd,thd->nhgt", r.abs(), k.abs()) / D ** 0.5).amax(-1)
+        s = s.masked_fill(~see[:, None, None, :], float("-inf"))
+        p = torch.softmax(s, -1)
+        o, a = (torch.einsum("nhgt,thd->nhgd", p, x) for x in (v, v.abs()))
+        ds = (D + 4) * 2.0 ** -23 * L
+        z = torch.logsumexp(s, -1)
+        lse_tol = ds + 2.0 ** -21 + T * 2.0 ** -24 + 2.0 ** -22 * z.abs()
+        assert ((lse[bt.rows(b)].double().view(c, H, g) - z).abs() <= lse_tol).all(), b
+        p_rel = 2 * ds + 2.0 ** -21 + T * 2.0 ** -24
+        tol = 2.0 ** -8 * o.abs() + (p_rel[..., None] + (2.0 ** -16 if split_p else 2.0 ** -8)) * a + 1e-30
+        assert ((out[bt.rows(b)].double().view(c, H, g, D) - o).abs() <= tol).all(), b
