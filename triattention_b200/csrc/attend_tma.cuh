@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
     attend_decode_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,
                          const __grid_constant__ CUtensorMap vmap, const int runs) {
   constexpr int TILE = kDecodeTile<D>, STAGES = kDecodeStages<D>, WARPS = kDecodeWarps;
+  static_assert(D / 8 <= 32, "a lane per 16-byte piece of a row");
   static_assert(STAGES % WARPS == 0, "a stage belongs to one warp: its barriers are never more than a phase ahead");
   constexpr int ROWS = SPLIT_P ? 8 : 16;
   constexpr uint32_t kTileBytes = TILE * D * 2;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
   if (wid >= WARPS) {
     attend_produce<D, TILE, STAGES>(p, wid == WARPS ? &kmap : &vmap, wid - WARPS, c, count, ROWS,
                                     base + (wid - WARPS) * kTileBytes, 2 * kTileBytes, ring.full[0], ring.empty[0], ring,
-                                    (wid == WARPS && p.sums != nullptr) || p.max_q * p.g > ROWS);
+                                    wid == WARPS && p.sums != nullptr);
     return;
   }
 
@@ -379,8 +380,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
             if (odd) *v = zero_nonfinite(*v);
           }
         }
-        // (D = 256: the other lanes' share of a row)
-        if constexpr (D / 8 > 32) static_assert(D <= 256, "one lane per 16-byte piece");
         __syncwarp();
       }
       // ---- P, and O += P V

@@ -54,16 +54,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[32]) {
       : "r"(addr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
@@ -156,7 +146,6 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
   }
   grid_dependency_wait();
   trigger_dependents();
-  unsigned err = 0u;
   const int run = (int)blockIdx.x / p.Hkv;
   AttendCursor c;
   int count;
@@ -479,6 +468,7 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
           tmem_ld32(t_o + q * 32, ov);
           tmem_ld_wait32(ov);
           if (odd && there) {
+            unsigned err = 0u;  // (the producers have reported it)
             const int lo = t_begin * TILE, hi = min((t_begin + piece) * TILE, c.r.vlen);
             for (int vp = p.block_list == nullptr ? max(lo, ctx) : lo; vp < hi; ++vp) {
               const TokenAt at = attend_token(p, c, vp, err);
