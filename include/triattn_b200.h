@@ -345,12 +345,14 @@ int triattn_compress_paged(const triattn_paged_layout* layout /* host */, void* 
  * if bit j of tree_mask[query_start_loc[b] + i] is set; tree_mask NULL means a chain (bits 0..i).
  *   out[n, hq, :] = softmax(scale * q . k) v in bf16 (statistics and sums in fp32);  lse[n, hq]: natural log of the
  *   sum of exponentials, fp32.  A row that sees nothing gives zeros and -inf.  Rows of q that no request owns are left as
- *   they are in out and lse.
+ *   they are in out and lse.  Values up to 2^127 give finite outputs; weights below 2^-86 of a row's
+ *   largest may vanish.  Probabilities enter the product with V as two bf16 parts where max_query_len * group_size <= 8,
+ *   as one above.
  * block_list (may be NULL) [num_reqs, num_kv_heads, num_listed]: distinct logical block indices each KV head reads (in
  * any order, negative entries are unused); the first min(num_listed, blocks of the request) entries count.
  * weight_sums (may be NULL) [num_blocks, num_kv_heads, block_size] fp32: every token read receives the sum over the
  * query rows of its KV head of exp(s - lse); older tokens add it to what is there (or start anew with
- * reset_weight_sums), the query's own tokens always start anew.  With weight_sums the requests of a call share no cache blocks
+ * reset_weight_sums, for all requests of the call), the query's own tokens always start anew.  With weight_sums the requests of a call share no cache blocks
  * (a shared block's sums would be updated by several of them at once); without, they may.
  * layout: num_reqs, group_size (query heads per KV head), the cache geometry; head_dim 64, 128 or 256; any block size and
  * strides that are multiples of 8 elements.  k_cache / v_cache: the layer's base pointers (device memory, 16-byte

@@ -1,4 +1,4 @@
-"""Recipes that INTEGRATION.md spells out in code, run as they stand there."""
+"""Recipes that the integration guide spells out in code, run as they stand there."""
 from __future__ import annotations
 
 import re

@@ -25,7 +25,8 @@ __device__ __forceinline__ void tma_load_tokens(uint32_t dst, const CUtensorMap*
 }
 
 // What the call does not read again leaves the L2 first, so that parts, sums and keys that it does read again stay: a tree of 26
-// on 4 x 6600 tokens 60 -> 56 us, the end of a prompt with weight sums (K read twice) 71 -> 68, decode of 64 x 2112 tokens 99 -> 96.
+// on 4 x 6600 tokens 60 -> 56 us on the device, the end of a prompt with weight sums (K read twice) 71 -> 65, decode of 64 x 2112 tokens
+// 100 -> 97, a tree of 64 on 8 x 32768 tokens 303 -> 300.
 __device__ __forceinline__ uint64_t l2_policy(bool read_again) {
   uint64_t once, keep;
   asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
@@ -195,6 +196,10 @@ constexpr size_t decode_smem_bytes() {
 // warps overlap without any barrier, and the warps meet only where a segment (or the CTA's run) ends.  mma.sync, not
 // tcgen05: with at most 16 live rows a tile's products take a fifth of the time its bytes need.  Bound by HBM: 64 requests of 2112
 // tokens, 8 KV heads, head dimension 128, in 96 us, 5.8 TB/s (88 % of the measured copy).
+// SPLIT_P (at most 8 rows): P goes into the product with V as bf16 and bf16 remainder, the remainders in the operand's rows that would be
+// padding.  With 9 to 16 rows there is no padding left and P is one bf16: the output's error against 64 bits is then 2.3e-3 instead of 1.7e-3
+// (its own rounding), inside the 2^-8 that a bf16 output allows; remainders would take every product with V twice.  16 rows: 124 us on
+// the same tokens.
 template <int D, bool SPLIT_P>
 __global__ void __launch_bounds__(kDecodeThreads, 1)
     attend_decode_kernel(const __grid_constant__ AttendParams p, const __grid_constant__ CUtensorMap kmap,

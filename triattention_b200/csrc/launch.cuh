@@ -18,8 +18,9 @@ inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline int check_launch() { return cudaGetLastError() == cudaSuccess ? TRIATTN_OK : TRIATTN_ERR_CUDA; }
 
 // Kernel launch, optionally as a programmatic dependent of the preceding kernel in the stream: the launch is
-// processed and its CTAs become resident while that kernel drains (every kernel of this library starts with
-// griddepcontrol.wait, so nothing is read or written before the predecessor has completed).
+// processed and its CTAs become resident while that kernel drains (every kernel of this library executes griddepcontrol.wait before it
+// writes anything or reads what its predecessor writes.  All but one start with it; attend_combine_kernel reads lengths and
+// offsets before, which is sound because the attention kernel releases it only after its own wait).
 template <typename... KArgs, typename... Args>
 int launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, bool pdl, Args&&... args) {
   cudaLaunchConfig_t cfg = {};

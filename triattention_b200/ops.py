@@ -490,16 +490,22 @@ def attend_paged(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Ten
 
     ``q`` ``[N, Hq, D]`` bf16, request ``b`` owning rows ``query_start_loc[b] .. query_start_loc[b + 1] - 1`` (at most
     ``max_query_len`` <= 64); the keys and values of these tokens are already in the cache, in the last slots of the
-    request's ``seq_lens[b]`` tokens.  ``kv_cache`` is the layer's 5-D tensor (see :func:`split_kv_axes`), ``block_table``
+    request's ``seq_lens[b]`` tokens.  ``max_query_len`` times the group size chooses the kernel: up to 8 rows the
+    probabilities enter the product with V in two bf16 parts, above in one, and above 16 a row tile is 128 rows; pass the
+    step's own maximum, not the largest there may be.  ``kv_cache`` is the layer's 5-D tensor (see :func:`split_kv_axes`), ``block_table``
     ``[B, width]`` int32.  Every query token sees all earlier tokens; among the request's own tokens it sees token ``j`` if
     bit ``j`` of its ``tree_mask`` word (``[N]`` int64) is set, without a mask the tokens up to itself.
 
-    ``block_list`` ``[B, Hkv, S]`` int32 (:func:`select_blocks`) restricts each KV head to the listed blocks.
+    ``block_list`` ``[B, Hkv, S]`` int32 (:func:`select_blocks`) restricts each KV head to the listed blocks: distinct logical
+    indices in any order, negative ones unused, of which the first ``min(S, blocks of the request)`` count.
     ``weight_sums`` ``[num_blocks, Hkv, block_size]`` fp32 receives, per cached token and KV head, the attention weight the
-    token got from this call's rows: added to what older tokens have (``reset_weight_sums``: starting anew), while the
+    token got from this call's rows: added to what older tokens have (``reset_weight_sums``: starting anew, for all requests of the
+    call - one whose blocks had another owner and others that go on take calls of their own), while the
     request's own tokens always start anew, whatever their slots held (the requests of such a call share no cache
     blocks).  ``out`` ``[N, Hq, D]`` bf16, ``lse`` ``[N, Hq]`` fp32
-    (natural log); rows that no request owns are left as they are.  ``workspace``: at least
+    (natural log); rows that no request owns are left as they are, and so are the rows of a request with bad lengths, which is
+    skipped: in an ``out`` and ``lse`` that this call allocates they hold anything.  ``status`` (int32) collects what
+    was skipped, as ``DEV_*`` bits; without it nobody learns of it.  ``workspace``: at least
     :func:`attend_workspace_bytes` bytes that no overlapping call uses.
     """
     lib = _native.load()
