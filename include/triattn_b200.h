@@ -345,9 +345,9 @@ int triattn_compress_paged(const triattn_paged_layout* layout /* host */, void* 
  * if bit j of tree_mask[query_start_loc[b] + i] is set; tree_mask NULL means a chain (bits 0..i).
  *   out[n, hq, :] = softmax(scale * q . k) v in bf16 (statistics and sums in fp32);  lse[n, hq]: natural log of the
  *   sum of exponentials, fp32.  A row that sees nothing gives zeros and -inf.  Rows of q that no request owns are left as
- *   they are in out and lse.  Values up to 2^127 give finite outputs; weights below 2^-86 of a row's
- *   largest may vanish.  Probabilities enter the product with V as two bf16 parts where max_query_len * group_size <= 8,
- *   as one above.
+ *   they are in out and lse.  Values up to 2^127 give finite outputs; of 2^n tokens (n at least 7), weights
+ *   below 2^(n - 84) of a row's largest may vanish (2^(n - 126) up to 16 rows per KV head).  Probabilities enter the product with V
+ *   as two bf16 parts where max_query_len * group_size <= 8, as one above.
  * block_list (may be NULL) [num_reqs, num_kv_heads, num_listed]: distinct logical block indices each KV head reads (in
  * any order, negative entries are unused); the first min(num_listed, blocks of the request) entries count.
  * weight_sums (may be NULL) [num_blocks, num_kv_heads, block_size] fp32: every token read receives the sum over the

@@ -5,11 +5,11 @@
 //
 // over the tokens a row sees: every token before the request's query tokens, and of these (their keys are the last
 // slots of the sequence) the ones whose bit is set in the row's 64-bit word.  The softmax runs in one pass with a
-// running maximum and sum in fp32, in the base-2 domain.  Exponentials are taken against a reference kHeadroom above the maximum:
-// a row's exponentials then add up to at most 1 over the 2^30 tokens a call may have, and the unnormalised o is finite for
-// all finite values (against the maximum itself, 700 values of 2^126 and equal weights gave infinities).  What that costs lies at the
-// other end: weights below 2^-96 of the largest vanish, and outputs below 2^-96 lose bits of fp32.  The larger exponents
-// round to 2^-20, an eighth of the two bf16 parts' step and less.
+// running maximum and sum in fp32, in the base-2 domain.  Exponentials are taken against a reference that lies the base-2
+// logarithm of the segment's tokens (rounded up) above the maximum: a row's exponentials then add up to at most 1, and the
+// unnormalised o is finite for all finite values (against the maximum itself, 700 values of 2^126 and equal weights gave infinities).
+// What that costs lies at the other end: of 2^n tokens, weights below 2^(n - 126) of the largest vanish, and outputs below
+// that size lose bits of fp32.
 //
 // Bound: K and V are read once, 4 D bytes per (KV head, token), for 4 D R operations with R rows; up to about 32 rows the cache
 // stream is the limit, so what counts is that all SMs stream all the time.  The work of a KV head - the sequence of
@@ -28,7 +28,6 @@ namespace triattn {
 constexpr int kAttendMaxQuery = 64;  // query tokens per request: bits of a mask word
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kHeadroom = 30.f;  // base 2; 2^30: the tokens a call may have at most (validate_attend)
 
 struct AttendParams {
   const uint16_t* q;  // [N, Hq, D] bf16
@@ -81,6 +80,9 @@ __device__ __forceinline__ AttendReq attend_req(const AttendParams& p, int b, in
   r.row_tiles = (r.n * p.g + rows_per_tile - 1) / rows_per_tile;
   return r;
 }
+
+// ceil(log2(n)) of n >= 1
+__device__ __forceinline__ int ceil_log2(int n) { return 32 - __clz(n - 1); }
 
 // sum of `v` over the CTA; `red` holds one value per warp
 template <int THREADS>
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_paged_kernel(const __gr
     for (int x = 0; x < 2; ++x) {
       mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
       mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-      const float mn = fmaxf(m[x], fmaf(mx[x], p.scale_log2, kHeadroom));
+      const float mn = fmaxf(m[x], fmaf(mx[x], p.scale_log2, (float)ceil_log2(c.r.vlen)));
       grew = grew || mn > m[x];
       base[x] = mn == -INFINITY ? 0.f : mn;
       mx[x] = mn;

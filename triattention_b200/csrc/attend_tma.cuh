@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1)
       for (int x = 0; x < (SPLIT_P ? 1 : 2); ++x) {
         mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
         mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-        const float mn = fmaxf(m[x], fmaf(mx[x], p.scale_log2, kHeadroom));
+        const float mn = fmaxf(m[x], fmaf(mx[x], p.scale_log2, (float)ceil_log2(c.r.vlen)));
         grew = grew || mn > m[x];
         mbase[x] = mn == -INFINITY ? 0.f : mn;
         mx[x] = mn;

@@ -18,11 +18,15 @@
 // Measured: 256 rows over 8 x 32768 tokens, 8 KV heads, in 294 us (825 TFLOP/s in bursts, 680 under the power cap), where the bytes take 165;
 // what bounds it is the alternation of the two groups: per tile and group 1500 cycles for its products and 2000 for its softmax, the
 // tensor cores' own time for both groups being 2050.
-// A row's exponentials are taken against a reference 2^40 above the maximum of the first tile it saw, which is raised only when the
-// 64 exponentials of a later tile's thread add up to 2^-24, 2^16 times that maximum: over the 2^30 tokens a call may have, a row's
-// exponentials add up to 1 at most, so that O is finite for all finite values (see attend.cuh; with the reference at the maximum and
-// a slack of 2^64, values of 2^70 gave infinities).  Precision is relative: a stale reference costs no accuracy, and no tile's
-// maximum is needed; weights below 2^-86 of the reference's maximum vanish.  P goes to tensor memory, over
+// A row's exponentials are taken against a reference above the maximum of the first tile it saw, which is raised only when the
+// 64 exponentials of a later tile's thread add up to 2^8 of that maximum.  The reference lies so far above it that even then the
+// exponentials of all tiles add up to 1 at most, and O is finite for all finite values (see attend.cuh; with the reference at the
+// maximum and a slack of 2^64, values of 2^70 gave infinities).  Where the logits spread, later tiles exceed the first by more (of
+// normal ones by 1.6 standard deviations in 32768): the reference is set ahead by twice the distance between the maxima of a thread's
+// quarters (1.1 standard deviations), 2^40 at most.  Without that, 256 rows of logits with a standard deviation of 6 (12) on
+// 8 x 32768 tokens raised in most tiles: 427 (431) us where those of deviation 1 take 297; with it 303 (319).  Precision is relative: a stale reference costs no
+// accuracy, and no tile's maximum is needed; of 2^n tokens (n at least 7), weights below 2^(n - 124), of a row whose logits spread
+// 2^(n - 84), of the first tile's largest vanish.  P goes to tensor memory, over
 // the logits, only when it is known to be in range; the rare raise starts from the logits again and rescales what the row has
 // accumulated, in its own threads.
 #pragma once
@@ -35,8 +39,8 @@ namespace triattn {
 constexpr int kTreeTile = 128;
 template <int D, int NT>
 constexpr int kTreeStages = 2 * (128 / D);  // of K and of V: 64 KB each
-constexpr float kTreeHeadroom = 40.f;             // base 2: the reference above a row's maximum
-constexpr float kTreeSlack = 1.f / (1 << 24);     // what a thread's 64 exponentials of a tile may add up to
+constexpr int kTreeSlack = 8;  // base 2: what a thread's 64 exponentials of a tile may add up to, above the maximum of the reference
+constexpr float kTreeAhead = 40.f;  // base 2: what a reference is set ahead at most, for logits that spread
 
 template <int NT>
 constexpr int kTreeThreads = NT * 256 + 96;  // softmax groups, MMA warp, K and V producers
@@ -284,6 +288,8 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
       const bool there = r < R;
       const unsigned long long word = there ? attend_word(p, c.r, r / p.g) : 0ull;
       const bool idle = c.rt * ROWS + g * 128 + (wid & 3) * 32 >= R;  // none of the warp's rows exists
+      // 2^-share: what a thread's exponentials of a tile may add up to, a row's over its 2 x tiles of them to 1
+      const int share = ceil_log2(2 * c.r.tiles);
       float m = -INFINITY, l = 0.f;
       for (int x = 0; x < piece; ++x) {
         const int n = it + x, s = n % STAGES;
@@ -358,10 +364,12 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
                 for (int j = 0; j < 32; ++j) m4[j & 3] = fmaxf(m4[j & 3], __uint_as_float(sv[j]));
               }
               float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+              const float low = fminf(fminf(m4[0], m4[1]), fminf(m4[2], m4[3]));
+              mx = fmaf(mx, p.scale_log2, fminf(2.f * p.scale_log2 * (mx - low), kTreeAhead));  // (no logit at all: -inf)
               pair_val[n & 1][g][half][row] = mx;
               row_over[n & 1][g][half][row] = over;
               pair_sync();
-              mx = over || row_over[n & 1][g][half ^ 1][row] ? fmaxf(m, fmaf(fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]), p.scale_log2, kTreeHeadroom)) : m;
+              mx = over || row_over[n & 1][g][half ^ 1][row] ? fmaxf(m, fmaxf(mx, pair_val[n & 1][g][half ^ 1][row]) + (float)(share + kTreeSlack)) : m;
               const float f = mx > m ? ex2(m - mx) : 1.f;
               l *= f;
               m = mx;
@@ -399,8 +407,8 @@ __global__ void __launch_bounds__(kTreeThreads<NT>, 1)
             }
             la = fadd2(la, lb);
             sum = la.x + la.y;
-            if (raise) break;  // nothing exceeds 2^-40
-            over = !(sum < kTreeSlack) || m == -INFINITY;
+            if (raise) break;  // nothing exceeds 2^-(share + kTreeSlack)
+            over = !(sum < __int_as_float((127 - share) << 23)) || m == -INFINITY;
             const bool any = __any_sync(0xffffffffu, over);
             if (lane == 0) pair_over[n & 1][g][half][wid & 3] = any;
             pair_sync();
